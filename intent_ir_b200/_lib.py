@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(HERE, "libintentir_b200.so")
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_BUFFER, ERR_DEVICE_WAIT = 0, -1, -2, -3, -4, -5
 F32, BF16, F16, I32, I64, BOOL, U8, I8, I16, F64 = range(10)
+E4M3 = 10  # held values of the serving entries
 REDUCE_SUM, REDUCE_MAX, REDUCE_ANY = 0, 1, 2
 ACT_NONE, ACT_RELU = 0, 1
 GEMM_ALLOW_TF32 = 1
@@ -69,6 +70,14 @@ SIGNATURES = {
     "ib200_gemm_scratch_bytes": (_sz, [_i, _i, _i64, _i64, _i64, _i, _i]),
     "ib200_check_status": (_i, [_vp, _vp]),
     "ib200_transpose2d": (_i, [_vp, _vp, _i, _i64, _i64, _vp]),
+    "ib200_rmsnorm": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _i64, _i64, _i64, _f, _vp]),
+    "ib200_w4_matmul": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i64, _vp, _sz, _vp, _vp]),
+    "ib200_w4_scratch_bytes": (_sz, [_i, _i64, _i64, _i64, _i64]),
+    "ib200_kv8_append": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _i64,
+                              _i64, _i64, _vp]),
+    "ib200_attention_kv8": (_i, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64,
+                                 _i64, _i64, _i64, _f, _vp, _sz, _vp]),
+    "ib200_attention_kv8_scratch_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
 }
 
 _lib: Optional[C.CDLL] = None

@@ -100,6 +100,14 @@ int launch_warp(const int8_t* src, const int16_t* offset, int8_t* out, int64_t c
 int launch_dropout(const float* x, float* y, int64_t n, const void* p_ptr, int p_dtype, float p_value, const void* seed_ptr, int seed_dtype,
                    long long seed_value, int rounds, cudaStream_t s);
 
+// the serving step (rmsnorm.cu, w4.cu; the cache's entries are in kv8.h)
+int launch_rmsnorm(const void* x, int64_t x_stride, const void* res, int64_t res_stride, const void* w, void* y, void* h, int64_t h_stride,
+                   float* scale, int dtype, int w_dtype, int out_dtype, int64_t rows, int64_t cols, int64_t group, float eps, cudaStream_t s);
+int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_groups, const void* q, const void* scales, const void* zeros,
+              const void* bias, void* y, int x_dtype, int s_dtype, int out_dtype, int64_t m, int64_t n, int64_t k, int64_t group,
+              void* scratch, size_t scratch_bytes, int32_t* status, cudaStream_t s);
+size_t w4_scratch_bytes(int x_dtype, int64_t m, int64_t n, int64_t k, int64_t group);
+
 #ifdef __CUDACC__
 // ---- element conversion ---------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return static_cast<float>(v); }

@@ -247,3 +247,223 @@ def transpose2d(x: torch.Tensor) -> torch.Tensor:
     rc = _lib.load().ib200_transpose2d(_ptr(x), _ptr(out), x.element_size(), x.shape[0], x.shape[1], _stream())
     _check(rc, "transpose2d")
     return out
+
+
+# ---- a decoder layer's serving step: activations, weights and the key / value cache in 8 or 4 bits ------------
+
+_FLOAT_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_HALF_CODE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_HELD_CODE = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.I8}
+
+
+def _on_device(dev: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is not None and (not isinstance(t, torch.Tensor) or t.device != dev):
+            raise B200RuntimeError(f"{name} must be a tensor on {dev}")
+
+
+def _dense(name: str, t: torch.Tensor, shape: Sequence[int], dtype: torch.dtype) -> None:
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise B200RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+
+
+def _rows(name: str, t: torch.Tensor) -> Tuple[int, int, int]:
+    """rows, columns and the row stride of a contiguous tensor, or of a matrix of evenly spaced contiguous rows."""
+    if t.dim() == 0:
+        raise B200RuntimeError(f"{name} must have at least one axis")
+    cols = t.shape[-1]
+    if t.is_contiguous():
+        return t.shape[:-1].numel(), cols, cols
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
+        return t.shape[0], cols, t.stride(0)
+    raise B200RuntimeError(f"{name} must be contiguous, or a matrix of evenly spaced contiguous rows")
+
+
+def _code(name: str, t: torch.Tensor, codes: Dict[torch.dtype, int]) -> int:
+    try:
+        return codes[t.dtype]
+    except KeyError:
+        raise B200LoweringError(f"{name}: unsupported dtype {t.dtype}") from None
+
+
+def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+            out_dtype: Optional[torch.dtype] = None, group: int = 0, residual_out: Optional[torch.Tensor] = None):
+    """``h = x + residual`` and ``y = h / sqrt(mean(h * h) + eps) * w`` over the last axis, in f32 from the unrounded sum; returns
+    ``(y, scale, h)``.  ``h`` has the type of ``x`` and is None without a residual; ``residual_out`` says where it goes (it may be
+    ``residual`` or ``x`` itself).  ``out_dtype`` float8_e4m3fn or int8 holds y in 8 bits, ``y * scale`` standing for the result,
+    with one f32 scale for each row (``group`` 0) or for each 32, 64, 128 or 256 columns; otherwise y has the type of x and
+    scale is None.  x is f32, bf16 or f16; w has its type or f32; x, residual and residual_out may be matrices of spaced rows."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise B200RuntimeError("x must be a CUDA tensor")
+    dev = x.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return rmsnorm(x, w, residual, eps, out_dtype, group, residual_out)
+    _on_device(dev, w=w, residual=residual, residual_out=residual_out)
+    rows, cols, xs = _rows("x", x)
+    code = _code("x", x, _FLOAT_CODE)
+    w_code = code
+    if w is not None:
+        w_code = _code("w", w, _FLOAT_CODE)
+        if w.numel() != cols or not w.is_contiguous():
+            raise B200RuntimeError(f"w must be contiguous with one element per column ({cols})")
+    rs = hs = 0
+    h = residual_out
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise B200RuntimeError("residual must have the shape and dtype of x")
+        rs = _rows("residual", residual)[2]
+        if h is None:
+            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        elif h.shape != x.shape or h.dtype != x.dtype:
+            raise B200RuntimeError("residual_out must have the shape and dtype of x")
+        hs = _rows("residual_out", h)[2]
+    elif h is not None:
+        raise B200RuntimeError("residual_out needs a residual")
+    out_dtype = out_dtype or x.dtype
+    held = _HELD_CODE.get(out_dtype)
+    if held is None and out_dtype != x.dtype:
+        raise B200LoweringError(f"rmsnorm: the result is {x.dtype}, float8_e4m3fn or int8, not {out_dtype}")
+    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    scale = None
+    if held is not None:
+        scale = torch.empty(x.shape[:-1] + ((cols + group - 1) // group if group > 0 else 1,), dtype=torch.float32, device=dev)
+    rc = _lib.load().ib200_rmsnorm(_ptr(x), xs, _ptr(residual), rs, _ptr(w), _ptr(y), _ptr(h), hs, _ptr(scale), code, w_code,
+                                   code if held is None else held, rows, cols, group, float(eps), _stream())
+    _check(rc, "rmsnorm")
+    return y, scale, h
+
+
+def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+              bias: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None, group: int = 128,
+              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x @ w.T + bias`` for weights of 4 bits, ``w[n, k] = scales[n, k // group] * (q[n, k] - zeros[n, k // group])``, with f32 sums.
+    ``q`` is uint8 [N, K/2] with the even k of a byte in its low half, ``scales`` [N, ceil(K / group)] f32 / bf16 / f16, ``zeros``
+    uint8 of that shape (default 8).  ``x`` [.., K] is bf16 or f16, or float8_e4m3fn / int8 with ``x_scale`` f32 [.., 1] or
+    [.., ceil(K / group)], as ``rmsnorm`` returns them.  ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.
+    K is a multiple of 32, the group 32, 64 or 128."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise B200RuntimeError("x must be a CUDA tensor")
+    dev = x.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return w4_matmul(x, q, scales, zeros, bias, x_scale, group, out_dtype)
+    _on_device(dev, q=q, scales=scales, zeros=zeros, bias=bias, x_scale=x_scale)
+    if q is None or scales is None or q.dim() != 2 or group not in (32, 64, 128):
+        raise B200LoweringError("w4_matmul: q is a matrix, the group 32, 64 or 128")
+    m, k, xs = _rows("x", x)
+    n = q.shape[0]
+    if k % 32:
+        raise B200LoweringError(f"w4_matmul: K = {k} is not a multiple of 32")
+    groups = (k + group - 1) // group
+    _dense("q", q, (n, k // 2), torch.uint8)
+    _dense("scales", scales, (n, groups), scales.dtype)
+    if zeros is not None:
+        _dense("zeros", zeros, (n, groups), torch.uint8)
+    x_code = _HELD_CODE.get(x.dtype)
+    x_groups = 0
+    if x_code is not None:
+        if x_scale is None or x_scale.shape[:-1] != x.shape[:-1] or x_scale.shape[-1] not in (1, groups):
+            raise B200RuntimeError(f"w4_matmul: 8-bit x needs x_scale of shape {tuple(x.shape[:-1])} + (1 or {groups},)")
+        _dense("x_scale", x_scale, x_scale.shape, torch.float32)
+        x_groups = x_scale.shape[-1]
+    else:
+        x_code = _code("x", x, _HALF_CODE)
+        if x_scale is not None:
+            raise B200RuntimeError("w4_matmul: x_scale belongs to 8-bit x")
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if x_groups else x.dtype
+    elif out_dtype not in _FLOAT_CODE:
+        raise B200LoweringError(f"w4_matmul: the result is float32, bfloat16 or float16, not {out_dtype}")
+    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    if bias is not None:
+        _dense("bias", bias, (n,), out_dtype)
+    lib = _lib.load()
+    need = lib.ib200_w4_scratch_bytes(x_code, m, n, k, group)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = lib.ib200_w4_matmul(_ptr(x), xs, _ptr(x_scale), x_groups, _ptr(q), _ptr(scales), _ptr(zeros), _ptr(bias), _ptr(y), x_code,
+                             _code("scales", scales, _FLOAT_CODE), _FLOAT_CODE[out_dtype], m, n, k, group, _ptr(scratch), need,
+                             status_word().data_ptr(), _stream())
+    _check(rc, "w4_matmul")
+    return y
+
+
+def _cache_extents(x: torch.Tensor, name: str, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new):
+    """Checks of the paged cache's arguments; the extents (pages, heads, block, dim, batch, table_blocks) and the held type's code."""
+    _on_device(x.device, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table, seq_lens=seq_lens, cu_new=cu_new)
+    if any(t is None for t in (k_cache, v_cache, k_scale, v_scale, block_table, seq_lens)):
+        raise B200RuntimeError("the caches, their scales, block_table and seq_lens are needed")
+    if k_cache.dim() != 4 or block_table.dim() != 2 or x.dim() != 3:
+        raise B200RuntimeError(f"{name} is [tokens, heads, dim], the caches [pages, heads, block, dim], block_table [sequences, blocks]")
+    held = _code("k_cache", k_cache, _HELD_CODE)
+    pages, heads, block, dim = k_cache.shape
+    batch, table_blocks = block_table.shape
+    _dense("k_cache", k_cache, k_cache.shape, k_cache.dtype)
+    _dense("v_cache", v_cache, k_cache.shape, k_cache.dtype)
+    _dense("k_scale", k_scale, (pages, heads), torch.float32)
+    _dense("v_scale", v_scale, (pages, heads), torch.float32)
+    _dense("block_table", block_table, (batch, table_blocks), torch.int32)
+    _dense("seq_lens", seq_lens, (batch,), torch.int32)
+    if cu_new is not None:
+        _dense("cu_new", cu_new, (batch + 1,), torch.int32)
+    if x.shape[2] != dim or (dim > 1 and x.stride(2) != 1):
+        raise B200RuntimeError(f"{name} must have the cache's width {dim} as its last, adjacent axis")
+    return held, pages, heads, block, dim, batch, table_blocks
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_new: Optional[torch.Tensor] = None) -> None:
+    """Writes new tokens' keys and values ``k``, ``v`` [tokens, heads, dim] (bf16 / f16, last axis adjacent) into the caches
+    [pages, heads, block, dim] (float8_e4m3fn or int8) with one f32 scale for each page and head, ``k_scale`` / ``v_scale``
+    [pages, heads].  ``block_table`` [sequences, blocks] int32 names the pages, ``seq_lens`` [sequences] int32 the lengths with the
+    new tokens, ``cu_new`` [sequences + 1] int32 where each sequence's new tokens lie (None: the same number for each).  A scale
+    grows with its block's largest value, and the values held before are rounded again; slots behind the end, tokens behind
+    ``cu_new[-1]``, and pages or tokens outside the cache and the table are left alone.  No two sequences may append to one page."""
+    if not isinstance(k, torch.Tensor) or not k.is_cuda:
+        raise B200RuntimeError("k must be a CUDA tensor")
+    dev = k.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
+    held, pages, heads, block, dim, batch, table_blocks = _cache_extents(k, "k", k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
+    _on_device(dev, v=v)
+    if v is None or v.shape != k.shape or v.dtype != k.dtype or k.shape[1] != heads or (dim > 1 and v.stride(2) != 1):
+        raise B200RuntimeError(f"k and v must be [tokens, {heads}, {dim}] tensors of one dtype with adjacent last axes")
+    rc = _lib.load().ib200_kv8_append(_ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(k_cache), _ptr(v_cache),
+                                      _ptr(k_scale), _ptr(v_scale), _ptr(block_table), _ptr(seq_lens), _ptr(cu_new),
+                                      _code("k", k, _HALF_CODE), held, k.shape[0], batch, heads, dim, pages, block, table_blocks, _stream())
+    _check(rc, "kv8_append")
+
+
+def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  block_table: torch.Tensor, seq_lens: torch.Tensor, cu_new: Optional[torch.Tensor] = None,
+                  scale: Optional[float] = None, window: int = 0, return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Attention of the new tokens' queries ``q`` [tokens, query heads, dim] over the cache that ``kv8_append`` has put their keys
+    and values into (same arguments): token i of a sequence's n new ones sees the keys up to its own place, seq_len - n + i, and
+    with ``window`` > 0 only the last that many of them.  ``scale`` defaults to 1 / sqrt(dim); consecutive query heads share a key
+    head.  Returns ``o`` of q's shape and dtype (``out``, if given), with ``return_lse`` also the f32 [tokens, query heads] logs of
+    the softmax's denominators.  Rows without keys are 0 (lse -inf); rows that need a page outside the cache or a token outside the
+    table are NaN; tokens behind ``cu_new[-1]`` are not written."""
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        raise B200RuntimeError("q must be a CUDA tensor")
+    dev = q.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new, scale, window, return_lse, out)
+    held, pages, heads, block, dim, batch, table_blocks = _cache_extents(q, "q", k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
+    tokens, q_heads = q.shape[0], q.shape[1]
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _on_device(dev, out=out)
+        _dense("out", out, q.shape, q.dtype)
+    lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=dev) if return_lse else None
+    lib = _lib.load()
+    need = lib.ib200_attention_kv8_scratch_bytes(tokens, batch, q_heads, heads, dim, block, table_blocks)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rc = lib.ib200_attention_kv8(_ptr(q), q.stride(0), q.stride(1), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+                                 _ptr(block_table), _ptr(seq_lens), _ptr(cu_new), _ptr(out), _ptr(lse), _code("q", q, _HALF_CODE), held,
+                                 tokens, batch, q_heads, heads, dim, pages, block, table_blocks, window,
+                                 dim ** -0.5 if scale is None else float(scale), _ptr(scratch), need, _stream())
+    _check(rc, "attention_kv8")
+    return (out, lse) if return_lse else out
