@@ -1,0 +1,642 @@
+// Attention of new tokens over the paged 8-bit cache (kv8.cu says what the cache is):
+//   o[t, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q . k_j - m),   k_j = k8 * ks(page, head),   v_j = v8 * vs(page, head)
+// in one pass over the keys with a running maximum m and sum, in f32.
+//
+// Work.  The queries that share a key head (new tokens x heads of a group) are rows, 8 * NT of them to a unit; a unit reads
+// its keys in tiles of 128.  All tiles of all units, in order, are cut into one equal range per CTA whatever the lengths are (each
+// CTA adds up the lengths itself), so a batch of mixed lengths fills the GPU evenly.  A unit that lies in one range is
+// finished there; the pieces of others go to scratch as (sum, maximum, unnormalised o), and a second launch joins them in order.
+//
+// Inside a CTA the four warps take 32 keys each of a tile, with copies of their own three stages deep (cp.async) and no
+// barrier between them until the unit ends.  Both products run on mma.sync with the keys as the 16 rows: S' = K Q' and
+// O' = V' P', so that 8 queries fill a fragment where queries as rows would need 16.  Bytes are widened to f16, which
+// is exact for both types; scales are applied to the scores and to p.  q is scaled by a power of two to below 2 (exact), p * vs
+// by another one to below 2^15, so that f16 holds them to 2^-12 over 2^39.
+#include "kv8.cuh"
+
+namespace ib200 {
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 32, kTile = kWarps * kStep, kStages = 3;
+template <int D> struct Cfg {
+  static constexpr int kStageBytes = 2 * kStep * D;  // keys, values
+  static constexpr int kSmem = kWarps * kStages * kStageBytes;
+  static constexpr int kCtas = D == 128 ? 2 : 4;  // per SM, by shared memory
+  static constexpr int kPitch = D + 4;            // floats between the rows of the joining buffer
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {  // zeros where nothing is taken
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// four bytes as two pairs of f16, exact
+template <int HELD> __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (HELD == HELD_E4M3) {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {  // the byte as 1024 + (i + 128), minus 1152
+    w ^= 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    uint32_t l = __byte_perm(w, 0x64646464u, 0x4140), h = __byte_perm(w, 0x64646464u, 0x4342);
+    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&l), off), b = __hsub2(*reinterpret_cast<__half2*>(&h), off);
+    lo = *reinterpret_cast<uint32_t*>(&a);
+    hi = *reinterpret_cast<uint32_t*>(&b);
+  }
+}
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Byte offset of 16-byte chunk c of token row r in a stage.  Eight lanes that read a quarter-warp's worth of chunks then touch all
+// banks once, for keys (two adjacent rows, four chunks) and for values (rows 0, 2, 4, 6, two chunks) alike.
+template <int D> __device__ __forceinline__ int at_chunk(int r, int c) {
+  if (D == 128) return r * 128 + ((c ^ ((r & 6) ^ ((r & 1) << 2))) << 4);
+  const int line = r >> 1;
+  return line * 128 + (((((r & 1) << 2) + c) ^ ((line & 3) << 1)) << 4);
+}
+
+struct Seq {  // what a sequence asks for
+  int first, n, len, keys, tile0, tiles, units_per_head;  // keys: those that the table has room for
+};
+__device__ __forceinline__ int first_key(const Kv8Attention& a, int64_t pos) {  // that the token at `pos` sees
+  return a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
+}
+__device__ __forceinline__ Seq seq_of(const Kv8Attention& a, int b, int rows) {
+  Seq s;
+  s.first = a.cu ? a.cu[b] : b * a.each;
+  s.n = a.cu ? a.cu[b + 1] - s.first : a.each;
+  s.len = a.lens[b];
+  const int64_t group = a.q_heads / a.heads;
+  if (s.n <= 0 || s.len <= 0 || s.first < 0 || (int64_t)s.first + s.n > a.tokens) s.n = 0, s.len = 0;  // nothing to do, or offsets that cannot be
+  s.keys = (int)min((int64_t)s.len, a.table_blocks * a.block);
+  s.tile0 = first_key(a, (int64_t)s.len - s.n) / kTile;
+  s.tiles = s.keys > 0 ? max(0, (s.keys - 1) / kTile + 1 - s.tile0) : 0;
+  s.units_per_head = (int)((s.n * group + rows - 1) / rows);
+  return s;
+}
+__device__ __forceinline__ int64_t work_of(const Kv8Attention& a, const Seq& s) { return (int64_t)a.heads * s.units_per_head * s.tiles; }
+
+// scratch: the work in front of every sequence and in all, then two partial results per CTA
+struct Scratch {
+  int64_t* before;  // [batch + 1]
+  float* part;      // [2 * CTAs][rows * (D + 2)]
+};
+__host__ __device__ inline size_t prefix_bytes(int64_t batch) { return ((size_t)(batch + 1) * 8 + 255) / 256 * 256; }
+__host__ __device__ inline Scratch carve(void* p, int64_t batch) {
+  return {static_cast<int64_t*>(p), reinterpret_cast<float*>(static_cast<char*>(p) + prefix_bytes(batch))};
+}
+
+template <typename V> __device__ __forceinline__ V scan_warp(V v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+template <typename T, int HELD, int D, int NT>
+__global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention a, const Scratch sc, const int q_vec) {
+  using C = Cfg<D>;
+  constexpr int ROWS = 8 * NT, HALVES = D / 64, MT = D / 16, CH = D / 16;  // CH: 16-byte chunks of a token
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int64_t sums[kWarps], found_before;
+  __shared__ int found;
+  __shared__ float stat[kWarps][ROWS][2], top_v[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int batch = (int)a.batch, group = (int)(a.q_heads / a.heads);
+
+  // ---- this CTA's range of tiles -------------------------------------------------------------------
+  int64_t mine = 0;
+  for (int b = threadIdx.x; b < batch; b += kThreads) mine += work_of(a, seq_of(a, b, ROWS));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) sums[warp] = mine;
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  const int64_t total = sums[0] + sums[1] + sums[2] + sums[3];
+  const int ctas = (int)min((int64_t)gridDim.x, total);  // with less work than CTAs, one tile to each
+  int64_t w = 0, w_end = 0;
+  if (blockIdx.x < ctas) {
+    w = total * blockIdx.x / ctas;
+    w_end = total * (blockIdx.x + 1) / ctas;
+  }
+  int64_t before = 0;
+  for (int base = 0; base < batch; base += kThreads) {
+    __syncthreads();
+    const int b = base + threadIdx.x;
+    const int64_t v = b < batch ? work_of(a, seq_of(a, b, ROWS)) : 0;
+    const int64_t upto = scan_warp(v, lane);
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int64_t front = before;
+    for (int i = 0; i < warp; ++i) front += sums[i];
+    front += upto - v;  // the work in front of sequence b
+    before += sums[0] + sums[1] + sums[2] + sums[3];
+    if (blockIdx.x == 0 && b < batch) sc.before[b] = front;
+    if (v > 0 && front <= w && w < front + v) {
+      found = b;
+      found_before = front;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) sc.before[batch] = total;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining launch may line up: it waits for this one's end
+  __syncthreads();
+  if (w >= w_end) return;
+
+  uint8_t* stages = smem + warp * kStages * C::kStageBytes;
+  const uint32_t stages_at = (uint32_t)__cvta_generic_to_shared(stages);
+  int b = found;
+  int64_t front = found_before;
+  Seq s = seq_of(a, b, ROWS);
+  bool first_piece = true;
+
+  while (w < w_end) {
+    // ---- a piece: one unit's tiles [from, to) -------------------------------------------------------
+    const int64_t rel = w - front;
+    const int unit = (int)(rel / s.tiles), from = (int)(rel - (int64_t)unit * s.tiles), to = (int)min((int64_t)s.tiles, from + (w_end - w));
+    const int head = unit / s.units_per_head, r0 = (unit - head * s.units_per_head) * ROWS;
+    const int rows = (int)min((int64_t)ROWS, (int64_t)s.n * group - r0);
+    const int start = s.len - s.n;  // place of the first new token (negative: fewer tokens than new ones)
+    const int pos_min = start + r0 / group, pos_max = start + (r0 + rows - 1) / group;
+    const int lo_min = first_key(a, pos_min), lo_max = first_key(a, pos_max);
+    // this warp's steps: 32 keys from 128 * tile + 32 * warp, those with a key that any row sees
+    const int off = warp * kStep;
+    int j0 = s.tile0 + from, j1 = s.tile0 + to;  // tiles
+    if (lo_min > off + kStep - 1) j0 = max(j0, (lo_min - off - kStep + 1 + kTile - 1) / kTile);
+    j1 = pos_max < off ? j0 : min(j1, (pos_max - off) / kTile + 1);
+    const int steps = max(0, j1 - j0);
+
+    // queries as the k x 8 operand: chunk bytes 4w .. 4w + 3 of half h are the k slots (2t, 2t + 1, 2t + 8, 2t + 9) of product 4h + w
+    uint32_t qf[NT][HALVES * 4][2];
+    float mult[NT][2];
+    int hi[NT][2], low[NT][2];  // the keys that this thread's two columns (rows of the unit) see: low .. hi
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = r0 + nt * 8 + g;
+      const bool real = nt * 8 + g < rows;
+      const int i = real ? row / group : 0, jq = real ? row - i * group : 0;
+      const T* q = static_cast<const T*>(a.q) + (int64_t)(s.first + i) * a.q_token + (int64_t)(head * group + jq) * a.q_head;
+      float v[HALVES * 4][4], top = 0.0f;
+#pragma unroll
+      for (int k = 0; k < HALVES * 4; ++k) {
+        const int d = (k >> 2) * 64 + t * 16 + (k & 3) * 4;
+        if (!real) {
+          v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.0f;
+        } else if (q_vec) {
+          load4(q + d, v[k]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[k][e] = to_f32(q[d + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(v[k][e]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e for top in [2^e, 2^(e+1)); 1 for a row of zeros or with an infinity
+      const int e = (int)(__float_as_uint(top) >> 23);
+      const float down = top == 0.0f || e == 255 ? 1.0f : __uint_as_float((uint32_t)min(253, max(1, 254 - e)) << 23);
+#pragma unroll
+      for (int k = 0; k < HALVES * 4; ++k) {
+        qf[nt][k][0] = pack16(v[k][0] * down, v[k][1] * down);
+        qf[nt][k][1] = pack16(v[k][2] * down, v[k][3] * down);
+      }
+      const float m = a.scale * 1.4426950408889634f / down;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mult[nt][c] = __shfl_sync(0xffffffffu, m, (2 * t + c) * 4);
+        const int rr = nt * 8 + 2 * t + c;
+        hi[nt][c] = rr < rows ? start + (r0 + rr) / group : -1;
+        low[nt][c] = first_key(a, hi[nt][c]);
+      }
+    }
+
+    float o[NT][MT][4], m[NT][2], l[NT][2], vtop = 0x1p-100f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) m[nt][c] = -INFINITY, l[nt][c] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.0f;
+    }
+
+    // Pages and scales, 16 steps at a time: lane 2i + h looks up the 16 keys of half h of step i.  The next 16 are fetched while these are used.
+    struct Meta { int page, slot; float ks, vs; };  // page: page * heads + head, -1: outside the cache
+    auto look_up = [&](int step0) {
+      Meta x{-1, 0, NAN, NAN};
+      const int step = step0 + (lane >> 1);
+      const int64_t key = (int64_t)(j0 + step) * kTile + off + (lane & 1) * 16;
+      if (step < steps && key < s.keys) {
+        const int blk = (int)(key / a.block);
+        x.slot = (int)(key - (int64_t)blk * a.block);
+        const int page = a.table[(int64_t)b * a.table_blocks + blk];
+        if ((unsigned)page < (unsigned)a.pages) x.page = page * (int)a.heads + head;
+      }
+      return x;
+    };
+    auto look_scales = [&](Meta& x) {
+      if (x.page >= 0) {
+        x.ks = a.k_scale[x.page];
+        x.vs = a.v_scale[x.page];
+      }
+    };
+    auto issue = [&](int step, const Meta& meta) {
+      const uint32_t dst = stages_at + (step % kStages) * C::kStageBytes;
+      const int key0 = (j0 + step) * kTile + off;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int page = __shfl_sync(0xffffffffu, meta.page, 2 * (step & 15) + h), slot = __shfl_sync(0xffffffffu, meta.slot, 2 * (step & 15) + h);
+        const int64_t base = page < 0 ? 0 : ((int64_t)page * a.block + slot) * D;
+        const int left = page < 0 ? 0 : s.keys - (key0 + h * 16);  // keys of these 16 that exist; what lies behind the last one is never read
+#pragma unroll
+        for (int i = 0; i < 16 * CH / 32; ++i) {
+          const int idx = i * 32 + lane, r = idx / CH, c = idx % CH;
+          const bool take = r < left;
+          const int64_t src = take ? base + r * D + c * 16 : 0;
+          const uint32_t to_at = dst + at_chunk<D>(h * 16 + r, c);
+          copy16(to_at, a.k_cache + src, take);
+          copy16(to_at + kStep * D, a.v_cache + src, take);
+        }
+      }
+    };
+
+    Meta cur = look_up(0);
+    look_scales(cur);
+    Meta nxt = cur;
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (i < steps) issue(i, cur);
+      copy_commit();
+    }
+    for (int step = 0; step < steps; ++step) {
+      if ((step & 15) == 0) {
+        if (step) cur = nxt;
+        nxt = look_up(step + 16);
+      } else if ((step & 15) == 8) {
+        look_scales(nxt);
+      }
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      {
+        const int ahead = step + kStages - 1;
+        if (ahead < steps) {
+          if ((ahead >> 4) == (step >> 4)) issue(ahead, cur); else issue(ahead, nxt);
+        }
+        copy_commit();
+      }
+      const uint8_t* kst = stages + (step % kStages) * C::kStageBytes;
+      const uint8_t* vst = kst + kStep * D;
+      const int key0 = (j0 + step) * kTile + off;
+
+      // ---- S' = K Q' --------------------------------------------------------------------------------
+      float sv[2][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sv[mt][nt][0] = sv[mt][nt][1] = sv[mt][nt][2] = sv[mt][nt][3] = 0.0f;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const uint4 x = *reinterpret_cast<const uint4*>(kst + at_chunk<D>(mt * 16 + g, h * 4 + t));
+          const uint4 y = *reinterpret_cast<const uint4*>(kst + at_chunk<D>(mt * 16 + 8 + g, h * 4 + t));
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t a0, a1, a2, a3;
+            widen<HELD>(xs[k], a0, a2);
+            widen<HELD>(ys[k], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816(sv[mt][nt], a0, a1, a2, a3, qf[nt][h * 4 + k][0], qf[nt][h * 4 + k][1]);
+          }
+        }
+      }
+
+      // ---- running maximum and sum ------------------------------------------------------------------
+      const float ks[2] = {__shfl_sync(0xffffffffu, cur.ks, 2 * (step & 15)), __shfl_sync(0xffffffffu, cur.ks, 2 * (step & 15) + 1)};
+      const float vs[2] = {__shfl_sync(0xffffffffu, cur.vs, 2 * (step & 15)), __shfl_sync(0xffffffffu, cur.vs, 2 * (step & 15) + 1)};
+      const bool masked = key0 + kStep - 1 > pos_min || key0 < lo_max;
+      // the power of two above the values' scales so far; NaN scales do not enter it (they reach p below)
+      const float vmax = fmaxf(vtop, fmaxf(fabsf(vs[0]), fabsf(vs[1])));
+      float grow = 1.0f;
+      if (vmax > vtop) {
+        const float up = __uint_as_float(min((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
+        grow = vtop / up;
+        vtop = up;
+      }
+      const float vf[2] = {vs[0] * (0x1p14f / vtop), vs[1] * (0x1p14f / vtop)};
+      uint32_t pf[NT][2][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float x = sv[mt][nt][c] * (mult[nt][c & 1] * ks[mt]);
+            if (masked) {
+              const int key = key0 + mt * 16 + (c >> 1) * 8 + g;
+              if (key > hi[nt][c & 1] || key < low[nt][c & 1]) x = -INFINITY;
+            }
+            sv[mt][nt][c] = x;
+            top[c & 1] = fmaxf(top[c & 1], x);
+          }
+        float base[2], keep[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
+          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
+          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
+          const float now = fmaxf(m[nt][c], top[c]);
+          base[c] = now == -INFINITY ? 0.0f : now;
+          keep[c] = exp2_fast(m[nt][c] - base[c]);
+          m[nt][c] = now;
+          l[nt][c] *= keep[c];
+        }
+        float p[2][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float x = exp2_fast(sv[mt][nt][c] - base[c & 1]);
+            l[nt][c & 1] += x;
+            p[mt][c] = x * vf[mt];
+            if (masked) {  // a NaN scale counts only for the rows that see the key
+              const int key = key0 + mt * 16 + (c >> 1) * 8 + g;
+              if (key > hi[nt][c & 1] || key < low[nt][c & 1]) p[mt][c] = 0.0f;
+            }
+          }
+          pf[nt][mt][0] = transpose8x8(pack16(p[mt][0], p[mt][1]));
+          pf[nt][mt][1] = transpose8x8(pack16(p[mt][2], p[mt][3]));
+        }
+        const float k0 = keep[0] * grow, k1 = keep[1] * grow;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          o[nt][i][0] *= k0;
+          o[nt][i][1] *= k1;
+          o[nt][i][2] *= k0;
+          o[nt][i][3] *= k1;
+        }
+      }
+
+      // ---- O' += V' P' ------------------------------------------------------------------------------
+      // thread (g, t) has d = (D / 8) g .. of keys 2t, 2t + 1, 2t + 8, 2t + 9: adjacent keys' bytes are paired, tile i has d = (D / 8) g + 2i in row g, + 1 in row g + 8
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        uint32_t vb[4][D / 32];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = mt * 16 + 2 * t + (e & 1) + (e >> 1) * 8;
+          if (D == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vst + at_chunk<D>(r, g));
+            vb[e][0] = x.x, vb[e][1] = x.y, vb[e][D / 32 - 2] = x.z, vb[e][D / 32 - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(vst + at_chunk<D>(r, g >> 1) + (g & 1) * 8);
+            vb[e][0] = x.x, vb[e][1] = x.y;
+          }
+        }
+        bool apart = false;  // a NaN among values that some rows do not see: the rows' products are taken one by one
+        if (HELD == HELD_E4M3 && masked) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) any |= __vcmpeq4(vb[e][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+          apart = __any_sync(0xffffffffu, any != 0);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          uint32_t f[2][4];
+          widen<HELD>(__byte_perm(vb[0][k], vb[1][k], 0x5140), f[0][0], f[0][1]);
+          widen<HELD>(__byte_perm(vb[2][k], vb[3][k], 0x5140), f[0][2], f[0][3]);
+          widen<HELD>(__byte_perm(vb[0][k], vb[1][k], 0x7362), f[1][0], f[1][1]);
+          widen<HELD>(__byte_perm(vb[2][k], vb[3][k], 0x7362), f[1][2], f[1][3]);
+          if (!apart) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) mma16816(o[nt][2 * k + i], f[i][0], f[i][1], f[i][2], f[i][3], pf[nt][mt][0], pf[nt][mt][1]);
+          } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              for (int col = 0; col < 8; ++col) {
+                const int last = __shfl_sync(0xffffffffu, (col & 1) ? hi[nt][1] : hi[nt][0], col >> 1), begin = __shfl_sync(0xffffffffu, (col & 1) ? low[nt][1] : low[nt][0], col >> 1);
+                uint32_t keep[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int key = key0 + mt * 16 + 2 * t + e * 8;
+                  keep[e] = (key <= last && key >= begin ? 0xffffu : 0u) | (key + 1 <= last && key + 1 >= begin ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                  mma16816(o[nt][2 * k + i], f[i][0] & keep[0], f[i][1] & keep[0], f[i][2] & keep[1], f[i][3] & keep[1], g == col ? pf[nt][mt][0] : 0u,
+                           g == col ? pf[nt][mt][1] : 0u);
+              }
+          }
+        }
+      }
+    }
+
+    // ---- join the warps -------------------------------------------------------------------------------
+    copy_wait<0>();
+    __syncthreads();  // all stages are read; their memory takes the warps' results
+    float* box = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float x = l[nt][c];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int row = nt * 8 + 2 * t + c;
+        if (g == 0) {
+          stat[warp][row][0] = m[nt][c];
+          stat[warp][row][1] = x;
+        }
+        float* to_row = box + (warp * ROWS + row) * C::kPitch + g * (D / 8);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(to_row + 2 * i) = make_float2(o[nt][i][c], o[nt][i][2 + c]);
+      }
+    }
+    if (lane == 0) top_v[warp] = vtop;
+    __syncthreads();
+    const bool whole = from == 0 && to == s.tiles;
+    float* part = sc.part + ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * (ROWS * (D + 2));
+    for (int idx = threadIdx.x; idx < ROWS * (D / 4); idx += kThreads) {
+      const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+      if (row >= rows) break;
+      float mm = fmaxf(fmaxf(stat[0][row][0], stat[1][row][0]), fmaxf(stat[2][row][0], stat[3][row][0]));
+      const float base = mm == -INFINITY ? 0.0f : mm;
+      float sum = 0.0f, v[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const float f = exp2_fast(stat[i][row][0] - base);
+        sum += stat[i][row][1] * f;
+        const float4 x = *reinterpret_cast<const float4*>(box + (i * ROWS + row) * C::kPitch + d);
+        const float fv = f * (top_v[i] * 0x1p-14f);
+        v[0] += x.x * fv, v[1] += x.y * fv, v[2] += x.z * fv, v[3] += x.w * fv;
+      }
+      if (whole) {
+        const int i = (r0 + row) / group;
+        const int64_t out = (int64_t)(s.first + i) * a.q_heads + head * group + (r0 + row - i * group);
+        const bool empty = start + i < 0;
+        if (start + i >= s.keys) sum = NAN;  // its own key is outside the table
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = empty ? 0.0f : v[e] / sum;
+        store4(static_cast<T*>(a.o) + out * D + d, v);
+        if (a.lse && d == 0) a.lse[out] = empty ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
+      } else {
+        *reinterpret_cast<float4*>(part + row * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) {
+          part[ROWS * D + row] = mm;
+          part[ROWS * D + ROWS + row] = sum;
+        }
+      }
+    }
+    __syncthreads();  // the next piece copies over the box
+    first_piece = false;
+    w += to - from;
+    if (w < w_end && w == front + work_of(a, s)) {
+      front = w;
+      do s = seq_of(a, ++b, ROWS); while (work_of(a, s) == 0);  // w < total: there is one
+    }
+  }
+}
+
+// One warp per row: a row whose unit was cut is joined from its pieces, one without keys is zero.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(128) join_kernel(const Kv8Attention a, const Scratch sc, const int grid) {
+  constexpr int ROWS = 8 * NT, PER = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (u >= a.tokens * a.q_heads) return;
+  const int t = (int)(u / a.q_heads), qh = (int)(u - (int64_t)t * a.q_heads), group = (int)(a.q_heads / a.heads);
+  int b, first, count;
+  if (!find_sequence(a.cu, (int)a.batch, a.each, t, b, first, count)) return;
+  const Seq s = seq_of(a, b, ROWS);
+  T* o = static_cast<T*>(a.o) + u * D + lane * PER;
+  const int64_t pos = (int64_t)a.lens[b] - count + (t - first);
+  if (pos < 0 || pos >= s.keys || s.tiles == 0) {  // no keys; or its own key is outside the table (or offsets that cannot be)
+#pragma unroll
+    for (int e = 0; e < PER; ++e) o[e] = from_f32<T>(pos < 0 ? 0.0f : NAN);
+    if (a.lse && lane == 0) a.lse[u] = pos < 0 ? -INFINITY : NAN;
+    return;
+  }
+  const int head = qh / group, r = (t - first) * group + (qh - head * group), row = r % ROWS;
+  const int64_t total = sc.before[a.batch], lo = sc.before[b] + ((int64_t)head * s.units_per_head + r / ROWS) * s.tiles, hi = lo + s.tiles - 1;
+  const int ctas = (int)min((int64_t)grid, total);
+  const int c0 = (int)(((lo + 1) * ctas - 1) / total), c1 = (int)(((hi + 1) * ctas - 1) / total);  // the CTAs whose ranges hold the first and the last tile
+  if (c0 == c1) return;
+  const int64_t size = ROWS * (D + 2);
+  const float* p0 = sc.part + ((int64_t)c0 * 2 + (lo == total * c0 / ctas ? 0 : 1)) * size;
+  auto piece = [&](int c) { return c == c0 ? p0 : sc.part + (int64_t)c * 2 * size; };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, piece(c)[ROWS * D + row]);
+  m = warp_reduce<MaxOp>(m);
+  const float base = m == -INFINITY ? 0.0f : m;
+  float sum = 0.0f, v[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) v[e] = 0.0f;
+#pragma unroll 4
+  for (int c = c0; c <= c1; ++c) {
+    const float* p = piece(c);
+    const float f = exp2_fast(p[ROWS * D + row] - base);
+    sum += p[ROWS * D + ROWS + row] * f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) v[e] += p[row * D + lane * PER + e] * f;
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = from_f32<T>(v[e] / sum);
+  if (a.lse && lane == 0) a.lse[u] = (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Rows of a unit, in eights: one where 8 rows suffice, two where a sequence has more (several new tokens, many heads to a group) so
+// that its keys are read half as often; with offsets the average number of new tokens decides.  (Four spill registers at D = 128.)
+int tiles_of_rows(int64_t tokens, int64_t batch, int64_t group) {
+  const int64_t rows = group * ((tokens + batch - 1) / batch);
+  return rows <= 8 ? 1 : 2;
+}
+int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, int nt) {
+  // no more CTAs than there can be tiles
+  const int64_t units = heads * ((tokens * group + 8 * nt - 1) / (8 * nt) + batch), tiles = table_blocks * block / kTile + 2;
+  const int64_t most = (int64_t)kSmCount * (dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas);
+  return units > most || units * tiles > most ? most : units * tiles;
+}
+
+template <typename T, int HELD, int D, int NT> int run_attention(const Kv8Attention& a, int grid, void* scratch, cudaStream_t s) {
+  auto* kern = attention_kernel<T, HELD, D, NT>;
+  IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
+  const Scratch sc = carve(scratch, a.batch);
+  const int q_vec = (reinterpret_cast<uintptr_t>(a.q) & 7) == 0 && a.q_token % 4 == 0 && a.q_head % 4 == 0;
+  kern<<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, q_vec);
+  if (cudaPeekAtLastError() != cudaSuccess) return cuda_fail(cudaGetLastError(), "attention_kv8 launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((a.tokens * a.q_heads + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, sc, grid));
+  return IB200_OK;
+}
+template <typename T, int HELD, int D> int run_nt(const Kv8Attention& a, int nt, int grid, void* scratch, cudaStream_t s) {
+  return nt == 1 ? run_attention<T, HELD, D, 1>(a, grid, scratch, s) : run_attention<T, HELD, D, 2>(a, grid, scratch, s);
+}
+template <typename T, int HELD> int run_dim(const Kv8Attention& a, int nt, int grid, void* scratch, cudaStream_t s) {
+  return a.dim == 128 ? run_nt<T, HELD, 128>(a, nt, grid, scratch, s) : run_nt<T, HELD, 64>(a, nt, grid, scratch, s);
+}
+
+}  // namespace
+
+size_t kv8_attention_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block, int64_t table_blocks) {
+  if (tokens <= 0 || batch <= 0 || heads <= 0 || q_heads < heads || (dim != 64 && dim != 128) || block <= 0 || table_blocks < 0 || batch > INT32_MAX ||
+      tokens > INT32_MAX || q_heads > 65535 || beyond_any_device(table_blocks, block))
+    return 0;  // the launch refuses these, or does nothing
+  const int nt = tiles_of_rows(tokens, batch, q_heads / heads);
+  return prefix_bytes(batch) + (size_t)grid_of(tokens, batch, heads, q_heads / heads, dim, block, table_blocks, nt) * 2 * 8 * nt * (dim + 2) * 4;
+}
+
+int launch_kv8_attention(Kv8Attention& a, int dtype, int held, void* scratch, size_t scratch_bytes, cudaStream_t s) {
+  if (int rc = check_kv8("attention_kv8", a.pages, a.heads, a.block, a.dim, a.batch, a.table_blocks, a.tokens, held, dtype, a.cu)) return rc;
+  if (a.q_heads < 0 || (a.heads > 0 ? a.q_heads % a.heads : a.q_heads)) return fail(IB200_ERR_INVALID, "attention_kv8: query heads must be a multiple of the cache's");
+  if (a.q_heads > 65535) return fail(IB200_ERR_UNSUPPORTED, "attention_kv8: fewer than 2^16 query heads");
+  if (a.window < 0) return fail(IB200_ERR_INVALID, "attention_kv8: negative window");
+  if (a.tokens == 0 || a.q_heads == 0 || a.batch == 0) return IB200_OK;
+  if (!a.q || !a.o || !a.lens || (a.table_blocks > 0 && !a.table) || (a.pages > 0 && (!a.k_cache || !a.v_cache || !a.k_scale || !a.v_scale)))
+    return fail(IB200_ERR_INVALID, "attention_kv8: null operand");
+  if (!aligned16(a.k_cache) || !aligned16(a.v_cache)) return fail(IB200_ERR_INVALID, "attention_kv8: caches must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a.o) & 7) return fail(IB200_ERR_INVALID, "attention_kv8: o must be 8-byte aligned");
+  if (a.tokens * a.q_heads >= INT32_MAX || beyond_any_device(a.tokens, a.q_heads, a.dim)) return fail(IB200_ERR_UNSUPPORTED, "attention_kv8: too many rows");
+  if (!scratch || scratch_bytes < kv8_attention_scratch_bytes(a.tokens, a.batch, a.q_heads, a.heads, a.dim, a.block, a.table_blocks))
+    return fail(IB200_ERR_BUFFER, "attention_kv8: scratch is smaller than ib200_attention_kv8_scratch_bytes");
+  if (a.pages == 0) a.k_cache = a.v_cache = static_cast<const uint8_t*>(scratch);  // an address for copies that take nothing
+  a.each = (int)(a.tokens / a.batch);
+  const int64_t group = a.q_heads / a.heads;
+  const int nt = tiles_of_rows(a.tokens, a.batch, group), grid = (int)grid_of(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, nt);
+  if (dtype == IB200_BF16)
+    return held == IB200_E4M3 ? run_dim<__nv_bfloat16, HELD_E4M3>(a, nt, grid, scratch, s) : run_dim<__nv_bfloat16, HELD_I8>(a, nt, grid, scratch, s);
+  return held == IB200_E4M3 ? run_dim<__half, HELD_E4M3>(a, nt, grid, scratch, s) : run_dim<__half, HELD_I8>(a, nt, grid, scratch, s);
+}
+
+}  // namespace ib200
