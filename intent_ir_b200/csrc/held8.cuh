@@ -44,6 +44,19 @@ template <int HELD> __device__ __forceinline__ float held_value(uint8_t b) {
   if (HELD == HELD_I8) return (float)(int8_t)b;
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(b, __NV_E4M3)));
 }
+// four bytes as two pairs of f16, exact
+template <int HELD> __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (HELD == HELD_E4M3) {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}" : "=r"(lo), "=r"(hi) : "r"(w));
+  } else {  // the byte as 1024 + (i + 128), minus 1152
+    w ^= 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    uint32_t l = __byte_perm(w, 0x64646464u, 0x4140), h = __byte_perm(w, 0x64646464u, 0x4342);
+    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&l), off), b = __hsub2(*reinterpret_cast<__half2*>(&h), off);
+    lo = *reinterpret_cast<uint32_t*>(&a);
+    hi = *reinterpret_cast<uint32_t*>(&b);
+  }
+}
 #endif
 
 }  // namespace ib200

@@ -3,6 +3,7 @@
 // q is [N, K/2], the even k of a byte in its low half; z is 8 where there are no zero points; xs (the scales of 8-bit
 // activations) is 1, one value per row, or one per row and group.  x * (q - z) is exact in f32 (and in the 16-bit types),
 // sums are f32.
+#include "async.cuh"
 #include "common.cuh"
 #include "held8.cuh"
 
@@ -19,58 +20,310 @@ struct W4Args {
   void* y;
   int64_t x_stride;
   int m, n, k, group, groups, xs_groups;
+  int x_type, s_type, y_type, x_vec, split;
 };
 
-enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
-template <int XK> __device__ __forceinline__ float x_value(const void* x, int64_t i) {
-  if (XK == X_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(x)[i]);
-  if (XK == X_F16) return __half2float(static_cast<const __half*>(x)[i]);
-  return held_value<XK == X_E4M3 ? HELD_E4M3 : HELD_I8>(static_cast<const uint8_t*>(x)[i]);
+__device__ __forceinline__ void cluster_arrive_wait() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float cluster_read(const float* local, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_map(local, (uint32_t)rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
+  if (type == IB200_F32) return static_cast<const float*>(p)[i];
+  if (type == IB200_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
 }
 
-// one warp per output and row of x; a lane takes 8 adjacent k (one word of q), which lie in one group
-template <int XK, typename TS, typename TY>
-__global__ void __launch_bounds__(256) w4_fma_kernel(const W4Args a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t total = (int64_t)a.n * a.m;
-  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < total; u += (int64_t)gridDim.x * 8) {
-    const int n = (int)(u % a.n), m = (int)(u / a.n);
-    float acc = 0.0f;
-    for (int k = lane * 8; k < a.k; k += 256) {
-      const int g = k / a.group;
-      const uint8_t* q = a.q + ((int64_t)n * a.k + k) / 2;
-      const float z = a.z ? (float)a.z[(int64_t)n * a.groups + g] : 8.0f;
-      float part = 0.0f;
-      for (int i = 0; i < 8; ++i) {
-        const float v = (float)((q[i >> 1] >> (4 * (i & 1))) & 15) - z;
-        part = fmaf(x_value<XK>(a.x, m * a.x_stride + k + i), v, part);
-      }
-      float s = to_f32(static_cast<const TS*>(a.s)[(int64_t)n * a.groups + g]);
-      if (a.xs) s *= a.xs[(int64_t)m * a.xs_groups + (a.xs_groups == 1 ? 0 : g)];
-      acc = fmaf(part, s, acc);
+// ---- few rows of x: weights stream through shared memory into mma.sync ----------------------------------
+// A CTA has 128 rows of q, 16 to a warp, and a slice of K; the CTAs of a cluster share the rows and split K, and add their
+// sums up through distributed shared memory in a fixed order.  Weights are the 16 rows of m16n8k16, 8 rows of x its
+// columns.  A thread's k slots need not be adjacent as long as both operands agree: inside a group of G, thread t of a quad owns
+// the G / 4 adjacent k from t * G / 4, one 32-bit word of q (8 k) per two products, which keeps every product inside one
+// group; the group's sum is then scaled in f32.  A word gives pairs (0, 4), (1, 5), (2, 6), (3, 7), so x is laid down in that order, in
+// the order in which the warps read it.  128 + q in bf16 (1024 + q in f16) is q under the exponent of 128 (1024); minus 128 + z it is exact.
+constexpr int kRows = 128, kThreads = 256, kStageK = 256, kStages = 4, kRowBytes = kStageK / 2, kStageBytes = kRows * kRowBytes;
+
+// 16-byte chunk c of row r: eight lanes of a 16-, 8- or 4-byte read touch all banks once
+__device__ __forceinline__ int at_chunk(int r, int c) { return r * kRowBytes + ((c ^ ((r & 6) ^ ((r & 1) << 2) ^ ((r >> 2) & 1))) << 4); }
+
+template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+struct Zero {  // what brings a nibble under an exponent back to q - z, both halves
+  uint32_t lo, hi;
+};
+template <bool BF> __device__ __forceinline__ Zero zero_of(uint32_t z) {
+  if (BF) return {(0x4300u | z) * 0x10001u, 0};
+  return {(0x6400u | z) * 0x10001u, (0xD400u | z << 4) * 0x10001u};  // 1024 + z; -(64 + z)
+}
+// the pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's eight q - z
+template <bool BF> __device__ __forceinline__ void weights_of(uint32_t w, const Zero& z, uint32_t (&v)[4]) {
+  if (BF) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&z.lo));
+      v[i] = *reinterpret_cast<const uint32_t*>(&d);
     }
-    acc = warp_reduce<SumOp>(acc);
-    if (lane == 0) {
-      if (a.bias) acc += to_f32(static_cast<const TY*>(a.bias)[n]);
-      static_cast<TY*>(a.y)[(int64_t)m * a.n + n] = from_f32<TY>(acc);
+  } else {
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2C00));
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const uint32_t x = w >> (4 * i), a = (x & 0x000f000fu) | 0x64006400u, b = (x & 0x00f000f0u) | 0x64006400u;  // 1024 + q, 1024 + 16 q
+      const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&z.lo));
+      const __half2 e = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, *reinterpret_cast<const __half2*>(&z.hi));
+      v[i] = *reinterpret_cast<const uint32_t*>(&d);
+      v[i + 1] = *reinterpret_cast<const uint32_t*>(&e);
     }
   }
 }
+// 8 adjacent x as the pairs above; 8-bit values become f16, which is exact
+__device__ __forceinline__ uint4 x_chunk(const W4Args& a, int row, int k) {
+  if (row >= a.m || k >= a.k) return make_uint4(0, 0, 0, 0);
+  const int64_t at = (int64_t)row * a.x_stride + k;
+  if (a.x_type == IB200_BF16 || a.x_type == IB200_F16) {
+    const uint16_t* p = static_cast<const uint16_t*>(a.x) + at;
+    uint4 r;
+    if (a.x_vec) {
+      r = *reinterpret_cast<const uint4*>(p);
+    } else {
+      r.x = p[0] | (uint32_t)p[1] << 16, r.y = p[2] | (uint32_t)p[3] << 16, r.z = p[4] | (uint32_t)p[5] << 16, r.w = p[6] | (uint32_t)p[7] << 16;
+    }
+    return make_uint4(__byte_perm(r.x, r.z, 0x5410), __byte_perm(r.x, r.z, 0x7632), __byte_perm(r.y, r.w, 0x5410), __byte_perm(r.y, r.w, 0x7632));
+  }
+  const uint8_t* p = static_cast<const uint8_t*>(a.x) + at;
+  uint32_t lo, hi;
+  if (a.x_vec) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    lo = r.x, hi = r.y;
+  } else {
+    lo = p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
+    hi = p[4] | (uint32_t)p[5] << 8 | (uint32_t)p[6] << 16 | (uint32_t)p[7] << 24;
+  }
+  uint4 r;
+  const uint32_t a01 = __byte_perm(lo, hi, 0x5140), a23 = __byte_perm(lo, hi, 0x7362);  // bytes 0 4 1 5, 2 6 3 7
+  if (a.x_type == IB200_E4M3) {
+    widen<HELD_E4M3>(a01, r.x, r.y);
+    widen<HELD_E4M3>(a23, r.z, r.w);
+  } else {
+    widen<HELD_I8>(a01, r.x, r.y);
+    widen<HELD_I8>(a23, r.z, r.w);
+  }
+  return r;
+}
 
-template <int XK, typename TS, typename TY> int run_w4(const W4Args& a, cudaStream_t s) {
-  const int64_t blocks = ((int64_t)a.n * a.m + 7) / 8;
-  w4_fma_kernel<XK, TS, TY><<<(unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), 256, 0, s>>>(a);
-  return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "w4_matmul launch");
+template <bool BF, int NT, int G>
+__global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) {
+  constexpr int GROUPS = kStageK / G, WORDS = G / 32, XBYTES = NT * 8 * kStageK * 2;  // groups of a stage, words of a thread in a group
+  constexpr int HOLD = (GROUPS + 3) / 4;                                               // scales that a lane of a quad holds for a row
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* xbuf = smem + kStages * kStageBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kRows, m0 = blockIdx.y * NT * 8;
+  const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
+
+  const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
+  auto issue = [&](int s) {  // 128 rows x 128 bytes; what lies outside is zero
+    const uint32_t dst = smem_at + ((s - s0) % kStages) * kStageBytes;
+#pragma unroll
+    for (int i = 0; i < kRows * 8 / kThreads; ++i) {
+      const int idx = i * kThreads + threadIdx.x, r = idx >> 3, c = idx & 7;
+      const bool take = n0 + r < a.n && s * kStageK + c * 32 < a.k;
+      const uint8_t* src = take ? a.q + ((int64_t)(n0 + r) * a.k + s * kStageK + c * 32) / 2 : a.q;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + at_chunk(r, c)), "l"(src), "r"(take ? 16 : 0) : "memory");
+    }
+  };
+  // x: chunk (8 k) of row m, where the warps read it: [group, word][tile of 8 rows][row][thread of the quad]
+  auto x_place = [&](int idx) {
+    const int row = idx / (kStageK / 8), k = idx % (kStageK / 8) * 8, in = k % G, th = in / (G / 4), word = in % (G / 4) / 8;
+    return (((k / G * WORDS + word) * NT + row / 8) * 8 + row % 8) * 4 + th;
+  };
+  uint4 xr[NT];
+  auto x_load = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int idx = i * kThreads + threadIdx.x;
+      xr[i] = x_chunk(a, m0 + idx / (kStageK / 8), s * kStageK + idx % (kStageK / 8) * 8);
+    }
+  };
+  auto x_store = [&](int s) {
+    uint4* to = reinterpret_cast<uint4*>(xbuf + ((s - s0) & 1) * XBYTES);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) to[x_place(i * kThreads + threadIdx.x)] = xr[i];
+  };
+  // scales and zero points of the thread's two rows (16 * warp + g, + 8): lane t of a quad holds groups t, t + 4 of the stage
+  const int row_a = n0 + warp * 16 + g;
+  float sc[2][HOLD];
+  uint32_t zp[2][HOLD];
+  auto scale_load = [&](int s) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int h = 0; h < HOLD; ++h) {
+        const int row = row_a + 8 * r, in = h * 4 + t, grp = s * GROUPS + in;
+        const bool take = row < a.n && in < GROUPS && grp < a.groups;
+        const int64_t at = (int64_t)row * a.groups + grp;
+        sc[r][h] = take ? float_of(a.s, at, a.s_type) : 0.0f;
+        zp[r][h] = take && a.z ? a.z[at] & 15u : 8u;
+      }
+  };
+
+  float sum[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.0f;
+
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (s0 + i < s1) issue(s0 + i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  if (s0 < s1) {
+    x_load(s0);
+    x_store(s0);
+    if (s0 + 1 < s1) x_load(s0 + 1);
+    scale_load(s0);
+  }
+  for (int s = s0; s < s1; ++s) {
+    float scn[2][HOLD];
+    uint32_t zpn[2][HOLD];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int h = 0; h < HOLD; ++h) scn[r][h] = sc[r][h], zpn[r][h] = zp[r][h];
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncthreads();
+    if (s + kStages - 1 < s1) issue(s + kStages - 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (s + 1 < s1) {
+      x_store(s + 1);
+      if (s + 2 < s1) x_load(s + 2);
+      scale_load(s + 1);
+    }
+    const uint8_t* wst = smem + ((s - s0) % kStages) * kStageBytes;
+    const uint4* xst = reinterpret_cast<const uint4*>(xbuf + ((s - s0) & 1) * XBYTES) + lane;
+#pragma unroll
+    for (int grp = 0; grp < GROUPS; ++grp) {
+      uint32_t wa[WORDS], wb[WORDS];
+      const int byte = grp * (G / 2) + t * (G / 8);  // of the row
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint8_t* p = wst + at_chunk(warp * 16 + g + 8 * r, byte >> 4) + (byte & 15);
+        uint32_t(&to)[WORDS] = r ? wb : wa;
+        if (G == 128) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p);
+          to[0] = v.x, to[WORDS > 1 ? 1 : 0] = v.y, to[WORDS > 2 ? 2 : 0] = v.z, to[WORDS > 3 ? 3 : 0] = v.w;
+        } else if (G == 64) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
+          to[0] = v.x, to[WORDS > 1 ? 1 : 0] = v.y;
+        } else {
+          to[0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      }
+      const int from = (lane & ~3) | (grp & 3);
+      const float sa = __shfl_sync(0xffffffffu, scn[0][grp >> 2], from), sb = __shfl_sync(0xffffffffu, scn[1][grp >> 2], from);
+      Zero za, zb;
+      if (a.z) {
+        za = zero_of<BF>(__shfl_sync(0xffffffffu, zpn[0][grp >> 2], from));
+        zb = zero_of<BF>(__shfl_sync(0xffffffffu, zpn[1][grp >> 2], from));
+      } else {
+        za = zb = zero_of<BF>(8);
+      }
+      float acc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        uint32_t va[4], vb[4];
+        weights_of<BF>(wa[w], za, va);
+        weights_of<BF>(wb[w], zb, vb);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 x = xst[((grp * WORDS + w) * NT + nt) * 32];
+          mma<BF>(acc[nt], va[0], vb[0], va[1], vb[1], x.x, x.y);
+          mma<BF>(acc[nt], va[2], vb[2], va[3], vb[3], x.z, x.w);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f0 = 1.0f, f1 = 1.0f;
+        if (a.xs_groups > 1) {
+          const int m = m0 + nt * 8 + 2 * t, at = s * GROUPS + grp;
+          f0 = m < a.m && at < a.groups ? a.xs[(int64_t)m * a.groups + at] : 0.0f;
+          f1 = m + 1 < a.m && at < a.groups ? a.xs[(int64_t)(m + 1) * a.groups + at] : 0.0f;
+        }
+        sum[nt][0] = fmaf(acc[nt][0], sa * f0, sum[nt][0]);
+        sum[nt][1] = fmaf(acc[nt][1], sa * f1, sum[nt][1]);
+        sum[nt][2] = fmaf(acc[nt][2], sb * f0, sum[nt][2]);
+        sum[nt][3] = fmaf(acc[nt][3], sb * f1, sum[nt][3]);
+      }
+    }
+  }
+
+  // ---- add up the cluster's slices and write --------------------------------------------------------------
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float* box = reinterpret_cast<float*>(smem);  // [NT * 8][128] sums of this CTA
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) box[(nt * 8 + 2 * t + (c & 1)) * kRows + warp * 16 + g + 8 * (c >> 1)] = sum[nt][c];
+  if (split > 1) cluster_arrive_wait(); else __syncthreads();
+  const int rows = min(NT * 8, a.m - m0);
+  for (int idx = rank * kThreads + threadIdx.x; idx < rows * kRows; idx += split * kThreads) {
+    const int m = m0 + idx / kRows, n = n0 + idx % kRows;
+    float v = 0.0f;
+    for (int r = 0; r < split; ++r) v += split > 1 ? cluster_read(box + idx, r) : box[idx];
+    if (n >= a.n) continue;
+    if (a.xs_groups == 1) v *= a.xs[m];
+    if (a.bias) v += float_of(a.bias, n, a.y_type);
+    const int64_t at = (int64_t)m * a.n + n;
+    if (a.y_type == IB200_F32) static_cast<float*>(a.y)[at] = v;
+    else if (a.y_type == IB200_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(a.y)[at] = __float2half_rn(v);
+  }
+  if (split > 1) cluster_arrive_wait();  // nobody leaves while its sums are read
 }
-template <int XK, typename TS> int run_w4_out(const W4Args& a, int out, cudaStream_t s) {
-  if (out == IB200_BF16) return run_w4<XK, TS, __nv_bfloat16>(a, s);
-  if (out == IB200_F16) return run_w4<XK, TS, __half>(a, s);
-  return run_w4<XK, TS, float>(a, s);
+
+template <bool BF, int NT, int G> int run_stream(W4Args a, cudaStream_t s) {
+  auto* kern = w4_stream_kernel<BF, NT, G>;
+  constexpr int SMEM = kStages * kStageBytes + 2 * NT * 8 * kStageK * 2;
+  IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+  // K is split until the CTAs fill two per SM: one wave, all of it loading from the start
+  const int tiles = (a.n + kRows - 1) / kRows, stages = (a.k + kStageK - 1) / kStageK, mt = (a.m + NT * 8 - 1) / (NT * 8);
+  int split = 1;
+  while (split < 8 && 2 * split <= stages && (int64_t)tiles * mt * split * 2 <= 2 * kSmCount) split *= 2;
+  a.split = split;
+  if ((int64_t)tiles * split > INT32_MAX || mt > 65535) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: too many rows");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * split), (unsigned)mt);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a));
+  return IB200_OK;
 }
-template <int XK> int run_w4_scale(const W4Args& a, int st, int out, cudaStream_t s) {
-  if (st == IB200_BF16) return run_w4_out<XK, __nv_bfloat16>(a, out, s);
-  if (st == IB200_F16) return run_w4_out<XK, __half>(a, out, s);
-  return run_w4_out<XK, float>(a, out, s);
+template <bool BF, int NT> int run_stream_group(const W4Args& a, cudaStream_t s) {
+  if (a.group == 128) return run_stream<BF, NT, 128>(a, s);
+  if (a.group == 64) return run_stream<BF, NT, 64>(a, s);
+  return run_stream<BF, NT, 32>(a, s);
+}
+template <bool BF> int run_stream_rows(const W4Args& a, cudaStream_t s) {
+  if (a.m <= 8) return run_stream_group<BF, 1>(a, s);
+  if (a.m <= 16) return run_stream_group<BF, 2>(a, s);
+  return run_stream_group<BF, 4>(a, s);
 }
 
 }  // namespace
@@ -97,12 +350,11 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
   if (!y || (k > 0 && (!x || !q || !scales || (held && !xs)))) return fail(IB200_ERR_INVALID, "w4_matmul: null operand");
   if (!aligned16(q)) return fail(IB200_ERR_INVALID, "w4_matmul: q must be 16-byte aligned");
   if (m > 1 && (x_stride < k || beyond_any_device(m, x_stride > 0 ? x_stride : 1))) return fail(IB200_ERR_INVALID, "w4_matmul: bad row stride of x");
+  const int e = held ? 1 : 2;
+  const bool x_vec = (reinterpret_cast<uintptr_t>(x) & (held ? 7 : 15)) == 0 && (m == 1 || x_stride * e % (held ? 8 : 16) == 0);
   W4Args a{x, static_cast<const uint8_t*>(q), scales, static_cast<const uint8_t*>(zeros), bias, xs, y, x_stride,
-           (int)m, (int)n, (int)k, (int)group, (int)groups, (int)xs_groups};
-  if (x_dtype == IB200_BF16) return run_w4_scale<X_BF16>(a, s_dtype, out_dtype, s);
-  if (x_dtype == IB200_F16) return run_w4_scale<X_F16>(a, s_dtype, out_dtype, s);
-  if (x_dtype == IB200_E4M3) return run_w4_scale<X_E4M3>(a, s_dtype, out_dtype, s);
-  return run_w4_scale<X_I8>(a, s_dtype, out_dtype, s);
+           (int)m, (int)n, (int)k, (int)group, (int)groups, (int)xs_groups, x_dtype, s_dtype, out_dtype, x_vec, 1};
+  return x_dtype == IB200_BF16 ? run_stream_rows<true>(a, s) : run_stream_rows<false>(a, s);
 }
 
 }  // namespace ib200
