@@ -282,25 +282,43 @@ IB200_API int ib200_transpose2d(const void* x, void* out, int elem_bytes, int64_
  * Strides are in elements; every other array is dense.
  * ====================================================================================== */
 
-/* h = x + residual;  y = h / sqrt(mean(h^2) + eps) * w  over rows of `cols` elements, computed from the unrounded sum.
+/* The entries take their arguments in a struct, read during the call; every field is 8 bytes wide, unused ones are 0.
+ *
+ * h = x + residual;  y = h / sqrt(mean(h^2) + eps) * w  over rows of `cols` elements, computed from the unrounded sum.
  * residual may be NULL (h = x); h (its rounded value, row stride h_stride) may be NULL, and may be the memory of x or
  * residual.  dtype (x, residual, h): IB200_F32, IB200_BF16 or IB200_F16; w (NULL: ones) has dtype or IB200_F32.  out_dtype:
  * dtype, or IB200_E4M3 / IB200_I8 with scale[rows, groups] (f32):  s = max|y| / Q over a group, y / s rounded to nearest even,
  * Q = 448 / 127.  group: 32, 64, 128 or 256 columns (the last one may be shorter), 0: the row.  A group of zeros (or below
  * 2^-119) holds zeros; one with a NaN or an infinity has a NaN or infinite scale and stands for NaN.  y is dense. */
-IB200_API int ib200_rmsnorm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* w, void* y,
-                  void* h, int64_t h_stride, float* scale, int dtype, int w_dtype, int out_dtype, int64_t rows, int64_t cols,
-                  int64_t group, float eps, void* stream);
+typedef struct ib200_rmsnorm_args {
+  const void *x, *residual, *w;
+  void *y, *h;
+  float* scale;
+  int64_t x_stride, residual_stride, h_stride;
+  int64_t dtype, w_dtype, out_dtype;
+  int64_t rows, cols, group;
+  double eps;
+} ib200_rmsnorm_args;
+IB200_API int ib200_rmsnorm(const ib200_rmsnorm_args* args, void* stream);
 
 /* y[m, n] = sum over groups g of scales[n, g] * x_scale[m, g] * (sum over k in g of x[m, k] * (q[n, k] - zeros[n, g])) + bias[n]
  * q: [N, K/2] bytes, 16-byte aligned, the even k of a pair in the low four bits; scales: [N, ceil(K / group)] of s_dtype (f32,
  * bf16, f16); zeros: bytes 0..15 of the same shape, or NULL (8); bias (NULL: none) and y have out_dtype (f32, bf16, f16).
  * x: [M, K] bf16 or f16 with x_scale NULL and x_scale_groups 0, or e4m3 / int8 with x_scale f32 [M, x_scale_groups], 1 or
  * ceil(K / group) of them.  group: 32, 64 or 128; K a multiple of 32; M and N any.  f32 sums.  scratch: 256-byte aligned,
- * ib200_w4_scratch_bytes(...) bytes, contents irrelevant, not shared with a launch that may run at the same time. */
-IB200_API int ib200_w4_matmul(const void* x, int64_t x_stride, const float* x_scale, int64_t x_scale_groups, const void* q, const void* scales,
-                    const void* zeros, const void* bias, void* y, int x_dtype, int s_dtype, int out_dtype, int64_t m, int64_t n,
-                    int64_t k, int64_t group, void* scratch, size_t scratch_bytes, int32_t* status, void* stream);
+ * ib200_w4_scratch_bytes(...) bytes, contents irrelevant, not shared with a launch that may run at the same time.  status: a device
+ * int32, zero, as for ib200_gemm_bias_act. */
+typedef struct ib200_w4_args {
+  const void* x;
+  const float* x_scale;
+  const void *q, *scales, *zeros, *bias;
+  void *y, *scratch;
+  int32_t* status;
+  int64_t x_stride, x_scale_groups;
+  int64_t x_dtype, s_dtype, out_dtype;
+  int64_t m, n, k, group, scratch_bytes;
+} ib200_w4_args;
+IB200_API int ib200_w4_matmul(const ib200_w4_args* args, void* stream);
 IB200_API size_t ib200_w4_scratch_bytes(int x_dtype, int64_t m, int64_t n, int64_t k, int64_t group);
 
 /* A paged key / value cache held in 8 bits: k_cache, v_cache [pages, heads, block, dim] of e4m3 or int8 (`held`), k_scale, v_scale
@@ -313,21 +331,37 @@ IB200_API size_t ib200_w4_scratch_bytes(int x_dtype, int64_t m, int64_t n, int64
  * append: the block of a head gets the scale s' = max(s, max|new| / Q), s = 0 where the block begins with a new token; values held before are
  * rounded again to q * s / s' where s' > s, new ones to x / s' (nearest even).  Slots behind a sequence's end are left as they are.
  * No two sequences may append to one page in the same call. */
-IB200_API int ib200_kv8_append(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
-                     int64_t v_head_stride, void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int32_t* table,
-                     const int32_t* lens, const int32_t* cu, int dtype, int held, int64_t tokens, int64_t batch, int64_t heads, int64_t dim,
-                     int64_t pages, int64_t block, int64_t table_blocks, void* stream);
+typedef struct ib200_kv8_append_args {
+  const void *k, *v; /* [tokens, heads, dim] */
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  const int32_t *table, *lens, *cu;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t dtype, held;
+  int64_t tokens, batch, heads, dim, pages, block, table_blocks;
+} ib200_kv8_append_args;
+IB200_API int ib200_kv8_append(const ib200_kv8_append_args* args, void* stream);
 
 /* Attention of the new tokens over that cache (they are in it already): o[t, h] = sum_j softmax_j(scale * q[t, h] . k[j]) v[j] over the keys
  * j <= p of the token's sequence, p = lens - (new tokens) + its place among them, and j > p - window where window > 0; query heads
- * h * q_heads / heads .. share a key head.  lse (f32 [tokens, q_heads], NULL: none) is the log of the softmax's denominator.  A row without keys is 0 with
- * lse -inf; one that needs a page outside the cache is NaN.  scratch: 256-byte aligned, ib200_attention_kv8_scratch_bytes(...) bytes,
- * contents irrelevant, not shared with a launch that may run at the same time. */
-IB200_API int ib200_attention_kv8(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache, const void* v_cache,
-                        const float* k_scale, const float* v_scale, const int32_t* table, const int32_t* lens, const int32_t* cu,
-                        void* o, float* lse, int dtype, int held, int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads,
-                        int64_t dim, int64_t pages, int64_t block, int64_t table_blocks, int64_t window, float scale, void* scratch,
-                        size_t scratch_bytes, void* stream);
+ * h * q_heads / heads .. share a key head.  o is dense and 8-byte aligned.  lse (f32 [tokens, q_heads], NULL: none) is the log of the softmax's
+ * denominator.  A row without keys is 0 with lse -inf; one that needs a page outside the cache or a token outside the table is NaN.
+ * scratch: 256-byte aligned, ib200_attention_kv8_scratch_bytes(...) bytes, contents irrelevant, not shared with a launch that may
+ * run at the same time. */
+typedef struct ib200_attention_kv8_args {
+  const void* q; /* [tokens, q_heads, dim] */
+  const void *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int32_t *table, *lens, *cu;
+  void* o;
+  float* lse;
+  void* scratch;
+  int64_t q_token_stride, q_head_stride;
+  int64_t dtype, held;
+  int64_t tokens, batch, q_heads, heads, dim, pages, block, table_blocks, window, scratch_bytes;
+  double scale;
+} ib200_attention_kv8_args;
+IB200_API int ib200_attention_kv8(const ib200_attention_kv8_args* args, void* stream);
 IB200_API size_t ib200_attention_kv8_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block,
                                          int64_t table_blocks);
 

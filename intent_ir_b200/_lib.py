@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -70,15 +71,20 @@ SIGNATURES = {
     "ib200_gemm_scratch_bytes": (_sz, [_i, _i, _i64, _i64, _i64, _i, _i]),
     "ib200_check_status": (_i, [_vp, _vp]),
     "ib200_transpose2d": (_i, [_vp, _vp, _i, _i64, _i64, _vp]),
-    "ib200_rmsnorm": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i, _i, _i, _i64, _i64, _i64, _f, _vp]),
-    "ib200_w4_matmul": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i64, _vp, _sz, _vp, _vp]),
+    "ib200_rmsnorm": (_i, [_cp, _vp]),
+    "ib200_w4_matmul": (_i, [_cp, _vp]),
     "ib200_w4_scratch_bytes": (_sz, [_i, _i64, _i64, _i64, _i64]),
-    "ib200_kv8_append": (_i, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _i64,
-                              _i64, _i64, _vp]),
-    "ib200_attention_kv8": (_i, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _i64, _i64, _i64, _i64,
-                                 _i64, _i64, _i64, _f, _vp, _sz, _vp]),
+    "ib200_kv8_append": (_i, [_cp, _vp]),
+    "ib200_attention_kv8": (_i, [_cp, _vp]),
     "ib200_attention_kv8_scratch_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
 }
+
+# the argument structs of the serving entries (every field 8 bytes: pointers, int64, double), in the header's order; a bytes
+# object packed by one of them costs a third of ctypes' conversion of as many positional arguments
+RMSNORM_ARGS = struct.Struct("=6Q9qd")
+W4_ARGS = struct.Struct("=9Q10q")
+KV8_APPEND_ARGS = struct.Struct("=9Q13q")
+ATTENTION_KV8_ARGS = struct.Struct("=11Q14qd")
 
 _lib: Optional[C.CDLL] = None
 

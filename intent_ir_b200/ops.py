@@ -8,6 +8,7 @@ frontends/cuda/runtime.py:641-669), enqueues the kernel on torch's current strea
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Dict, Optional, Sequence, Tuple
 
 import torch
@@ -48,7 +49,8 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the handle of torch.cuda.current_stream(), without building the Stream object (3 us of a 10 us call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def code_of(t: torch.Tensor) -> int:
@@ -250,16 +252,26 @@ def transpose2d(x: torch.Tensor) -> torch.Tensor:
 
 
 # ---- a decoder layer's serving step: activations, weights and the key / value cache in 8 or 4 bits ------------
+# One-token steps are launch-bound, so these calls test all their arguments in one expression and look for the one
+# to name only when it fails.
 
 _FLOAT_CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _HALF_CODE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _HELD_CODE = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.I8}
 
 
-def _on_device(dev: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+def _on_device(index: int, **tensors: Optional[torch.Tensor]) -> None:
     for name, t in tensors.items():
-        if t is not None and (not isinstance(t, torch.Tensor) or t.device != dev):
-            raise B200RuntimeError(f"{name} must be a tensor on {dev}")
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index):
+            raise B200RuntimeError(f"{name} must be a tensor on cuda:{index}")
+
+
+def _first(name: str, t) -> int:
+    """The device of a call's first tensor."""
+    index = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if index < 0:
+        raise B200RuntimeError(f"{name} must be a CUDA tensor")
+    return index
 
 
 def _dense(name: str, t: torch.Tensor, shape: Sequence[int], dtype: torch.dtype) -> None:
@@ -267,15 +279,13 @@ def _dense(name: str, t: torch.Tensor, shape: Sequence[int], dtype: torch.dtype)
         raise B200RuntimeError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
 
 
-def _rows(name: str, t: torch.Tensor) -> Tuple[int, int, int]:
-    """rows, columns and the row stride of a contiguous tensor, or of a matrix of evenly spaced contiguous rows."""
-    if t.dim() == 0:
-        raise B200RuntimeError(f"{name} must have at least one axis")
-    cols = t.shape[-1]
-    if t.is_contiguous():
-        return t.shape[:-1].numel(), cols, cols
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= cols:
-        return t.shape[0], cols, t.stride(0)
+def _row_stride(name: str, t: torch.Tensor) -> int:
+    """The row stride of a contiguous tensor, or of a matrix of evenly spaced contiguous rows."""
+    if t.dim() > 0:
+        if t.is_contiguous():
+            return t.shape[-1]
+        if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+            return t.stride(0)
     raise B200RuntimeError(f"{name} must be contiguous, or a matrix of evenly spaced contiguous rows")
 
 
@@ -286,6 +296,10 @@ def _code(name: str, t: torch.Tensor, codes: Dict[torch.dtype, int]) -> int:
         raise B200LoweringError(f"{name}: unsupported dtype {t.dtype}") from None
 
 
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
             out_dtype: Optional[torch.dtype] = None, group: int = 0, residual_out: Optional[torch.Tensor] = None):
     """``h = x + residual`` and ``y = h / sqrt(mean(h * h) + eps) * w`` over the last axis, in f32 from the unrounded sum; returns
@@ -293,44 +307,48 @@ def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optiona
     ``residual`` or ``x`` itself).  ``out_dtype`` float8_e4m3fn or int8 holds y in 8 bits, ``y * scale`` standing for the result,
     with one f32 scale for each row (``group`` 0) or for each 32, 64, 128 or 256 columns; otherwise y has the type of x and
     scale is None.  x is f32, bf16 or f16; w has its type or f32; x, residual and residual_out may be matrices of spaced rows."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise B200RuntimeError("x must be a CUDA tensor")
-    dev = x.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    index = _first("x", x)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return rmsnorm(x, w, residual, eps, out_dtype, group, residual_out)
-    _on_device(dev, w=w, residual=residual, residual_out=residual_out)
-    rows, cols, xs = _rows("x", x)
-    code = _code("x", x, _FLOAT_CODE)
-    w_code = code
+    stride = _row_stride("x", x)
+    shape, dtype = x.shape, x.dtype
+    cols = shape[-1]
+    code = w_code = _code("x", x, _FLOAT_CODE)
     if w is not None:
+        if not isinstance(w, torch.Tensor) or w.get_device() != index or w.numel() != cols or not w.is_contiguous():
+            raise B200RuntimeError(f"w must be contiguous on cuda:{index} with one element per column ({cols})")
         w_code = _code("w", w, _FLOAT_CODE)
-        if w.numel() != cols or not w.is_contiguous():
-            raise B200RuntimeError(f"w must be contiguous with one element per column ({cols})")
-    rs = hs = 0
+    res_stride = h_stride = 0
     h = residual_out
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise B200RuntimeError("residual must have the shape and dtype of x")
-        rs = _rows("residual", residual)[2]
+        if not isinstance(residual, torch.Tensor) or residual.get_device() != index or residual.shape != shape or residual.dtype != dtype:
+            raise B200RuntimeError(f"residual must be on cuda:{index} with the shape and dtype of x")
+        res_stride = _row_stride("residual", residual)
         if h is None:
-            h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        elif h.shape != x.shape or h.dtype != x.dtype:
-            raise B200RuntimeError("residual_out must have the shape and dtype of x")
-        hs = _rows("residual_out", h)[2]
+            h = torch.empty_like(x) if stride == cols else x.new_empty(shape)
+            h_stride = cols
+        else:
+            if not isinstance(h, torch.Tensor) or h.get_device() != index or h.shape != shape or h.dtype != dtype:
+                raise B200RuntimeError(f"residual_out must be on cuda:{index} with the shape and dtype of x")
+            h_stride = _row_stride("residual_out", h)
     elif h is not None:
         raise B200RuntimeError("residual_out needs a residual")
-    out_dtype = out_dtype or x.dtype
-    held = _HELD_CODE.get(out_dtype)
-    if held is None and out_dtype != x.dtype:
-        raise B200LoweringError(f"rmsnorm: the result is {x.dtype}, float8_e4m3fn or int8, not {out_dtype}")
-    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
     scale = None
-    if held is not None:
-        scale = torch.empty(x.shape[:-1] + ((cols + group - 1) // group if group > 0 else 1,), dtype=torch.float32, device=dev)
-    rc = _lib.load().ib200_rmsnorm(_ptr(x), xs, _ptr(residual), rs, _ptr(w), _ptr(y), _ptr(h), hs, _ptr(scale), code, w_code,
-                                   code if held is None else held, rows, cols, group, float(eps), _stream())
-    _check(rc, "rmsnorm")
+    out_code = code
+    if out_dtype is None or out_dtype == dtype:
+        y = torch.empty_like(x) if stride == cols else x.new_empty(shape)
+    else:
+        out_code = _HELD_CODE.get(out_dtype)
+        if out_code is None:
+            raise B200LoweringError(f"rmsnorm: the result is {dtype}, float8_e4m3fn or int8, not {out_dtype}")
+        y = x.new_empty(shape, dtype=out_dtype)
+        scale = x.new_empty(shape[:-1] + ((cols + group - 1) // group if group > 0 else 1,), dtype=torch.float32)
+    args = _lib.RMSNORM_ARGS.pack(x.data_ptr(), _address(residual), _address(w), y.data_ptr(), _address(h), _address(scale), stride, res_stride, h_stride,
+                                  code, w_code, out_code, shape[:-1].numel(), cols, group, eps)
+    rc = _lib.load().ib200_rmsnorm(args, _stream())
+    if rc:
+        _check(rc, "rmsnorm")
     return y, scale, h
 
 
@@ -342,29 +360,29 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
     uint8 of that shape (default 8).  ``x`` [.., K] is bf16 or f16, or float8_e4m3fn / int8 with ``x_scale`` f32 [.., 1] or
     [.., ceil(K / group)], as ``rmsnorm`` returns them.  ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.
     K is a multiple of 32, the group 32, 64 or 128."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise B200RuntimeError("x must be a CUDA tensor")
-    dev = x.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    index = _first("x", x)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return w4_matmul(x, q, scales, zeros, bias, x_scale, group, out_dtype)
-    _on_device(dev, q=q, scales=scales, zeros=zeros, bias=bias, x_scale=x_scale)
+    _on_device(index, q=q, scales=scales, zeros=zeros, bias=bias, x_scale=x_scale)
     if q is None or scales is None or q.dim() != 2 or group not in (32, 64, 128):
         raise B200LoweringError("w4_matmul: q is a matrix, the group 32, 64 or 128")
-    m, k, xs = _rows("x", x)
-    n = q.shape[0]
+    stride = _row_stride("x", x)
+    front, k, n = x.shape[:-1], x.shape[-1], q.shape[0]
     if k % 32:
         raise B200LoweringError(f"w4_matmul: K = {k} is not a multiple of 32")
     groups = (k + group - 1) // group
-    _dense("q", q, (n, k // 2), torch.uint8)
-    _dense("scales", scales, (n, groups), scales.dtype)
+    if q.dtype is not torch.uint8 or q.shape[1] * 2 != k or not q.is_contiguous():
+        _dense("q", q, (n, k // 2), torch.uint8)
+    if scales.shape != (n, groups) or not scales.is_contiguous():
+        _dense("scales", scales, (n, groups), scales.dtype)
     if zeros is not None:
         _dense("zeros", zeros, (n, groups), torch.uint8)
     x_code = _HELD_CODE.get(x.dtype)
     x_groups = 0
     if x_code is not None:
-        if x_scale is None or x_scale.shape[:-1] != x.shape[:-1] or x_scale.shape[-1] not in (1, groups):
-            raise B200RuntimeError(f"w4_matmul: 8-bit x needs x_scale of shape {tuple(x.shape[:-1])} + (1 or {groups},)")
+        if x_scale is None or x_scale.dim() != x.dim() or x_scale.shape[:-1] != front or x_scale.shape[-1] not in (1, groups):
+            raise B200RuntimeError(f"w4_matmul: 8-bit x needs x_scale of shape {tuple(front)} + (1 or {groups},)")
         _dense("x_scale", x_scale, x_scale.shape, torch.float32)
         x_groups = x_scale.shape[-1]
     else:
@@ -375,40 +393,68 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
         out_dtype = torch.bfloat16 if x_groups else x.dtype
     elif out_dtype not in _FLOAT_CODE:
         raise B200LoweringError(f"w4_matmul: the result is float32, bfloat16 or float16, not {out_dtype}")
-    y = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=dev)
+    y = x.new_empty(front + (n,), dtype=out_dtype)
     if bias is not None:
         _dense("bias", bias, (n,), out_dtype)
-    lib = _lib.load()
-    need = lib.ib200_w4_scratch_bytes(x_code, m, n, k, group)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    rc = lib.ib200_w4_matmul(_ptr(x), xs, _ptr(x_scale), x_groups, _ptr(q), _ptr(scales), _ptr(zeros), _ptr(bias), _ptr(y), x_code,
-                             _code("scales", scales, _FLOAT_CODE), _FLOAT_CODE[out_dtype], m, n, k, group, _ptr(scratch), need,
-                             status_word().data_ptr(), _stream())
-    _check(rc, "w4_matmul")
+    m = front.numel()
+    need = _w4_scratch(x_code, m, n, k, group)
+    scratch = x.new_empty(need, dtype=torch.uint8) if need else None
+    args = _lib.W4_ARGS.pack(x.data_ptr(), _address(x_scale), q.data_ptr(), scales.data_ptr(), _address(zeros), _address(bias), y.data_ptr(), _address(scratch),
+                             0, stride, x_groups, x_code, _code("scales", scales, _FLOAT_CODE), _FLOAT_CODE[out_dtype], m, n, k, group, need)
+    rc = _lib.load().ib200_w4_matmul(args, _stream())
+    if rc:
+        _check(rc, "w4_matmul")
     return y
 
 
-def _cache_extents(x: torch.Tensor, name: str, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new):
-    """Checks of the paged cache's arguments; the extents (pages, heads, block, dim, batch, table_blocks) and the held type's code."""
-    _on_device(x.device, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table, seq_lens=seq_lens, cu_new=cu_new)
+@functools.lru_cache(maxsize=4096)
+def _w4_scratch(*extents: int) -> int:
+    return _lib.load().ib200_w4_scratch_bytes(*extents)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_scratch(*extents: int) -> int:
+    return _lib.load().ib200_attention_kv8_scratch_bytes(*extents)
+
+
+def _cache_extents(index: int, name: str, x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new):
+    """The checked extents of the paged cache's arguments: held type's code, pages, heads, block, dim, batch, table_blocks."""
+    try:
+        pages, heads, block, dim = cache = k_cache.shape
+        batch, table_blocks = block_table.shape
+        f32, i32 = torch.float32, torch.int32
+        good = (x.dim() == 3 and x.shape[2] == dim and x.stride(2) == 1 and v_cache.shape == cache and k_scale.shape == (pages, heads)
+                and v_scale.shape == (pages, heads) and seq_lens.shape == (batch,)
+                and v_cache.dtype is k_cache.dtype and k_scale.dtype is f32 and v_scale.dtype is f32 and block_table.dtype is i32 and seq_lens.dtype is i32
+                and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()
+                and block_table.is_contiguous() and seq_lens.is_contiguous()
+                and k_cache.get_device() == index and v_cache.get_device() == index and k_scale.get_device() == index and v_scale.get_device() == index
+                and block_table.get_device() == index and seq_lens.get_device() == index
+                and (cu_new is None or (cu_new.shape == (batch + 1,) and cu_new.dtype is i32 and cu_new.is_contiguous() and cu_new.get_device() == index)))
+    except (AttributeError, ValueError):
+        good = False
+    if not good:
+        _name_the_fault(index, name, x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
+    return _code("k_cache", k_cache, _HELD_CODE), pages, heads, block, dim, batch, table_blocks
+
+
+def _name_the_fault(index: int, name: str, x, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new) -> None:
+    _on_device(index, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table, seq_lens=seq_lens, cu_new=cu_new)
     if any(t is None for t in (k_cache, v_cache, k_scale, v_scale, block_table, seq_lens)):
         raise B200RuntimeError("the caches, their scales, block_table and seq_lens are needed")
     if k_cache.dim() != 4 or block_table.dim() != 2 or x.dim() != 3:
         raise B200RuntimeError(f"{name} is [tokens, heads, dim], the caches [pages, heads, block, dim], block_table [sequences, blocks]")
-    held = _code("k_cache", k_cache, _HELD_CODE)
-    pages, heads, block, dim = k_cache.shape
-    batch, table_blocks = block_table.shape
+    pages, heads = k_cache.shape[:2]
+    batch = block_table.shape[0]
     _dense("k_cache", k_cache, k_cache.shape, k_cache.dtype)
     _dense("v_cache", v_cache, k_cache.shape, k_cache.dtype)
     _dense("k_scale", k_scale, (pages, heads), torch.float32)
     _dense("v_scale", v_scale, (pages, heads), torch.float32)
-    _dense("block_table", block_table, (batch, table_blocks), torch.int32)
+    _dense("block_table", block_table, block_table.shape, torch.int32)
     _dense("seq_lens", seq_lens, (batch,), torch.int32)
     if cu_new is not None:
         _dense("cu_new", cu_new, (batch + 1,), torch.int32)
-    if x.shape[2] != dim or (dim > 1 and x.stride(2) != 1):
-        raise B200RuntimeError(f"{name} must have the cache's width {dim} as its last, adjacent axis")
-    return held, pages, heads, block, dim, batch, table_blocks
+    raise B200RuntimeError(f"{name} must have the cache's width {k_cache.shape[3]} as its last, adjacent axis")
 
 
 def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -419,20 +465,22 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     new tokens, ``cu_new`` [sequences + 1] int32 where each sequence's new tokens lie (None: the same number for each).  A scale
     grows with its block's largest value, and the values held before are rounded again; slots behind the end, tokens behind
     ``cu_new[-1]``, and pages or tokens outside the cache and the table are left alone.  No two sequences may append to one page."""
-    if not isinstance(k, torch.Tensor) or not k.is_cuda:
-        raise B200RuntimeError("k must be a CUDA tensor")
-    dev = k.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    index = _first("k", k)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
-    held, pages, heads, block, dim, batch, table_blocks = _cache_extents(k, "k", k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
-    _on_device(dev, v=v)
-    if v is None or v.shape != k.shape or v.dtype != k.dtype or k.shape[1] != heads or (dim > 1 and v.stride(2) != 1):
-        raise B200RuntimeError(f"k and v must be [tokens, {heads}, {dim}] tensors of one dtype with adjacent last axes")
-    rc = _lib.load().ib200_kv8_append(_ptr(k), k.stride(0), k.stride(1), _ptr(v), v.stride(0), v.stride(1), _ptr(k_cache), _ptr(v_cache),
-                                      _ptr(k_scale), _ptr(v_scale), _ptr(block_table), _ptr(seq_lens), _ptr(cu_new),
-                                      _code("k", k, _HALF_CODE), held, k.shape[0], batch, heads, dim, pages, block, table_blocks, _stream())
-    _check(rc, "kv8_append")
+    held, pages, heads, block, dim, batch, table_blocks = _cache_extents(index, "k", k, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
+    if (not isinstance(v, torch.Tensor) or v.get_device() != index or v.shape != k.shape or v.dtype != k.dtype or k.shape[1] != heads
+            or v.stride(2) != 1):
+        raise B200RuntimeError(f"k and v must be [tokens, {heads}, {dim}] tensors of one dtype on cuda:{index} with adjacent last axes")
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    args = _lib.KV8_APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                     block_table.data_ptr(), seq_lens.data_ptr(), _address(cu_new), k_token, k_head, v_token, v_head,
+                                     _code("k", k, _HALF_CODE), held, k.shape[0], batch, heads, dim, pages, block, table_blocks)
+    rc = _lib.load().ib200_kv8_append(args, _stream())
+    if rc:
+        _check(rc, "kv8_append")
 
 
 def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -444,26 +492,26 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     head.  Returns ``o`` of q's shape and dtype (``out``, if given), with ``return_lse`` also the f32 [tokens, query heads] logs of
     the softmax's denominators.  Rows without keys are 0 (lse -inf); rows that need a page outside the cache or a token outside the
     table are NaN; tokens behind ``cu_new[-1]`` are not written."""
-    if not isinstance(q, torch.Tensor) or not q.is_cuda:
-        raise B200RuntimeError("q must be a CUDA tensor")
-    dev = q.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
+    index = _first("q", q)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
             return attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new, scale, window, return_lse, out)
-    held, pages, heads, block, dim, batch, table_blocks = _cache_extents(q, "q", k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
-    tokens, q_heads = q.shape[0], q.shape[1]
+    held, pages, heads, block, dim, batch, table_blocks = _cache_extents(index, "q", q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
+    tokens, q_heads, _ = shape = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     else:
-        _on_device(dev, out=out)
-        _dense("out", out, q.shape, q.dtype)
-    lse = torch.empty((tokens, q_heads), dtype=torch.float32, device=dev) if return_lse else None
-    lib = _lib.load()
-    need = lib.ib200_attention_kv8_scratch_bytes(tokens, batch, q_heads, heads, dim, block, table_blocks)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    rc = lib.ib200_attention_kv8(_ptr(q), q.stride(0), q.stride(1), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
-                                 _ptr(block_table), _ptr(seq_lens), _ptr(cu_new), _ptr(out), _ptr(lse), _code("q", q, _HALF_CODE), held,
-                                 tokens, batch, q_heads, heads, dim, pages, block, table_blocks, window,
-                                 dim ** -0.5 if scale is None else float(scale), _ptr(scratch), need, _stream())
-    _check(rc, "attention_kv8")
+        _on_device(index, out=out)
+        _dense("out", out, shape, q.dtype)
+    lse = q.new_empty((tokens, q_heads), dtype=torch.float32) if return_lse else None
+    need = _attention_scratch(tokens, batch, q_heads, heads, dim, block, table_blocks)
+    scratch = q.new_empty(need, dtype=torch.uint8) if need else None
+    q_token, q_head, _ = q.stride()
+    args = _lib.ATTENTION_KV8_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
+                                        seq_lens.data_ptr(), _address(cu_new), out.data_ptr(), _address(lse), _address(scratch), q_token, q_head,
+                                        _code("q", q, _HALF_CODE), held, tokens, batch, q_heads, heads, dim, pages, block, table_blocks, window, need,
+                                        dim ** -0.5 if scale is None else scale)
+    rc = _lib.load().ib200_attention_kv8(args, _stream())
+    if rc:
+        _check(rc, "attention_kv8")
     return (out, lse) if return_lse else out

@@ -14,44 +14,47 @@ ODD = ctypes.c_void_p(0x7F0000000008)
 BIG = 1 << 62
 
 
+def _call(entry, layout, pointers, fields, changes):
+    """The entry with these arguments, `changes` made."""
+    a = {**{p: P for p in pointers.split()}, **fields}
+    assert set(changes) <= set(a)
+    a.update(changes)
+    return getattr(_lib.load(), entry)(layout.pack(*(v or 0 if v is None or isinstance(v, (int, float)) else v.value for v in a.values())), None)
+
+
 def _norm(**k):
-    a = dict(x=P, xs=64, res=P, rs=64, w=P, y=P, h=P, hs=64, scale=P, dtype=_lib.BF16, wt=_lib.BF16, out=_lib.E4M3, rows=4, cols=64, group=32, eps=1e-6)
-    a.update(k)
-    return _lib.load().ib200_rmsnorm(*a.values(), None)
+    return _call("ib200_rmsnorm", _lib.RMSNORM_ARGS, "x res w y h scale",
+                 dict(xs=64, rs=64, hs=64, dtype=_lib.BF16, wt=_lib.BF16, out=_lib.E4M3, rows=4, cols=64, group=32, eps=1e-6), k)
 
 
 def _w4(**k):
-    a = dict(x=P, xs=64, xsc=None, xg=0, q=P, s=P, z=P, bias=P, y=P, xt=_lib.BF16, st=_lib.BF16, out=_lib.BF16, m=4, n=8, k=64, group=32, scratch=None,
-             bytes=0, status=None)
-    a.update(k)
-    return _lib.load().ib200_w4_matmul(*a.values(), None)
+    return _call("ib200_w4_matmul", _lib.W4_ARGS, "x xsc q s z bias y scratch status",
+                 dict(xs=64, xg=0, xt=_lib.BF16, st=_lib.BF16, out=_lib.BF16, m=4, n=8, k=64, group=32, bytes=1 << 40), k)
 
 
 def _append(**k):
-    a = dict(k=P, kt=128, kh=64, v=P, vt=128, vh=64, kc=P, vc=P, ks=P, vs=P, table=P, lens=P, cu=None, dtype=_lib.BF16, held=_lib.I8, tokens=4, batch=2, heads=2,
-             dim=64, pages=9, block=16, blocks=4)
-    a.update(k)
-    return _lib.load().ib200_kv8_append(*a.values(), None)
+    return _call("ib200_kv8_append", _lib.KV8_APPEND_ARGS, "k v kc vc ks vs table lens cu",
+                 dict(kt=128, kh=64, vt=128, vh=64, dtype=_lib.BF16, held=_lib.I8, tokens=4, batch=2, heads=2, dim=64, pages=9, block=16, blocks=4),
+                 {"cu": None, **k})
 
 
 def _attention(**k):
-    a = dict(q=P, qt=256, qh=64, kc=P, vc=P, ks=P, vs=P, table=P, lens=P, cu=None, o=P, lse=P, dtype=_lib.BF16, held=_lib.I8, tokens=4, batch=2, qheads=4, heads=2,
-             dim=64, pages=9, block=16, blocks=4, window=0, scale=0.1, scratch=P, bytes=1 << 40)
-    a.update(k)
-    return _lib.load().ib200_attention_kv8(*a.values(), None)
+    return _call("ib200_attention_kv8", _lib.ATTENTION_KV8_ARGS, "q kc vc ks vs table lens cu o lse scratch",
+                 dict(qt=256, qh=64, dtype=_lib.BF16, held=_lib.I8, tokens=4, batch=2, qheads=4, heads=2, dim=64, pages=9, block=16, blocks=4, window=0,
+                      bytes=1 << 40, scale=0.1), {"cu": None, **k})
 
 
 @pytest.mark.parametrize("call,bad", [
     (_norm, dict(rows=-1)), (_norm, dict(cols=-1)), (_norm, dict(rows=BIG)), (_norm, dict(rows=1 << 30, cols=1 << 30)), (_norm, dict(x=None)), (_norm, dict(y=None)),
     (_norm, dict(scale=None)), (_norm, dict(res=None)), (_norm, dict(xs=63)), (_norm, dict(rs=1)), (_norm, dict(hs=-64)), (_norm, dict(xs=BIG)),
     (_w4, dict(m=-1)), (_w4, dict(n=-1)), (_w4, dict(k=-32)), (_w4, dict(n=1 << 30, k=1 << 30)), (_w4, dict(x=None)), (_w4, dict(q=None)), (_w4, dict(s=None)), (_w4, dict(y=None)),
-    (_w4, dict(q=ODD)), (_w4, dict(xs=63)), (_w4, dict(xg=1)), (_w4, dict(xt=_lib.I8)), (_w4, dict(xt=_lib.I8, xg=3, xsc=P)), (_w4, dict(xt=_lib.I8, xg=1)),
+    (_w4, dict(q=ODD)), (_w4, dict(xs=63)), (_w4, dict(xg=1)), (_w4, dict(xt=_lib.I8)), (_w4, dict(xt=_lib.I8, xg=3, xsc=P)), (_w4, dict(xt=_lib.I8, xg=1, xsc=None)),
     (_w4, dict(scratch=ODD)),
     (_append, dict(tokens=-1)), (_append, dict(batch=-1)), (_append, dict(pages=-1)), (_append, dict(tokens=3)), (_append, dict(k=None)), (_append, dict(vs=None)),
     (_append, dict(table=None)), (_append, dict(lens=None)), (_append, dict(kc=ODD)), (_append, dict(pages=1 << 31 - 1, heads=1 << 15, block=1024)), (_append, dict(blocks=1 << 40)),
     (_attention, dict(tokens=-1)), (_attention, dict(blocks=-1)), (_attention, dict(tokens=3)), (_attention, dict(qheads=3)), (_attention, dict(qheads=-2)), (_attention, dict(heads=0)),
     (_attention, dict(window=-1)), (_attention, dict(q=None)), (_attention, dict(o=None)), (_attention, dict(ks=None)), (_attention, dict(table=None)),
-    (_attention, dict(vc=ODD)), (_attention, dict(scratch=ODD)),
+    (_attention, dict(vc=ODD)), (_attention, dict(scratch=ODD)), (_attention, dict(o=ctypes.c_void_p(0x7F0000000004))),
 ])
 def test_arguments_that_cannot_be_meant_are_invalid(call, bad):
     assert call(**bad) == _lib.ERR_INVALID, (bad, _lib.last_error())
@@ -67,6 +70,13 @@ def test_arguments_that_cannot_be_meant_are_invalid(call, bad):
 ])
 def test_what_the_kernels_do_not_cover_is_unsupported(call, bad):
     assert call(**bad) == _lib.ERR_UNSUPPORTED, (bad, _lib.last_error())
+
+
+def test_scratch_that_is_too_small_is_refused_and_no_arguments_are_invalid():
+    need = _lib.load().ib200_attention_kv8_scratch_bytes(4, 2, 4, 2, 64, 16, 4)
+    assert need > 0 and _attention(bytes=need - 1) == _lib.ERR_BUFFER and _attention(scratch=None) == _lib.ERR_BUFFER
+    for entry in ("ib200_rmsnorm", "ib200_w4_matmul", "ib200_kv8_append", "ib200_attention_kv8"):
+        assert getattr(_lib.load(), entry)(None, None) == _lib.ERR_INVALID
 
 
 def test_empty_work_launches_nothing():
