@@ -85,44 +85,53 @@ template <bool BF> __device__ __forceinline__ void weights_of(uint32_t w, const 
     }
   }
 }
-// 8 adjacent x as the pairs above; 8-bit values become f16, which is exact
-__device__ __forceinline__ uint4 x_chunk(const W4Args& a, int row, int k) {
-  if (row >= a.m || k >= a.k) return make_uint4(0, 0, 0, 0);
+// 8 adjacent x as they lie in memory.  Loading and converting are apart: a converted value makes its warp wait for the load.
+__device__ __forceinline__ uint4 x_raw(const W4Args& a, int row, int k) {
+  uint4 r = make_uint4(0, 0, 0, 0);
+  if (row >= a.m || k >= a.k) return r;
   const int64_t at = (int64_t)row * a.x_stride + k;
   if (a.x_type == IB200_BF16 || a.x_type == IB200_F16) {
     const uint16_t* p = static_cast<const uint16_t*>(a.x) + at;
-    uint4 r;
+    if (a.x_vec) return *reinterpret_cast<const uint4*>(p);
+    r.x = p[0] | (uint32_t)p[1] << 16, r.y = p[2] | (uint32_t)p[3] << 16, r.z = p[4] | (uint32_t)p[5] << 16, r.w = p[6] | (uint32_t)p[7] << 16;
+  } else {
+    const uint8_t* p = static_cast<const uint8_t*>(a.x) + at;
     if (a.x_vec) {
-      r = *reinterpret_cast<const uint4*>(p);
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      r.x = v.x, r.y = v.y;
     } else {
-      r.x = p[0] | (uint32_t)p[1] << 16, r.y = p[2] | (uint32_t)p[3] << 16, r.z = p[4] | (uint32_t)p[5] << 16, r.w = p[6] | (uint32_t)p[7] << 16;
+      r.x = p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
+      r.y = p[4] | (uint32_t)p[5] << 8 | (uint32_t)p[6] << 16 | (uint32_t)p[7] << 24;
     }
-    return make_uint4(__byte_perm(r.x, r.z, 0x5410), __byte_perm(r.x, r.z, 0x7632), __byte_perm(r.y, r.w, 0x5410), __byte_perm(r.y, r.w, 0x7632));
-  }
-  const uint8_t* p = static_cast<const uint8_t*>(a.x) + at;
-  uint32_t lo, hi;
-  if (a.x_vec) {
-    const uint2 r = *reinterpret_cast<const uint2*>(p);
-    lo = r.x, hi = r.y;
-  } else {
-    lo = p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
-    hi = p[4] | (uint32_t)p[5] << 8 | (uint32_t)p[6] << 16 | (uint32_t)p[7] << 24;
-  }
-  uint4 r;
-  const uint32_t a01 = __byte_perm(lo, hi, 0x5140), a23 = __byte_perm(lo, hi, 0x7362);  // bytes 0 4 1 5, 2 6 3 7
-  if (a.x_type == IB200_E4M3) {
-    widen<HELD_E4M3>(a01, r.x, r.y);
-    widen<HELD_E4M3>(a23, r.z, r.w);
-  } else {
-    widen<HELD_I8>(a01, r.x, r.y);
-    widen<HELD_I8>(a23, r.z, r.w);
   }
   return r;
+}
+// as the pairs above; 8-bit values become f16, which is exact
+__device__ __forceinline__ uint4 x_pairs(const uint4& r, int type) {
+  if (type == IB200_BF16 || type == IB200_F16)
+    return make_uint4(__byte_perm(r.x, r.z, 0x5410), __byte_perm(r.x, r.z, 0x7632), __byte_perm(r.y, r.w, 0x5410), __byte_perm(r.y, r.w, 0x7632));
+  uint4 v;
+  const uint32_t a01 = __byte_perm(r.x, r.y, 0x5140), a23 = __byte_perm(r.x, r.y, 0x7362);  // bytes 0 4 1 5, 2 6 3 7
+  if (type == IB200_E4M3) {
+    widen<HELD_E4M3>(a01, v.x, v.y);
+    widen<HELD_E4M3>(a23, v.z, v.w);
+  } else {
+    widen<HELD_I8>(a01, v.x, v.y);
+    widen<HELD_I8>(a23, v.z, v.w);
+  }
+  return v;
+}
+__device__ __forceinline__ uint32_t raw_of(const void* p, int64_t i, int type) {
+  return type == IB200_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float value_of(uint32_t raw, int type) {
+  if (type == IB200_F16) return __half2float(__ushort_as_half((unsigned short)raw));
+  return __uint_as_float(type == IB200_BF16 ? raw << 16 : raw);
 }
 
 template <bool BF, int NT, int G>
 __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) {
-  constexpr int GROUPS = kStageK / G, WORDS = G / 32, XBYTES = NT * 8 * kStageK * 2;  // groups of a stage, words of a thread in a group
+  constexpr int GROUPS = kStageK / G, WORDS = G / 32, XBYTES = NT * 8 * (kStageK * 2 + GROUPS * 4);  // groups of a stage, words of a thread in a group
   constexpr int HOLD = (GROUPS + 3) / 4;                                               // scales that a lane of a quad holds for a row
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* xbuf = smem + kStages * kStageBytes;
@@ -147,22 +156,27 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) 
     return (((k / G * WORDS + word) * NT + row / 8) * 8 + row % 8) * 4 + th;
   };
   uint4 xr[NT];
+  float xsr = 1.0f;  // a scale of x, behind the stage's x: [group][row]
   auto x_load = [&](int s) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int idx = i * kThreads + threadIdx.x;
-      xr[i] = x_chunk(a, m0 + idx / (kStageK / 8), s * kStageK + idx % (kStageK / 8) * 8);
+      xr[i] = x_raw(a, m0 + idx / (kStageK / 8), s * kStageK + idx % (kStageK / 8) * 8);
+    }
+    if (a.xs_groups > 1 && threadIdx.x < GROUPS * NT * 8) {
+      const int m = m0 + threadIdx.x % (NT * 8), grp = s * GROUPS + threadIdx.x / (NT * 8);
+      xsr = m < a.m && grp < a.groups ? a.xs[(int64_t)m * a.groups + grp] : 0.0f;
     }
   };
   auto x_store = [&](int s) {
     uint4* to = reinterpret_cast<uint4*>(xbuf + ((s - s0) & 1) * XBYTES);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) to[x_place(i * kThreads + threadIdx.x)] = xr[i];
+    for (int i = 0; i < NT; ++i) to[x_place(i * kThreads + threadIdx.x)] = x_pairs(xr[i], a.x_type);
+    if (threadIdx.x < GROUPS * NT * 8) reinterpret_cast<float*>(to + NT * 8 * kStageK / 8)[threadIdx.x] = xsr;
   };
   // scales and zero points of the thread's two rows (16 * warp + g, + 8): lane t of a quad holds groups t, t + 4 of the stage
   const int row_a = n0 + warp * 16 + g;
-  float sc[2][HOLD];
-  uint32_t zp[2][HOLD];
+  uint32_t sc[2][HOLD], zp[2][HOLD];
   auto scale_load = [&](int s) {
 #pragma unroll
     for (int r = 0; r < 2; ++r)
@@ -171,8 +185,8 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) 
         const int row = row_a + 8 * r, in = h * 4 + t, grp = s * GROUPS + in;
         const bool take = row < a.n && in < GROUPS && grp < a.groups;
         const int64_t at = (int64_t)row * a.groups + grp;
-        sc[r][h] = take ? float_of(a.s, at, a.s_type) : 0.0f;
-        zp[r][h] = take && a.z ? a.z[at] & 15u : 8u;
+        sc[r][h] = take ? raw_of(a.s, at, a.s_type) : 0u;
+        zp[r][h] = take && a.z ? a.z[at] : 8u;
       }
   };
 
@@ -180,15 +194,17 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) 
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.0f;
 
+  if (s0 < s1) {
+    x_load(s0);
+    scale_load(s0);
+  }
   for (int i = 0; i < kStages - 1; ++i) {
     if (s0 + i < s1) issue(s0 + i);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   if (s0 < s1) {
-    x_load(s0);
     x_store(s0);
     if (s0 + 1 < s1) x_load(s0 + 1);
-    scale_load(s0);
   }
   for (int s = s0; s < s1; ++s) {
     float scn[2][HOLD];
@@ -196,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) 
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int h = 0; h < HOLD; ++h) scn[r][h] = sc[r][h], zpn[r][h] = zp[r][h];
+      for (int h = 0; h < HOLD; ++h) scn[r][h] = value_of(sc[r][h], a.s_type), zpn[r][h] = zp[r][h] & 15u;
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
     if (s + kStages - 1 < s1) issue(s + kStages - 1);
@@ -254,9 +270,8 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) 
       for (int nt = 0; nt < NT; ++nt) {
         float f0 = 1.0f, f1 = 1.0f;
         if (a.xs_groups > 1) {
-          const int m = m0 + nt * 8 + 2 * t, at = s * GROUPS + grp;
-          f0 = m < a.m && at < a.groups ? a.xs[(int64_t)m * a.groups + at] : 0.0f;
-          f1 = m + 1 < a.m && at < a.groups ? a.xs[(int64_t)(m + 1) * a.groups + at] : 0.0f;
+          const float2 f = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(xst - lane + NT * 8 * kStageK / 8) + grp * NT * 8 + nt * 8 + 2 * t);
+          f0 = f.x, f1 = f.y;
         }
         sum[nt][0] = fmaf(acc[nt][0], sa * f0, sum[nt][0]);
         sum[nt][1] = fmaf(acc[nt][1], sa * f1, sum[nt][1]);
@@ -293,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a) 
 
 template <bool BF, int NT, int G> int run_stream(W4Args a, cudaStream_t s) {
   auto* kern = w4_stream_kernel<BF, NT, G>;
-  constexpr int SMEM = kStages * kStageBytes + 2 * NT * 8 * kStageK * 2;
+  constexpr int SMEM = kStages * kStageBytes + 2 * NT * 8 * (kStageK * 2 + kStageK / G * 4);
   IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
   // K is split until the CTAs fill two per SM: one wave, all of it loading from the start
   const int tiles = (a.n + kRows - 1) / kRows, stages = (a.k + kStageK - 1) / kStageK, mt = (a.m + NT * 8 - 1) / (NT * 8);
