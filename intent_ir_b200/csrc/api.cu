@@ -158,7 +158,7 @@ int ib200_kv8_append(const ib200_kv8_append_args* a, void* stream) {
   if (!a) return fail(IB200_ERR_INVALID, "kv8_append: no arguments");
   Kv8Append k{a->k, a->v, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, static_cast<uint8_t*>(a->k_cache),
               static_cast<uint8_t*>(a->v_cache), a->k_scale, a->v_scale, a->table, a->lens, a->cu, a->pages, a->heads, a->block, a->dim, a->batch,
-              a->table_blocks, a->tokens, 0};
+              a->table_blocks, a->tokens, 0, 0};
   return launch_kv8_append(k, code(a->dtype), code(a->held), static_cast<cudaStream_t>(stream));
 }
 

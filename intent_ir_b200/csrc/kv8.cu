@@ -11,42 +11,120 @@ namespace ib200 {
 namespace {
 
 // ---- append -----------------------------------------------------------------------------------------
-// One CTA per (new token, head, K or V); the CTA of a block's first new token does the whole block, the others leave at once.
+// A unit is the new tokens of one block: for a head, one warp (few tokens) or CTA for the keys and one for the values.
 //   s' = max(s, max|new| / Q), s = 0 for a block that begins here; held values become round(q * s / s') where s' > s, new ones round(x / s')
-// Divisions are IEEE divisions: the held values then depend on nothing but their definition.
-template <typename T, int HELD, int THREADS>
-__global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a) {
+// Divisions are IEEE divisions: the held values then depend on nothing but their definition.  The new values are read once
+// into registers (up to KEEP vectors of 8 a thread, blocks of 64 tokens of 128; more are read again) and written 8 bytes at a time.
+constexpr int KEEP = 8;
+template <typename T> __device__ __forceinline__ uint4 read_new(const T* p, bool vec) {
+  if (vec) return __ldcs(reinterpret_cast<const uint4*>(p));
+  const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+  return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+}
+template <typename T> __device__ __forceinline__ void floats_of(const uint4& r, float (&v)[8]) {
+  const T* p = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
+}
+template <int HELD> __device__ __forceinline__ uint2 hold_quotients(const float (&v)[8], float div) {
+  return make_uint2(hold4<HELD>(v[0] / div, v[1] / div, v[2] / div, v[3] / div), hold4<HELD>(v[4] / div, v[5] / div, v[6] / div, v[7] / div));
+}
+
+template <typename T, int HELD, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, const int vec) {
+  constexpr int PER = D / 8;  // vectors of a token
   __shared__ float slots[32];
-  const int t = blockIdx.x, head = blockIdx.y;
-  int b, first, count;
-  if (!find_sequence(a.cu, a.batch, a.each, t, b, first, count)) return;
-  const int64_t start = (int64_t)a.lens[b] - count, pos = start + (t - first);
-  if (pos < 0) return;
-  const int64_t blk = pos / a.block;
-  const int slot = (int)(pos - blk * a.block);
-  if (!(t == first || slot == 0 || pos == 0) || blk >= a.table_blocks) return;
+  const int head = blockIdx.y, tid = threadIdx.x, block = (int)a.block;
+  // Unit u: with offsets, sequence b has the units from cu[b] / block + 2 b, which leaves room for (its new tokens) / block + 2; without,
+  // the same number for each.
+  const int64_t u = blockIdx.x;
+  int b, first, count, j;
+  if (a.cu) {
+    int lo = 0, hi = (int)a.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu[mid] / block + 2 * (int64_t)mid <= u) lo = mid; else hi = mid;
+    }
+    b = lo;
+    first = a.cu[b];
+    count = a.cu[b + 1] - first;
+    j = (int)(u - (first / block + 2 * (int64_t)b));
+    if (first < 0 || count <= 0 || j < 0 || (int64_t)first + count > a.tokens) return;
+  } else {
+    b = (int)(u / a.per);
+    j = (int)(u - (int64_t)b * a.per);
+    first = b * a.each;
+    count = a.each;
+  }
+  const int64_t start = (int64_t)a.lens[b] - count, end = start + count;  // places of the new tokens
+  const int64_t blk = max((int64_t)0, start) / block + j;
+  const int64_t from = max(max((int64_t)0, start), blk * block), to = min(end, (blk + 1) * block);
+  if (from >= to || blk >= a.table_blocks) return;
   const int page = a.table[(int64_t)b * a.table_blocks + blk];
   if ((unsigned)page >= (unsigned)a.pages) return;
-  const int fresh = (int)min(min((int64_t)first + count, a.tokens) - t, (int64_t)(a.block - slot));  // new tokens of this block
   const bool is_v = blockIdx.z;
-  const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (int64_t)t * (is_v ? a.v_token : a.k_token) + (int64_t)head * (is_v ? a.v_head : a.k_head);
+  const int slot = (int)(from - blk * block), fresh = (int)(to - from), vectors = fresh * PER;
   const int64_t x_token = is_v ? a.v_token : a.k_token;
+  const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (first + (from - start)) * x_token + (int64_t)head * (is_v ? a.v_head : a.k_head);
   const int64_t at = (int64_t)page * a.heads + head;
-  uint8_t* cache = (is_v ? a.v_cache : a.k_cache) + at * a.block * a.dim;
+  uint8_t* cache = (is_v ? a.v_cache : a.k_cache) + at * block * D;
   float* scale = (is_v ? a.v_scale : a.k_scale) + at;
-  float top = 0.0f;
-  for (int i = threadIdx.x; i < fresh * a.dim; i += THREADS) top = max_nan(top, fabsf(to_f32(x[(i / a.dim) * x_token + i % a.dim])));
-  top = block_reduce<MaxOp>(top, slots);
   const float before = slot ? *scale : 0.0f;
-  const float after = max_nan(before, top / held_top<HELD>());
-  const bool grown = !(after == before);
-  const float div = after == 0.0f ? 1.0f : after;
-  if (grown)
-    for (int i = threadIdx.x; i < slot * a.dim; i += THREADS) cache[i] = (uint8_t)hold1<HELD>(held_value<HELD>(cache[i]) * before / div);
-  for (int i = threadIdx.x; i < fresh * a.dim; i += THREADS)
-    cache[slot * a.dim + i] = (uint8_t)hold1<HELD>(to_f32(x[(i / a.dim) * x_token + i % a.dim]) / div);
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) *scale = after;
+
+  auto source = [&](int i) { return x + (i / PER) * x_token + i % PER * 8; };
+  uint4 keep[KEEP];
+  float top = 0.0f;
+  auto enter = [&](const uint4& r) {
+    float v[8];
+    floats_of<T>(r, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(v[e]));
+  };
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+    if (tid + k * THREADS < vectors) keep[k] = read_new(source(tid + k * THREADS), vec);
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+    if (tid + k * THREADS < vectors) enter(keep[k]);
+  for (int i = tid + KEEP * THREADS; i < vectors; i += THREADS) enter(read_new(source(i), vec));
+  top = THREADS == 32 ? warp_reduce<MaxOp>(top) : block_reduce<MaxOp>(top, slots);  // (the barrier: every thread has read the old scale)
+  const float after = max_nan(before, top / held_top<HELD>()), div = after == 0.0f ? 1.0f : after;
+  if (THREADS == 32) __syncwarp();
+  if (tid == 0) *scale = after;
+  if (!(after == before)) {
+    for (int i = tid; i < slot * PER; i += THREADS) {
+      const uint2 old = *reinterpret_cast<const uint2*>(cache + i * 8);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = held_value<HELD>((uint8_t)((e < 4 ? old.x : old.y) >> (8 * (e & 3)))) * before;
+      *reinterpret_cast<uint2*>(cache + i * 8) = hold_quotients<HELD>(v, div);
+    }
+  }
+  uint8_t* out = cache + slot * D;
+  auto leave = [&](int i, const uint4& r) {
+    float v[8];
+    floats_of<T>(r, v);
+    *reinterpret_cast<uint2*>(out + i * 8) = hold_quotients<HELD>(v, div);
+  };
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+    if (tid + k * THREADS < vectors) leave(tid + k * THREADS, keep[k]);
+  for (int i = tid + KEEP * THREADS; i < vectors; i += THREADS) leave(i, read_new(source(i), vec));
+}
+
+template <typename T, int HELD, int D> int run_append(const Kv8Append& a, cudaStream_t s) {
+  const int64_t units = a.cu ? a.tokens / a.block + 2 * a.batch + 1 : a.batch * a.per;
+  if (units > INT32_MAX) return fail(IB200_ERR_UNSUPPORTED, "kv8_append: too many blocks");
+  const int vec = aligned16(a.k) && aligned16(a.v) && a.k_token % 8 == 0 && a.k_head % 8 == 0 && a.v_token % 8 == 0 && a.v_head % 8 == 0;
+  const dim3 grid((unsigned)units, (unsigned)a.heads, 2);
+  // a warp holds 16 tokens of 128 in its registers; where a block takes more, a CTA
+  const int64_t expect = (a.tokens + a.batch - 1) / a.batch;
+  if ((expect < a.block ? expect : a.block) * D <= 32 * KEEP * 8) append_kernel<T, HELD, D, 32><<<grid, 32, 0, s>>>(a, vec);
+  else append_kernel<T, HELD, D, 128><<<grid, 128, 0, s>>>(a, vec);
+  return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "kv8_append launch");
+}
+template <typename T, int HELD> int run_append_dim(const Kv8Append& a, cudaStream_t s) {
+  return a.dim == 128 ? run_append<T, HELD, 128>(a, s) : run_append<T, HELD, 64>(a, s);
 }
 
 }  // namespace
@@ -72,15 +150,9 @@ int launch_kv8_append(Kv8Append& a, int dtype, int held, cudaStream_t s) {
   if (!a.k || !a.v || !a.k_cache || !a.v_cache || !a.k_scale || !a.v_scale || !a.table || !a.lens) return fail(IB200_ERR_INVALID, "kv8_append: null operand");
   if (!aligned16(a.k_cache) || !aligned16(a.v_cache)) return fail(IB200_ERR_INVALID, "kv8_append: caches must be 16-byte aligned");
   a.each = (int)(a.tokens / a.batch);
-  const dim3 grid((unsigned)a.tokens, (unsigned)a.heads, 2);
-  if (dtype == IB200_BF16) {
-    if (held == IB200_E4M3) append_kernel<__nv_bfloat16, HELD_E4M3, 128><<<grid, 128, 0, s>>>(a);
-    else append_kernel<__nv_bfloat16, HELD_I8, 128><<<grid, 128, 0, s>>>(a);
-  } else {
-    if (held == IB200_E4M3) append_kernel<__half, HELD_E4M3, 128><<<grid, 128, 0, s>>>(a);
-    else append_kernel<__half, HELD_I8, 128><<<grid, 128, 0, s>>>(a);
-  }
-  return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "kv8_append launch");
+  a.per = (int)((a.each + a.block - 2) / a.block + 1);
+  if (dtype == IB200_BF16) return held == IB200_E4M3 ? run_append_dim<__nv_bfloat16, HELD_E4M3>(a, s) : run_append_dim<__nv_bfloat16, HELD_I8>(a, s);
+  return held == IB200_E4M3 ? run_append_dim<__half, HELD_E4M3>(a, s) : run_append_dim<__half, HELD_I8>(a, s);
 }
 
 }  // namespace ib200

@@ -12,7 +12,7 @@ struct Kv8Append {
   float *k_scale, *v_scale;
   const int *table, *lens, *cu;
   int64_t pages, heads, block, dim, batch, table_blocks, tokens;
-  int each;  // new tokens per sequence without cu; filled by the launcher
+  int each, per;  // without cu: new tokens per sequence, blocks that they can touch; filled by the launcher
 };
 
 struct Kv8Attention {

@@ -15,6 +15,7 @@ struct RmsArgs {
   int64_t x_stride, res_stride, h_stride;
   int64_t rows, cols, groups;  // groups: scales per row
   int group;                   // columns per scale, 0: the whole row
+  int out_type, wide_w;        // IB200_E4M3, IB200_I8 or the rows' type; whether w is f32
   float eps;
 };
 
@@ -45,12 +46,215 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const float (
   }
 }
 
-// One CTA per row, three passes over it (sum of squares, scales, values); any width.
-template <typename T, typename TW, int HELD, int THREADS>
+template <typename T> __device__ __forceinline__ void load_w8(const RmsArgs& a, int64_t at, float (&v)[VE], bool vec, int left) {
+  if (a.wide_w) load8(static_cast<const float*>(a.w) + at, v, vec, left);
+  else load8(static_cast<const T*>(a.w) + at, v, vec, left);
+}
+template <typename T> __device__ __forceinline__ float load_w(const RmsArgs& a, int64_t at) {
+  return a.wide_w ? static_cast<const float*>(a.w)[at] : to_f32(static_cast<const T*>(a.w)[at]);
+}
+__device__ __forceinline__ float top_of(int type) { return type == IB200_E4M3 ? held_top<HELD_E4M3>() : held_top<HELD_I8>(); }
+__device__ __forceinline__ float inverse_of(int type, float top) { return type == IB200_E4M3 ? held_inverse<HELD_E4M3>(top) : held_inverse<HELD_I8>(top); }
+
+// ---- rows that fit the registers of a warp or a CTA -------------------------------------------------------
+// One read of x and the residual, one write of everything: HBM-bound.  With VEC a thread has vectors of 8 adjacent columns, 8 * 32
+// or 8 * THREADS apart (16-byte accesses).  Rows that do not begin on 16-byte boundaries are read element by
+// element; a warp then has 256 * NV adjacent columns, lane by lane (coalesced).  Either way the columns that share a scale
+// lie in one warp.
+template <typename T> struct Raw { uint4 v[sizeof(T) / 2]; };  // 8 elements as they lie in memory
+template <typename T> __device__ __forceinline__ Raw<T> read8(const T* p) {
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  return r;
+}
+template <typename T> __device__ __forceinline__ void floats8(const Raw<T>& r, float (&v)[VE]) {
+  const T* p = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) v[i] = to_f32(p[i]);
+}
+template <typename T> __device__ __forceinline__ void write8(T* p, const float (&v)[VE]) {
+  Raw<T> r;
+  T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) e[i] = from_f32<T>(v[i]);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, r.v[i]);
+}
+
+template <typename T, bool HELD, int THREADS, int NV, bool VEC>
+__global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_resident(const RmsArgs a) {
+  __shared__ float slots[2][32];
+  const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31, cols = (int)a.cols;
+  const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.rows) return;  // whole warps, and nothing below waits for other rows' warps
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
+  auto total = [&](float v, float* at) { return THREADS == 32 ? warp_reduce<SumOp>(v) : block_reduce<SumOp>(v, at); };
+  // column of element i of vector k
+  auto col = [&](int k, int i) { return VEC ? (k * THREADS + tid) * VE + i : (tid >> 5) * (256 * NV) + (k * VE + i) * 32 + lane; };
+
+  float e[NV][VE];
+  if (VEC) {
+    Raw<T> xr[NV], rr[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (col(k, 0) < cols) xr[k] = read8(x + col(k, 0));
+    if (res) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (col(k, 0) < cols) rr[k] = read8(res + col(k, 0));
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = col(k, 0) < cols;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) e[k][i] = 0.0f;
+      if (in) {
+        floats8(xr[k], e[k]);
+        if (res) {
+          float r[VE];
+          floats8(rr[k], r);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) e[k][i] += r[i];
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) e[k][i] = col(k, i) < cols ? to_f32(x[col(k, i)]) : 0.0f;
+    if (res) {
+      float r[NV][VE];
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) r[k][i] = col(k, i) < cols ? to_f32(res[col(k, i)]) : 0.0f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) e[k][i] += r[k][i];
+    }
+  }
+  if (a.h) {
+    T* h = static_cast<T*>(a.h) + row * a.h_stride;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (VEC) {
+        if (col(k, 0) < cols) write8(h + col(k, 0), e[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          if (col(k, i) < cols) h[col(k, i)] = from_f32<T>(e[k][i]);
+      }
+    }
+  }
+  auto squares = [&](float pre) {
+    float s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) s = fmaf(e[k][i] * pre, e[k][i] * pre, s);
+    return s;
+  };
+  float ss = total(squares(1.0f), slots[0]), rstd;
+  if (isinf(ss)) {  // values beyond 2^60: their squares overflow f32, so the row is summed again scaled down (uniform over the row's threads)
+    rstd = kScaleDown / sqrtf(total(squares(kScaleDown), slots[1]) / (float)cols);
+    if (THREADS != 32) __syncthreads();  // the slots are used again
+  } else {
+    rstd = 1.0f / sqrtf(ss / (float)cols + a.eps);
+  }
+  float top = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    float w[VE];
+    if (a.w) {
+      if (VEC) {
+        if (col(k, 0) < cols) load_w8<T>(a, col(k, 0), w, true, VE);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = col(k, i) < cols ? load_w<T>(a, col(k, i)) : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      e[k][i] *= rstd;
+      if (a.w && col(k, VEC ? 0 : i) < cols) e[k][i] *= w[i];
+      if (HELD) top = max_nan(top, fabsf(e[k][i]));
+    }
+  }
+  if constexpr (!HELD) {
+    T* y = static_cast<T*>(a.y) + row * a.cols;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (VEC) {
+        if (col(k, 0) < cols) write8(y + col(k, 0), e[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          if (col(k, i) < cols) y[col(k, i)] = from_f32<T>(e[k][i]);
+      }
+    }
+  } else {
+    uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.cols;
+    float inv = 0.0f;
+    if (a.group == 0) {
+      top = THREADS == 32 ? warp_reduce<MaxOp>(top) : block_reduce<MaxOp>(top, slots[1]);
+      if (tid == 0) a.scale[row] = top / top_of(a.out_type);
+      inv = inverse_of(a.out_type, top);
+    }
+    const int lanes = a.group / VE, steps = a.group / 32;  // of a scale: lanes with VEC, elements of a lane without
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (VEC) {
+        if (a.group) {
+          float m = 0.0f;
+#pragma unroll
+          for (int i = 0; i < VE; ++i) m = max_nan(m, fabsf(e[k][i]));
+          for (int o = lanes >> 1; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+          const int c = col(k, 0);
+          if (c < cols && (tid & (lanes - 1)) == 0) a.scale[row * a.groups + c / a.group] = m / top_of(a.out_type);
+          inv = inverse_of(a.out_type, m);
+        }
+        if (col(k, 0) < cols) {
+          if (a.out_type == IB200_E4M3) hold8<HELD_E4M3>(y + col(k, 0), e[k], inv, true, VE);
+          else hold8<HELD_I8>(y + col(k, 0), e[k], inv, true, VE);
+        }
+      } else {
+        float m[VE];  // the maximum of element i's group
+        if (a.group) {
+#pragma unroll
+          for (int i = 0; i < VE; ++i) m[i] = warp_reduce<MaxOp>(fabsf(e[k][i]));
+#pragma unroll
+          for (int o = 1; o < VE; o <<= 1)
+            if (o < steps) {
+              float n[VE];
+#pragma unroll
+              for (int i = 0; i < VE; ++i) n[i] = max_nan(m[i], m[i ^ o]);
+#pragma unroll
+              for (int i = 0; i < VE; ++i) m[i] = n[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const int c = col(k, i);
+          if (a.group) {
+            inv = inverse_of(a.out_type, m[i]);
+            if (c < cols && lane == 0 && i % steps == 0) a.scale[row * a.groups + c / a.group] = m[i] / top_of(a.out_type);
+          }
+          if (c < cols) y[c] = (uint8_t)(a.out_type == IB200_E4M3 ? hold1<HELD_E4M3>(e[k][i] * inv) : hold1<HELD_I8>(e[k][i] * inv));
+        }
+      }
+    }
+  }
+}
+
+// ---- wider rows: one CTA per row, three passes over it (sum of squares, scales, values) -------------------
+template <typename T, bool HELD, int THREADS>
 __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const bool vec) {
   __shared__ float slots[2][32];
   const int64_t nv = (a.cols + VE - 1) / VE, nv_warp = (nv + 31) / 32 * 32;  // whole warps take part in the group maxima
-  const TW* w = static_cast<const TW*>(a.w);
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
@@ -68,9 +272,9 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
     };
     auto norm8 = [&](int64_t v, float rstd, float(&out)[VE], int left) {
       float ww[VE];
-      if (w) load8(w + v * VE, ww, vec, left);
+      if (a.w) load_w8<T>(a, v * VE, ww, vec, left);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) out[i] = out[i] * rstd * (w ? ww[i] : 1.0f);
+      for (int i = 0; i < VE; ++i) out[i] = out[i] * rstd * (a.w ? ww[i] : 1.0f);
     };
     auto squares = [&](float pre, float* at) {
       float ss = 0.0f;
@@ -91,7 +295,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
       rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
     }
     float row_max = 0.0f;
-    if (HELD != HELD_NONE && a.group == 0) {
+    if (HELD && a.group == 0) {
       for (int64_t v = threadIdx.x; v < nv; v += THREADS) {
         float e[VE];
         const int left = sum8(v, e);
@@ -100,7 +304,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
         for (int i = 0; i < VE; ++i) row_max = max_nan(row_max, fabsf(e[i]));
       }
       row_max = block_reduce<MaxOp>(row_max, slots[1]);
-      if (threadIdx.x == 0) a.scale[row] = row_max / held_top<HELD>();
+      if (threadIdx.x == 0) a.scale[row] = row_max / top_of(a.out_type);
     }
     for (int64_t v = threadIdx.x; v < nv_warp; v += THREADS) {
       float e[VE];
@@ -113,7 +317,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
 #pragma unroll
         for (int i = 0; i < VE; ++i) e[i] = 0.0f;
       }
-      if constexpr (HELD == HELD_NONE) {
+      if constexpr (!HELD) {
         if (v < nv) store8(static_cast<T*>(a.y) + row * a.cols + v * VE, e, vec, left);
       } else {
         float top = row_max;
@@ -123,25 +327,36 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
 #pragma unroll
           for (int i = 0; i < VE; ++i) top = max_nan(top, fabsf(e[i]));
           for (int o = lanes >> 1; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (v < nv && (v % lanes) == 0) a.scale[row * a.groups + v / lanes] = top / held_top<HELD>();
+          if (v < nv && (v % lanes) == 0) a.scale[row * a.groups + v / lanes] = top / top_of(a.out_type);
         }
-        if (v < nv) hold8<HELD>(static_cast<uint8_t*>(a.y) + row * a.cols + v * VE, e, held_inverse<HELD>(top), vec, left);
+        if (v < nv) {
+          uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.cols + v * VE;
+          if (a.out_type == IB200_E4M3) hold8<HELD_E4M3>(y, e, held_inverse<HELD_E4M3>(top), vec, left);
+          else hold8<HELD_I8>(y, e, held_inverse<HELD_I8>(top), vec, left);
+        }
       }
     }
     __syncthreads();  // the next row reuses the reduction slots
   }
 }
 
-template <typename T, typename TW, int HELD> int run_rms(const RmsArgs& a, bool vec, cudaStream_t s) {
-  constexpr int THREADS = 256;
-  const int64_t grid = a.rows < (1 << 20) ? a.rows : (1 << 20);
-  rmsnorm_stream<T, TW, HELD, THREADS><<<(unsigned)grid, THREADS, 0, s>>>(a, vec);
+template <typename T, bool HELD, int THREADS, int NV> int run_resident(const RmsArgs& a, bool vec, cudaStream_t s) {
+  const unsigned grid = (unsigned)(THREADS == 32 ? (a.rows + 7) / 8 : a.rows), threads = THREADS == 32 ? 256 : THREADS;
+  if (vec) rmsnorm_resident<T, HELD, THREADS, NV, true><<<grid, threads, 0, s>>>(a);
+  else rmsnorm_resident<T, HELD, THREADS, NV, false><<<grid, threads, 0, s>>>(a);
   return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "rmsnorm launch");
 }
-template <typename T, typename TW> int run_rms_held(const RmsArgs& a, int out_dtype, bool vec, cudaStream_t s) {
-  if (out_dtype == IB200_E4M3) return run_rms<T, TW, HELD_E4M3>(a, vec, s);
-  if (out_dtype == IB200_I8) return run_rms<T, TW, HELD_I8>(a, vec, s);
-  return run_rms<T, TW, HELD_NONE>(a, vec, s);
+template <typename T, bool HELD> int run_rms(const RmsArgs& a, bool vec, cudaStream_t s) {
+  if (a.rows <= INT32_MAX) {
+    if (a.cols <= 1024) return run_resident<T, HELD, 32, 4>(a, vec, s);
+    if (a.cols <= 2048) return run_resident<T, HELD, 256, 1>(a, vec, s);
+    if (a.cols <= 4096) return run_resident<T, HELD, 256, 2>(a, vec, s);
+    if (a.cols <= 8192) return run_resident<T, HELD, 256, 4>(a, vec, s);
+    if (a.cols <= 16384) return run_resident<T, HELD, 512, 4>(a, vec, s);
+  }
+  const int64_t grid = a.rows < (1 << 20) ? a.rows : (1 << 20);
+  rmsnorm_stream<T, HELD, 512><<<(unsigned)grid, 512, 0, s>>>(a, vec);
+  return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "rmsnorm launch");
 }
 
 }  // namespace
@@ -165,16 +380,15 @@ int launch_rmsnorm(const void* x, int64_t x_stride, const void* res, int64_t res
       (h && beyond_any_device(rows, h_stride > 0 ? h_stride : 1)))
     return fail(IB200_ERR_INVALID, "rmsnorm: a row stride beyond any device");
   const int e = dtype_size(dtype);
-  RmsArgs a{x, res, w, y, h, scale, x_stride, res_stride, h_stride, rows, cols, group ? (cols + group - 1) / group : 1, (int)group, eps};
+  RmsArgs a{x, res, w, y, h, scale, x_stride, res_stride, h_stride, rows, cols, group ? (cols + group - 1) / group : 1, (int)group, out_dtype,
+            w_dtype == IB200_F32, eps};
   // 16-byte loads: every row of every operand has to begin on a 16-byte boundary (8 bytes for the held result)
   auto even = [&](const void* p, int64_t stride, int bytes) { return !p || (aligned16(p) && (rows == 1 || stride * bytes % 16 == 0)); };
-  const bool vec = even(x, x_stride, e) && even(res, res_stride, e) && even(h, h_stride, e) && even(w, 0, 4) &&
-                   (held ? (reinterpret_cast<uintptr_t>(y) & 7) == 0 && (rows == 1 || cols % 8 == 0) : even(y, cols, e));
-  const bool wide_w = w_dtype == IB200_F32 || !w;
-  if (dtype == IB200_F32) return run_rms_held<float, float>(a, out_dtype, vec, s);
-  if (dtype == IB200_BF16)
-    return wide_w ? run_rms_held<__nv_bfloat16, float>(a, out_dtype, vec, s) : run_rms_held<__nv_bfloat16, __nv_bfloat16>(a, out_dtype, vec, s);
-  return wide_w ? run_rms_held<__half, float>(a, out_dtype, vec, s) : run_rms_held<__half, __half>(a, out_dtype, vec, s);
+  const bool vec = cols % VE == 0 && even(x, x_stride, e) && even(res, res_stride, e) && even(h, h_stride, e) && even(w, 0, 4) &&
+                   (held ? (reinterpret_cast<uintptr_t>(y) & 7) == 0 : even(y, cols, e));
+  if (dtype == IB200_F32) return held ? run_rms<float, true>(a, vec, s) : run_rms<float, false>(a, vec, s);
+  if (dtype == IB200_BF16) return held ? run_rms<__nv_bfloat16, true>(a, vec, s) : run_rms<__nv_bfloat16, false>(a, vec, s);
+  return held ? run_rms<__half, true>(a, vec, s) : run_rms<__half, false>(a, vec, s);
 }
 
 }  // namespace ib200
