@@ -127,9 +127,10 @@ int ib200_check_status(const int32_t* status, void* stream) {
     static const char* where[] = {"", "producer waiting for a free ring stage", "MMA issuer waiting for a drained accumulator",
                                   "MMA issuer waiting for a TMA stage", "epilogue waiting for a finished accumulator",
                                   "normalisation waiting for a staged row segment", "normalisation waiting for its cluster's statistics",
-                                  "long-row kernel waiting for the other segments of its row"};
+                                  "long-row kernel waiting for the other segments of its row",
+                                  "4-bit product waiting for a stage of weights"};
     return fail(IB200_ERR_DEVICE_WAIT, std::string("bounded device wait expired (") +
-                                           (host > 0 && host < 8 ? where[host] : "unknown site") + ")");
+                                           (host > 0 && host < 9 ? where[host] : "unknown site") + ")");
   }
   return IB200_OK;
 }

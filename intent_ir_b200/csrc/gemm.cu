@@ -995,4 +995,18 @@ int launch_gemm(const void* a, const void* b, const void* bias, void* c, int in_
   return fail(IB200_ERR_UNSUPPORTED, "gemm: operand dtypes must be f32, f16 or bf16");
 }
 
+// row-major [rows, row_bytes] bytes (base 16-byte aligned, row_bytes a multiple of 16), box [box_rows, 128 bytes], 128-byte swizzle
+int make_byte_map(CUtensorMap* map, const void* base, int64_t rows, int64_t row_bytes, int box_rows) {
+  EncodeTiledFn enc;
+  if (int rc = get_encoder(&enc)) return rc;
+  cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(IB200_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r));
+  return IB200_OK;
+}
+
 }  // namespace ib200

@@ -7,24 +7,32 @@
 // CTA adds up the lengths itself), so a batch of mixed lengths fills the GPU evenly.  A unit that lies in one range is
 // finished there; the pieces of others go to scratch as (sum, maximum, unnormalised o), and a second launch joins them in order.
 //
-// Inside a CTA the four warps take 32 keys each of a tile, with copies of their own three stages deep (cp.async) and no
+// Inside a CTA the four warps take 32 keys each of a tile, with copies of their own two stages deep (cp.async) and no
 // barrier between them until the unit ends.  Both products run on mma.sync with the keys as the 16 rows: S' = K Q' and
 // O' = V' P', so that 8 queries fill a fragment where queries as rows would need 16.  Bytes are widened to f16, which
 // is exact for both types; scales are applied to the scores and to p.  q is scaled by a power of two to below 2 (exact), p * vs
 // by another one to below 2^15, so that f16 holds them to 2^-12 over 2^39.
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace ib200 {
 namespace {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 32, kTile = kWarps * kStep, kStages = 3;
+constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 32, kTile = kWarps * kStep, kStages = 2;
+// What beginning a unit costs, in tiles: tables, pages and queries are fetched one after the other and the warps' results joined.
+// 64 sequences of up to 8193 tokens: 115 us with 0, 106 with 1, 98 with 2, 95 with 4, 96 with 6.
+constexpr int kStart = 4;
 template <int D> struct Cfg {
   static constexpr int kStageBytes = 2 * kStep * D;  // keys, values
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
-  static constexpr int kCtas = D == 128 ? 2 : 4;  // per SM, by shared memory
+  static constexpr int kCtas = D == 128 ? 3 : 4;  // per SM with one eight of rows; one less with two (registers)
   static constexpr int kPitch = D + 4;            // floats between the rows of the joining buffer
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {  // zeros where nothing is taken
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
@@ -60,6 +68,7 @@ template <int D> __device__ __forceinline__ int at_chunk(int r, int c) {
 
 struct Seq {  // what a sequence asks for
   int first, n, len, keys, tile0, tiles, units_per_head;  // keys: those that the table has room for
+  int64_t unit_work, work;  // a unit's, all units' (0 where there are no tiles)
 };
 __device__ __forceinline__ int first_key(const Kv8Attention& a, int64_t pos) {  // that the token at `pos` sees
   return a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
@@ -75,9 +84,10 @@ __device__ __forceinline__ Seq seq_of(const Kv8Attention& a, int b, int rows) {
   s.tile0 = first_key(a, (int64_t)s.len - s.n) / kTile;
   s.tiles = s.keys > 0 ? max(0, (s.keys - 1) / kTile + 1 - s.tile0) : 0;
   s.units_per_head = (int)((s.n * group + rows - 1) / rows);
+  s.unit_work = s.tiles ? s.tiles + kStart : 0;
+  s.work = a.heads * s.units_per_head * s.unit_work;
   return s;
 }
-__device__ __forceinline__ int64_t work_of(const Kv8Attention& a, const Seq& s) { return (int64_t)a.heads * s.units_per_head * s.tiles; }
 
 // scratch: the work in front of every sequence and in all, then two partial results per CTA
 struct Scratch {
@@ -99,7 +109,7 @@ template <typename V> __device__ __forceinline__ V scan_warp(V v, int lane) {  /
 }
 
 template <typename T, int HELD, int D, int NT>
-__global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention a, const Scratch sc, const int q_vec) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kCtas - 1) attention_kernel(const Kv8Attention a, const Scratch sc, const int q_vec) {
   using C = Cfg<D>;
   constexpr int ROWS = 8 * NT, HALVES = D / 64, MT = D / 16, CH = D / 16;  // CH: 16-byte chunks of a token
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -110,25 +120,30 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
   const int batch = (int)a.batch, group = (int)(a.q_heads / a.heads);
 
   // ---- this CTA's range of tiles -------------------------------------------------------------------
-  int64_t mine = 0;
-  for (int b = threadIdx.x; b < batch; b += kThreads) mine += work_of(a, seq_of(a, b, ROWS));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) sums[warp] = mine;
   if (threadIdx.x == 0) found = -1;
-  __syncthreads();
-  const int64_t total = sums[0] + sums[1] + sums[2] + sums[3];
-  const int ctas = (int)min((int64_t)gridDim.x, total);  // with less work than CTAs, one tile to each
-  int64_t w = 0, w_end = 0;
-  if (blockIdx.x < ctas) {
-    w = total * blockIdx.x / ctas;
-    w_end = total * (blockIdx.x + 1) / ctas;
+  int64_t total = 0, w = 0, w_end = 0;
+  auto range = [&] {
+    const int ctas = (int)min((int64_t)gridDim.x, total);  // with less work than CTAs, one tile to each
+    if (blockIdx.x < ctas) {
+      w = total * blockIdx.x / ctas;
+      w_end = total * (blockIdx.x + 1) / ctas;
+    }
+  };
+  if (batch > kThreads) {
+    int64_t mine = 0;
+    for (int b = threadIdx.x; b < batch; b += kThreads) mine += seq_of(a, b, ROWS).work;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    total = sums[0] + sums[1] + sums[2] + sums[3];
+    range();
   }
   int64_t before = 0;
   for (int base = 0; base < batch; base += kThreads) {
     __syncthreads();
     const int b = base + threadIdx.x;
-    const int64_t v = b < batch ? work_of(a, seq_of(a, b, ROWS)) : 0;
+    const int64_t v = b < batch ? seq_of(a, b, ROWS).work : 0;
     const int64_t upto = scan_warp(v, lane);
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
@@ -136,6 +151,10 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
     for (int i = 0; i < warp; ++i) front += sums[i];
     front += upto - v;  // the work in front of sequence b
     before += sums[0] + sums[1] + sums[2] + sums[3];
+    if (batch <= kThreads) {
+      total = before;
+      range();
+    }
     if (blockIdx.x == 0 && b < batch) sc.before[b] = front;
     if (v > 0 && front <= w && w < front + v) {
       found = b;
@@ -152,12 +171,15 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
   int b = found;
   int64_t front = found_before;
   Seq s = seq_of(a, b, ROWS);
-  bool first_piece = true;
+  const int64_t w_start = w;
 
   while (w < w_end) {
     // ---- a piece: one unit's tiles [from, to) -------------------------------------------------------
-    const int64_t rel = w - front;
-    const int unit = (int)(rel / s.tiles), from = (int)(rel - (int64_t)unit * s.tiles), to = (int)min((int64_t)s.tiles, from + (w_end - w));
+    // a unit's work is kStart for beginning it, then its tiles; a piece without tiles is nothing
+    const int64_t rel = w - front, unit64 = rel >> 32 ? rel / s.unit_work : (int64_t)((unsigned)rel / (unsigned)s.unit_work), in = rel - unit64 * s.unit_work, piece_start = w;
+    const int unit = (int)unit64, from = (int)max((int64_t)0, in - kStart), to = (int)min((int64_t)s.tiles, in + (w_end - w) - kStart);
+    w = min(w_end, front + (unit64 + 1) * s.unit_work);
+    if (to > from) {
     const int head = unit / s.units_per_head, r0 = (unit - head * s.units_per_head) * ROWS;
     const int rows = (int)min((int64_t)ROWS, (int64_t)s.n * group - r0);
     const int start = s.len - s.n;  // place of the first new token (negative: fewer tokens than new ones)
@@ -170,6 +192,63 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
     j1 = pos_max < off ? j0 : min(j1, (pos_max - off) / kTile + 1);
     const int steps = max(0, j1 - j0);
 
+    // Pages and scales, 16 steps at a time: lane 2i + h looks up the 16 keys of half h of step i.  The next 16 are fetched while these are used.
+    struct Meta { int page, slot; float ks, vs; };  // page: page * heads + head, -1: outside the cache
+    auto look_up = [&](int step0) {
+      Meta x{-1, 0, NAN, NAN};
+      const int step = step0 + (lane >> 1);
+      const unsigned key = (unsigned)(j0 + step) * kTile + off + (lane & 1) * 16, block = (unsigned)a.block;  // (32-bit division)
+      if (step < steps && key < (unsigned)s.keys) {
+        const unsigned blk = key / block;
+        x.slot = (int)(key - blk * block);
+        const int page = a.table[(int64_t)b * a.table_blocks + blk];
+        if ((unsigned)page < (unsigned)a.pages) x.page = page * (int)a.heads + head;
+      }
+      return x;
+    };
+    auto look_scales = [&](Meta& x) {
+      if (x.page >= 0) {
+        x.ks = a.k_scale[x.page];
+        x.vs = a.v_scale[x.page];
+      }
+    };
+    // The 16 keys of a half are one run of bytes in memory.  Chunk i * 32 + lane of it goes to row (i * 32 + lane) / CH; rows 8 apart are
+    // swizzled alike, so two places of a lane give all others by adding constants.
+    const uint32_t place0 = at_chunk<D>(lane / CH, lane % CH), place1 = at_chunk<D>((32 + lane) / CH, lane % CH) - 512;
+    auto issue = [&](int step, const Meta& meta) {
+      const uint32_t dst = stages_at + (step % kStages) * C::kStageBytes;
+      const int key0 = (j0 + step) * kTile + off;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int page = __shfl_sync(0xffffffffu, meta.page, 2 * (step & 15) + h), slot = __shfl_sync(0xffffffffu, meta.slot, 2 * (step & 15) + h);
+        const int left = page < 0 ? 0 : s.keys - (key0 + h * 16);  // keys of these 16 that exist; what lies behind the last one is never read
+        const int64_t base = page < 0 ? 0 : ((int64_t)page * a.block + slot) * D;
+        const uint8_t *ksrc = a.k_cache + base + lane * 16, *vsrc = a.v_cache + base + lane * 16;
+        const uint32_t even = dst + h * 16 * D + place0, odd = dst + h * 16 * D + place1;
+        if (left >= 16) {
+#pragma unroll
+          for (int i = 0; i < 16 * CH / 32; ++i) {
+            copy16((i & 1 ? odd : even) + i * 512, ksrc + i * 512);
+            copy16((i & 1 ? odd : even) + i * 512 + kStep * D, vsrc + i * 512);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 * CH / 32; ++i) {
+            const bool take = (i * 32 + lane) / CH < left;
+            copy16((i & 1 ? odd : even) + i * 512, take ? ksrc + i * 512 : a.k_cache, take);
+            copy16((i & 1 ? odd : even) + i * 512 + kStep * D, take ? vsrc + i * 512 : a.v_cache, take);
+          }
+        }
+      }
+    };
+
+    Meta cur = look_up(0);
+    look_scales(cur);
+    Meta nxt = cur;
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (i < steps) issue(i, cur);
+      copy_commit();
+    }
     // queries as the k x 8 operand: chunk bytes 4w .. 4w + 3 of half h are the k slots (2t, 2t + 1, 2t + 8, 2t + 9) of product 4h + w
     uint32_t qf[NT][HALVES * 4][2];
     float mult[NT][2];
@@ -226,69 +305,9 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
         for (int c = 0; c < 4; ++c) o[nt][i][c] = 0.0f;
     }
 
-    // Pages and scales, 16 steps at a time: lane 2i + h looks up the 16 keys of half h of step i.  The next 16 are fetched while these are used.
-    struct Meta { int page, slot; float ks, vs; };  // page: page * heads + head, -1: outside the cache
-    auto look_up = [&](int step0) {
-      Meta x{-1, 0, NAN, NAN};
-      const int step = step0 + (lane >> 1);
-      const int64_t key = (int64_t)(j0 + step) * kTile + off + (lane & 1) * 16;
-      if (step < steps && key < s.keys) {
-        const int blk = (int)(key / a.block);
-        x.slot = (int)(key - (int64_t)blk * a.block);
-        const int page = a.table[(int64_t)b * a.table_blocks + blk];
-        if ((unsigned)page < (unsigned)a.pages) x.page = page * (int)a.heads + head;
-      }
-      return x;
-    };
-    auto look_scales = [&](Meta& x) {
-      if (x.page >= 0) {
-        x.ks = a.k_scale[x.page];
-        x.vs = a.v_scale[x.page];
-      }
-    };
-    auto issue = [&](int step, const Meta& meta) {
-      const uint32_t dst = stages_at + (step % kStages) * C::kStageBytes;
-      const int key0 = (j0 + step) * kTile + off;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int page = __shfl_sync(0xffffffffu, meta.page, 2 * (step & 15) + h), slot = __shfl_sync(0xffffffffu, meta.slot, 2 * (step & 15) + h);
-        const int64_t base = page < 0 ? 0 : ((int64_t)page * a.block + slot) * D;
-        const int left = page < 0 ? 0 : s.keys - (key0 + h * 16);  // keys of these 16 that exist; what lies behind the last one is never read
-#pragma unroll
-        for (int i = 0; i < 16 * CH / 32; ++i) {
-          const int idx = i * 32 + lane, r = idx / CH, c = idx % CH;
-          const bool take = r < left;
-          const int64_t src = take ? base + r * D + c * 16 : 0;
-          const uint32_t to_at = dst + at_chunk<D>(h * 16 + r, c);
-          copy16(to_at, a.k_cache + src, take);
-          copy16(to_at + kStep * D, a.v_cache + src, take);
-        }
-      }
-    };
-
-    Meta cur = look_up(0);
-    look_scales(cur);
-    Meta nxt = cur;
-    for (int i = 0; i < kStages - 1; ++i) {
-      if (i < steps) issue(i, cur);
-      copy_commit();
-    }
-    for (int step = 0; step < steps; ++step) {
-      if ((step & 15) == 0) {
-        if (step) cur = nxt;
-        nxt = look_up(step + 16);
-      } else if ((step & 15) == 8) {
-        look_scales(nxt);
-      }
-      copy_wait<kStages - 2>();
-      __syncwarp();
-      {
-        const int ahead = step + kStages - 1;
-        if (ahead < steps) {
-          if ((ahead >> 4) == (step >> 4)) issue(ahead, cur); else issue(ahead, nxt);
-        }
-        copy_commit();
-      }
+    // one step; masked: some row does not see all of its keys
+    auto compute = [&](int step, auto kind) {
+      constexpr bool masked = decltype(kind)::value;
       const uint8_t* kst = stages + (step % kStages) * C::kStageBytes;
       const uint8_t* vst = kst + kStep * D;
       const int key0 = (j0 + step) * kTile + off;
@@ -318,7 +337,6 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
       // ---- running maximum and sum ------------------------------------------------------------------
       const float ks[2] = {__shfl_sync(0xffffffffu, cur.ks, 2 * (step & 15)), __shfl_sync(0xffffffffu, cur.ks, 2 * (step & 15) + 1)};
       const float vs[2] = {__shfl_sync(0xffffffffu, cur.vs, 2 * (step & 15)), __shfl_sync(0xffffffffu, cur.vs, 2 * (step & 15) + 1)};
-      const bool masked = key0 + kStep - 1 > pos_min || key0 < lo_max;
       // the power of two above the values' scales so far; NaN scales do not enter it (they reach p below)
       const float vmax = fmaxf(vtop, fmaxf(fabsf(vs[0]), fabsf(vs[1])));
       float grow = 1.0f;
@@ -337,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float x = sv[mt][nt][c] * (mult[nt][c & 1] * ks[mt]);
-            if (masked) {
+            if constexpr (masked) {
               const int key = key0 + mt * 16 + (c >> 1) * 8 + g;
               if (key > hi[nt][c & 1] || key < low[nt][c & 1]) x = -INFINITY;
             }
@@ -364,7 +382,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
             const float x = exp2_fast(sv[mt][nt][c] - base[c & 1]);
             l[nt][c & 1] += x;
             p[mt][c] = x * vf[mt];
-            if (masked) {  // a NaN scale counts only for the rows that see the key
+            if constexpr (masked) {  // a NaN scale counts only for the rows that see the key
               const int key = key0 + mt * 16 + (c >> 1) * 8 + g;
               if (key > hi[nt][c & 1] || key < low[nt][c & 1]) p[mt][c] = 0.0f;
             }
@@ -399,7 +417,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
           }
         }
         bool apart = false;  // a NaN among values that some rows do not see: the rows' products are taken one by one
-        if (HELD == HELD_E4M3 && masked) {
+        if constexpr (HELD == HELD_E4M3 && masked) {
           uint32_t any = 0;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
@@ -422,6 +440,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
           } else {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
+#pragma unroll 1
               for (int col = 0; col < 8; ++col) {
                 const int last = __shfl_sync(0xffffffffu, (col & 1) ? hi[nt][1] : hi[nt][0], col >> 1), begin = __shfl_sync(0xffffffffu, (col & 1) ? low[nt][1] : low[nt][0], col >> 1);
                 uint32_t keep[2];
@@ -438,6 +457,26 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
           }
         }
       }
+    };
+
+    for (int step = 0; step < steps; ++step) {
+      if ((step & 15) == 0) {
+        if (step) cur = nxt;
+        nxt = look_up(step + 16);
+      } else if ((step & 15) == 8) {
+        look_scales(nxt);
+      }
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      {
+        const int ahead = step + kStages - 1;
+        if (ahead < steps) {
+          if ((ahead >> 4) == (step >> 4)) issue(ahead, cur); else issue(ahead, nxt);
+        }
+        copy_commit();
+      }
+      const int key0 = (j0 + step) * kTile + off;
+      if (key0 + kStep - 1 > pos_min || key0 < lo_max) compute(step, std::true_type()); else compute(step, std::false_type());
     }
 
     // ---- join the warps -------------------------------------------------------------------------------
@@ -465,7 +504,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
     if (lane == 0) top_v[warp] = vtop;
     __syncthreads();
     const bool whole = from == 0 && to == s.tiles;
-    float* part = sc.part + ((int64_t)blockIdx.x * 2 + (first_piece ? 0 : 1)) * (ROWS * (D + 2));
+    float* part = sc.part + ((int64_t)blockIdx.x * 2 + (piece_start == w_start ? 0 : 1)) * (ROWS * (D + 2));
     for (int idx = threadIdx.x; idx < ROWS * (D / 4); idx += kThreads) {
       const int row = idx / (D / 4), d = idx % (D / 4) * 4;
       if (row >= rows) break;
@@ -498,61 +537,80 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const Kv8Attention 
       }
     }
     __syncthreads();  // the next piece copies over the box
-    first_piece = false;
-    w += to - from;
-    if (w < w_end && w == front + work_of(a, s)) {
+    }
+    if (w < w_end && w == front + s.work) {
       front = w;
-      do s = seq_of(a, ++b, ROWS); while (work_of(a, s) == 0);  // w < total: there is one
+      do s = seq_of(a, ++b, ROWS); while (s.work == 0);  // w < total: there is one
     }
   }
 }
 
-// One warp per row: a row whose unit was cut is joined from its pieces, one without keys is zero.
+// One CTA per row: a row whose unit was cut is joined from its pieces, four at a time, one without keys is zero.
+constexpr int kJoin = 128;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) join_kernel(const Kv8Attention a, const Scratch sc, const int grid) {
-  constexpr int ROWS = 8 * NT, PER = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (u >= a.tokens * a.q_heads) return;
+__global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const Scratch sc, const int grid) {
+  constexpr int ROWS = 8 * NT, PER = D / 32, WARPS = kJoin / 32;
+  __shared__ float slots[2][32], weight[kJoin], box[WARPS][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
+  const int64_t u = blockIdx.x;
   const int t = (int)(u / a.q_heads), qh = (int)(u - (int64_t)t * a.q_heads), group = (int)(a.q_heads / a.heads);
   int b, first, count;
   if (!find_sequence(a.cu, (int)a.batch, a.each, t, b, first, count)) return;
   const Seq s = seq_of(a, b, ROWS);
-  T* o = static_cast<T*>(a.o) + u * D + lane * PER;
   const int64_t pos = (int64_t)a.lens[b] - count + (t - first);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  T* o = static_cast<T*>(a.o) + u * D;
   if (pos < 0 || pos >= s.keys || s.tiles == 0) {  // no keys; or its own key is outside the table (or offsets that cannot be)
-#pragma unroll
-    for (int e = 0; e < PER; ++e) o[e] = from_f32<T>(pos < 0 ? 0.0f : NAN);
-    if (a.lse && lane == 0) a.lse[u] = pos < 0 ? -INFINITY : NAN;
+    for (int d = tid; d < D; d += kJoin) o[d] = from_f32<T>(pos < 0 ? 0.0f : NAN);
+    if (a.lse && tid == 0) a.lse[u] = pos < 0 ? -INFINITY : NAN;
     return;
   }
   const int head = qh / group, r = (t - first) * group + (qh - head * group), row = r % ROWS;
-  const int64_t total = sc.before[a.batch], lo = sc.before[b] + ((int64_t)head * s.units_per_head + r / ROWS) * s.tiles, hi = lo + s.tiles - 1;
-  const int ctas = (int)min((int64_t)grid, total);
-  const int c0 = (int)(((lo + 1) * ctas - 1) / total), c1 = (int)(((hi + 1) * ctas - 1) / total);  // the CTAs whose ranges hold the first and the last tile
+  // the CTAs whose ranges hold the unit's first and last tile
+  const int64_t total = sc.before[a.batch], unit = sc.before[b] + ((int64_t)head * s.units_per_head + r / ROWS) * s.unit_work;
+  const int64_t ctas = min((int64_t)grid, total), lo = unit + kStart, hi = unit + s.unit_work - 1;
+  const int c0 = (int)(((lo + 1) * ctas - 1) / total), c1 = (int)(((hi + 1) * ctas - 1) / total);
   if (c0 == c1) return;
   const int64_t size = ROWS * (D + 2);
-  const float* p0 = sc.part + ((int64_t)c0 * 2 + (lo == total * c0 / ctas ? 0 : 1)) * size;
+  const float* p0 = sc.part + ((int64_t)c0 * 2 + (total * c0 / ctas >= unit ? 0 : 1)) * size;
   auto piece = [&](int c) { return c == c0 ? p0 : sc.part + (int64_t)c * 2 * size; };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, piece(c)[ROWS * D + row]);
-  m = warp_reduce<MaxOp>(m);
-  const float base = m == -INFINITY ? 0.0f : m;
-  float sum = 0.0f, v[PER];
+  float m = -INFINITY, sum = 0.0f, v[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) v[e] = 0.0f;
-#pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const float* p = piece(c);
-    const float f = exp2_fast(p[ROWS * D + row] - base);
-    sum += p[ROWS * D + ROWS + row] * f;
+  for (int base = c0; base <= c1; base += kJoin) {  // kJoin pieces at a time
+    const int c = base + tid, n = min(kJoin, c1 - base + 1);
+    const float pm = c <= c1 ? piece(c)[ROWS * D + row] : -INFINITY, pl = c <= c1 ? piece(c)[ROWS * D + ROWS + row] : 0.0f;
+    const float now = fmaxf(m, block_reduce<MaxOp>(pm, slots[0])), from = now == -INFINITY ? 0.0f : now;
+    const float keep = exp2_fast(m - from), f = exp2_fast(pm - from);
+    weight[tid] = f;
+    sum = sum * keep + block_reduce<SumOp>(c <= c1 ? pl * f : 0.0f, slots[1]);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] += p[row * D + lane * PER + e] * f;
+    for (int e = 0; e < PER; ++e) v[e] *= keep;
+    m = now;
+#pragma unroll 8
+    for (int i = warp; i < n; i += WARPS) {
+      const float* p = piece(base + i) + row * D + lane * PER;
+      const float g = weight[i];
+      if (PER == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] += x.x * g, v[1] += x.y * g, v[PER - 2] += x.z * g, v[PER - 1] += x.w * g;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        v[0] += x.x * g, v[1] += x.y * g;
+      }
+    }
+    __syncthreads();
   }
 #pragma unroll
-  for (int e = 0; e < PER; ++e) o[e] = from_f32<T>(v[e] / sum);
-  if (a.lse && lane == 0) a.lse[u] = (m + log2f(sum)) * 0.6931471805599453f;
+  for (int e = 0; e < PER; ++e) box[warp][lane * PER + e] = v[e];
+  __syncthreads();
+  for (int d = tid; d < D; d += kJoin) {
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) x += box[i][d];
+    o[d] = from_f32<T>(x / sum);
+  }
+  if (a.lse && tid == 0) a.lse[u] = (m + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Rows of a unit, in eights: one where 8 rows suffice, two where a sequence has more (several new tokens, many heads to a group) so
@@ -563,8 +621,8 @@ int tiles_of_rows(int64_t tokens, int64_t batch, int64_t group) {
 }
 int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, int nt) {
   // no more CTAs than there can be tiles
-  const int64_t units = heads * ((tokens * group + 8 * nt - 1) / (8 * nt) + batch), tiles = table_blocks * block / kTile + 2;
-  const int64_t most = (int64_t)kSmCount * (dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas);
+  const int64_t units = heads * ((tokens * group + 8 * nt - 1) / (8 * nt) + batch), tiles = table_blocks * block / kTile + 2 + kStart;
+  const int64_t most = (int64_t)kSmCount * ((dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas) - (nt > 1));
   return units > most || units * tiles > most ? most : units * tiles;
 }
 
@@ -576,8 +634,8 @@ template <typename T, int HELD, int D, int NT> int run_attention(const Kv8Attent
   kern<<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, q_vec);
   if (cudaPeekAtLastError() != cudaSuccess) return cuda_fail(cudaGetLastError(), "attention_kv8 launch");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.tokens * a.q_heads + 3) / 4));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)(a.tokens * a.q_heads));
+  cfg.blockDim = dim3(kJoin);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

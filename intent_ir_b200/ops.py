@@ -400,11 +400,21 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
     need = _w4_scratch(x_code, m, n, k, group)
     scratch = x.new_empty(need, dtype=torch.uint8) if need else None
     args = _lib.W4_ARGS.pack(x.data_ptr(), _address(x_scale), q.data_ptr(), scales.data_ptr(), _address(zeros), _address(bias), y.data_ptr(), _address(scratch),
-                             0, stride, x_groups, x_code, _code("scales", scales, _FLOAT_CODE), _FLOAT_CODE[out_dtype], m, n, k, group, need)
+                             _status_address(index), stride, x_groups, x_code, _code("scales", scales, _FLOAT_CODE), _FLOAT_CODE[out_dtype], m, n, k, group, need)
     rc = _lib.load().ib200_w4_matmul(args, _stream())
     if rc:
         _check(rc, "w4_matmul")
     return y
+
+
+def _status_address(index: int) -> int:
+    """The device's status word; none inside a capture that comes before any other call (its zeroing would become part of the graph)."""
+    word = _status.get(index)
+    if word is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        word = status_word()
+    return word.data_ptr()
 
 
 @functools.lru_cache(maxsize=4096)
