@@ -21,7 +21,7 @@ struct W4Args {
   void* y;
   int64_t x_stride;
   int m, n, k, group, groups, xs_groups;
-  int x_type, s_type, y_type, x_vec, split;
+  int x_type, s_type, y_type, x_vec, s_vec, z_vec, split;
   int32_t* status;
 };
 
@@ -47,7 +47,21 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
 // the G / 4 adjacent k from t * G / 4, one 32-bit word of q (8 k) per two products, which keeps every product inside one
 // group; the group's sum is then scaled in f32.  A word gives pairs (0, 4), (1, 5), (2, 6), (3, 7), so x is laid down in that order, in
 // the order in which the warps read it.  128 + q in bf16 (1024 + q in f16) is q under the exponent of 128 (1024); minus 128 + z it is exact.
-constexpr int kRows = 128, kThreads = 256, kStageK = 256, kStages = 4, kRowBytes = kStageK / 2, kStageBytes = kRows * kRowBytes;
+// x, scales and zero points come by cp.async as far ahead as the weights: a load that a warp waits for costs more than a stage's work.
+constexpr int kRows = 128, kThreads = 256, kStageK = 256, kRowBytes = kStageK / 2;
+enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
+template <int XK, int NT, int G> struct Stage {  // bytes of a stage's parts
+  static constexpr int kStages = NT == 1 ? 4 : 3, GROUPS = kStageK / G;
+  static constexpr int X_CHUNK = XK >= X_E4M3 ? 8 : 16;                     // 8 k of a row
+  static constexpr int X_AT = kRows * kRowBytes;                              // after q: x in the order of its reads
+  static constexpr int XS_AT = X_AT + NT * 8 * (kStageK / 8) * X_CHUNK;       // scales of x: [group][row]
+  static constexpr int S_PITCH = GROUPS * 4, S_AT = XS_AT + GROUPS * NT * 8 * 4;  // scales of a row: f32, or 16 bits and up to 2 bytes of slack
+  static constexpr int Z_PITCH = (GROUPS + 3) / 4 * 4 + (GROUPS == 4 ? 4 : 8), Z_AT = S_AT + kRows * S_PITCH;  // zero points and up to 3 bytes of slack
+  static constexpr int BYTES = (Z_AT + kRows * Z_PITCH + 1023) / 1024 * 1024;
+};
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {  // the rest of the 4 is zero
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 
 template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (BF)
@@ -57,60 +71,54 @@ template <bool BF> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 128 + z (1024 + z) in both halves of a word: what brings a nibble under the exponent back to q - z
-template <bool BF> __device__ __forceinline__ uint32_t zero_of(uint32_t z) { return ((BF ? 0x4300u : 0x6400u) | z) * 0x10001u; }
-// the pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's eight q - z
-template <bool BF> __device__ __forceinline__ void weights_of(uint32_t w, uint32_t zero, uint32_t (&v)[4]) {
+// (x & mask) | magic in one instruction; the compiler splits it when both are constants
+template <uint32_t MASK> __device__ __forceinline__ uint32_t under(uint32_t x, uint32_t magic) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(MASK), "r"(magic));
+  return y;
+}
+// What brings a nibble under an exponent back to q - z, in both halves: 128 + z in bf16; 1024 + z, and -(64 + z) for nibbles four bits up, in f16
+struct Zero {
+  uint32_t lo, hi;
+};
+template <bool BF> __device__ __forceinline__ Zero zero_of(uint32_t z) {
+  const uint32_t zz = z * 0x10001u;
+  if (BF) return {0x43004300u | zz, 0};
+  return {0x64006400u | zz, 0xD400D400u | zz << 4};
+}
+template <typename H> __device__ __forceinline__ H as_pair(uint32_t x) { return *reinterpret_cast<const H*>(&x); }
+// the pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's eight q - z; `magic`: the exponent, in a register
+template <bool BF> __device__ __forceinline__ void weights_of(uint32_t w, const Zero& z, uint32_t magic, uint32_t (&v)[4]) {
+  if (BF) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = ((w >> (4 * i)) & 0x000f000fu) | (BF ? 0x43004300u : 0x64006400u);
-    if (BF) {
-      const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&zero));
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 d = __hsub2(as_pair<__nv_bfloat162>(under<0x000f000fu>(w >> (4 * i), magic)), as_pair<__nv_bfloat162>(z.lo));
       v[i] = *reinterpret_cast<const uint32_t*>(&d);
-    } else {
-      const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&zero));
+    }
+  } else {  // a nibble four bits up is 16 q: one shift for two pairs
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2C00));
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const uint32_t x = w >> (4 * i);
+      const __half2 d = __hsub2(as_pair<__half2>(under<0x000f000fu>(x, magic)), as_pair<__half2>(z.lo));
+      const __half2 e = __hfma2(as_pair<__half2>(under<0x00f000f0u>(x, magic)), sixteenth, as_pair<__half2>(z.hi));
       v[i] = *reinterpret_cast<const uint32_t*>(&d);
+      v[i + 1] = *reinterpret_cast<const uint32_t*>(&e);
     }
   }
 }
-// 8 adjacent x as they lie in memory.  Loading and converting are apart: a converted value makes its warp wait for the load.
-__device__ __forceinline__ uint4 x_raw(const W4Args& a, int row, int k) {
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (row >= a.m || k >= a.k) return r;
-  const int64_t at = (int64_t)row * a.x_stride + k;
-  if (a.x_type == IB200_BF16 || a.x_type == IB200_F16) {
-    const uint16_t* p = static_cast<const uint16_t*>(a.x) + at;
-    if (a.x_vec) return *reinterpret_cast<const uint4*>(p);
-    r.x = p[0] | (uint32_t)p[1] << 16, r.y = p[2] | (uint32_t)p[3] << 16, r.z = p[4] | (uint32_t)p[5] << 16, r.w = p[6] | (uint32_t)p[7] << 16;
-  } else {
-    const uint8_t* p = static_cast<const uint8_t*>(a.x) + at;
-    if (a.x_vec) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      r.x = v.x, r.y = v.y;
-    } else {
-      r.x = p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16 | (uint32_t)p[3] << 24;
-      r.y = p[4] | (uint32_t)p[5] << 8 | (uint32_t)p[6] << 16 | (uint32_t)p[7] << 24;
-    }
-  }
-  return r;
-}
-// as the pairs above; 8-bit values become f16, which is exact
-__device__ __forceinline__ uint4 x_pairs(const uint4& r, int type) {
-  if (type == IB200_BF16 || type == IB200_F16)
+// eight adjacent x as the pairs above; 8-bit values become f16, which is exact
+template <int XK> __device__ __forceinline__ uint4 x_pairs(const uint8_t* p) {
+  if (XK == X_BF16 || XK == X_F16) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
     return make_uint4(__byte_perm(r.x, r.z, 0x5410), __byte_perm(r.x, r.z, 0x7632), __byte_perm(r.y, r.w, 0x5410), __byte_perm(r.y, r.w, 0x7632));
-  uint4 v;
-  const uint32_t a01 = __byte_perm(r.x, r.y, 0x5140), a23 = __byte_perm(r.x, r.y, 0x7362);  // bytes 0 4 1 5, 2 6 3 7
-  if (type == IB200_E4M3) {
-    widen<HELD_E4M3>(a01, v.x, v.y);
-    widen<HELD_E4M3>(a23, v.z, v.w);
-  } else {
-    widen<HELD_I8>(a01, v.x, v.y);
-    widen<HELD_I8>(a23, v.z, v.w);
   }
+  constexpr int HELD = XK == X_E4M3 ? HELD_E4M3 : HELD_I8;
+  const uint2 r = *reinterpret_cast<const uint2*>(p);
+  uint4 v;
+  widen<HELD>(__byte_perm(r.x, r.y, 0x5140), v.x, v.y);  // bytes 0 4 1 5, 2 6 3 7
+  widen<HELD>(__byte_perm(r.x, r.y, 0x7362), v.z, v.w);
   return v;
-}
-__device__ __forceinline__ uint32_t raw_of(const void* p, int64_t i, int type) {
-  return type == IB200_F32 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
 }
 __device__ __forceinline__ float value_of(uint32_t raw, int type) {
   if (type == IB200_F16) return __half2float(__ushort_as_half((unsigned short)raw));
@@ -121,71 +129,102 @@ __device__ __forceinline__ float value_of(uint32_t raw, int type) {
 // read and sixteen of an 8-byte one touch all banks once.
 template <int G> __device__ __forceinline__ int row_of(int g) { return G == 128 ? (g >> 1) + 4 * (g & 1) : G == 64 ? (g & 3) * 2 + (g >> 2) : g; }
 
-template <bool BF, int NT, int G>
+template <int XK, int NT, int G>
 __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, const __grid_constant__ CUtensorMap map) {
-  constexpr int GROUPS = kStageK / G, HALF = GROUPS / 2, WORDS = G / 32;  // groups of a stage, of a warp's half; words of a thread in a group
-  constexpr int XBYTES = NT * 8 * (kStageK * 2 + GROUPS * 4);
+  using S = Stage<XK, NT, G>;
+  constexpr bool BF = XK == X_BF16;
+  constexpr int GROUPS = S::GROUPS, HALF = GROUPS / 2, WORDS = G / 32;  // groups of a stage, of a warp's half; words of a thread in a group
+  constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[kStages];
-  uint8_t* xbuf = smem + kStages * kStageBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wr = warp & 3, wk = warp >> 2, pg = row_of<G>(g);
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kRows, m0 = blockIdx.y * NT * 8;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
+  const uint32_t smem_at = smem_addr(smem);
 
-  auto issue = [&](int s) {  // (one thread)
+  auto issue_q = [&](int s) {  // (one thread)
     const int i = (s - s0) % kStages;
-    mbarrier_expect_tx(&full[i], kStageBytes);
+    mbarrier_expect_tx(&full[i], kRows * kRowBytes);
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(smem_addr(smem + i * kStageBytes)), "l"(&map), "r"(smem_addr(&full[i])), "r"(s * kRowBytes), "r"(n0) : "memory");
+                 ::"r"(smem_at + i * S::BYTES), "l"(&map), "r"(smem_addr(&full[i])), "r"(s * kRowBytes), "r"(n0) : "memory");
   };
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1);
     mbarrier_init_fence();
     for (int i = 0; i < kStages - 1; ++i)
-      if (s0 + i < s1) issue(s0 + i);
+      if (s0 + i < s1) issue_q(s0 + i);
   }
-  // x: chunk (8 k) of row m, where the warps read it: [group, word][tile of 8 rows][row][thread of the quad]
-  auto x_place = [&](int idx) {
-    const int row = idx / (kStageK / 8), k = idx % (kStageK / 8) * 8, in = k % G, th = in / (G / 4), word = in % (G / 4) / 8;
-    return (((k / G * WORDS + word) * NT + row / 8) * 8 + row % 8) * 4 + th;
+  // The other operands.  Two threads share a row of scales and zero points and take every other 4 bytes of it, from the 4-byte boundary
+  // in front of the stage's first group to the one behind its last, never beyond the end of the array.
+  const int srow = threadIdx.x >> 1, s_bytes = a.s_type == IB200_F32 ? 4 : 2;
+  const int64_t first = (int64_t)min(n0 + srow, a.n - 1) * a.groups;
+  const uint8_t *sc_row = static_cast<const uint8_t*>(a.s) + first * s_bytes, *sc_end = static_cast<const uint8_t*>(a.s) + (int64_t)a.n * a.groups * s_bytes;
+  const uint8_t *z_row = a.z + first, *z_end = a.z + (int64_t)a.n * a.groups;
+  auto row_pieces = [&](uint32_t dst, const uint8_t* from, int bytes, const uint8_t* end) {
+    const uint8_t *p = from - (reinterpret_cast<uintptr_t>(from) & 3) + (threadIdx.x & 1) * 4, *stop = from + bytes;
+    for (dst += (threadIdx.x & 1) * 4; p < stop; p += 8, dst += 8) {
+      const int left = (int)(end - p);
+      copy4(dst, left > 0 ? p : from - (reinterpret_cast<uintptr_t>(from) & 3), min(4, max(0, left)));
+    }
   };
-  uint4 xr[NT];
-  float xsr = 1.0f;  // a scale of x, behind the stage's x: [group][row]
-  auto x_load = [&](int s) {
+  auto issue = [&](int s) {
+    const uint32_t dst = smem_at + (s - s0) % kStages * S::BYTES;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int idx = i * kThreads + threadIdx.x;
-      xr[i] = x_raw(a, m0 + idx / (kStageK / 8), s * kStageK + idx % (kStageK / 8) * 8);
-    }
-    if (a.xs_groups > 1 && threadIdx.x < GROUPS * NT * 8) {
-      const int m = m0 + threadIdx.x % (NT * 8), grp = s * GROUPS + threadIdx.x / (NT * 8);
-      xsr = m < a.m && grp < a.groups ? a.xs[(int64_t)m * a.groups + grp] : 0.0f;
-    }
-  };
-  auto x_store = [&](int s) {
-    uint4* to = reinterpret_cast<uint4*>(xbuf + ((s - s0) & 1) * XBYTES);
+      // chunk (8 k) of row m, where the warps read it: [group, word][tile of 8 rows][row][thread of the quad]
+      const int idx = i * kThreads + threadIdx.x, row = idx / (kStageK / 8), k = idx % (kStageK / 8) * 8, in = k % G, th = in / (G / 4), word = in % (G / 4) / 8;
+      const uint32_t to = dst + S::X_AT + ((((k / G * WORDS + word) * NT + row / 8) * 8 + row % 8) * 4 + th) * S::X_CHUNK;
+      const bool take = m0 + row < a.m && s * kStageK + k < a.k;
+      const uint8_t* src = static_cast<const uint8_t*>(a.x) + (take ? ((int64_t)(m0 + row) * a.x_stride + s * kStageK + k) * (S::X_CHUNK / 8) : 0);
+      if (a.x_vec) {
+        if (S::X_CHUNK == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(take ? 16 : 0) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(src), "r"(take ? 8 : 0) : "memory");
+      } else {
+        uint8_t* out = smem + (to - smem_at);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) to[x_place(i * kThreads + threadIdx.x)] = x_pairs(xr[i], a.x_type);
-    if (a.xs_groups > 1 && threadIdx.x < GROUPS * NT * 8) reinterpret_cast<float*>(to + NT * 8 * kStageK / 8)[threadIdx.x] = xsr;
+        for (int e = 0; e < 8; ++e) {
+          if (S::X_CHUNK == 16) reinterpret_cast<uint16_t*>(out)[e] = take ? reinterpret_cast<const uint16_t*>(src)[e] : (uint16_t)0;
+          else out[e] = take ? src[e] : (uint8_t)0;
+        }
+      }
+    }
+    if (XK >= X_E4M3 && a.xs_groups > 1 && threadIdx.x < GROUPS * NT * 8) {
+      const int m = m0 + threadIdx.x % (NT * 8), grp = s * GROUPS + threadIdx.x / (NT * 8);
+      const bool take = m < a.m && grp < a.groups;
+      copy4(dst + S::XS_AT + threadIdx.x * 4, a.xs + (take ? (int64_t)m * a.groups + grp : 0), take ? 4 : 0);
+    }
+    if (a.s_vec) {  // 16-bit scales, every row's stage in one aligned piece
+      if (threadIdx.x < kRows) {
+        const void* from = static_cast<const uint8_t*>(a.s) + ((int64_t)min(n0 + (int)threadIdx.x, a.n - 1) * a.groups + s * GROUPS) * 2;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + S::S_AT + threadIdx.x * S::S_PITCH), "l"(from), "n"(GROUPS * 2) : "memory");
+      }
+    } else {
+      row_pieces(dst + S::S_AT + srow * S::S_PITCH, sc_row + s * (GROUPS * s_bytes), GROUPS * s_bytes, sc_end);
+    }
+    if (a.z_vec) {
+      if (GROUPS >= 4 && threadIdx.x >= kRows) {
+        const void* from = a.z + (int64_t)min(n0 + (int)threadIdx.x - kRows, a.n - 1) * a.groups + s * GROUPS;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + S::Z_AT + (threadIdx.x - kRows) * S::Z_PITCH), "l"(from), "n"(GROUPS >= 4 ? GROUPS : 4) : "memory");
+      }
+    } else if (a.z) {
+      row_pieces(dst + S::Z_AT + srow * S::Z_PITCH, z_row + s * GROUPS, GROUPS, z_end);
+    }
   };
-  // scales and zero points of the thread's four rows (32 * wr + pg, + 8, + 16, + 24) in its half of the stage: lane t of a quad holds group t
-  uint32_t sc[4], zp[4];
-  int64_t row_at[4];
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (s0 + i < s1) issue(s0 + i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  // this thread's rows: 32 * wr + pg, + 8, + 16, + 24; where their scales and zero points lie in a stage
+  int sc_at[4];
+  uintptr_t z_mis[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int row = n0 + wr * 32 + pg + 8 * r;
-    row_at[r] = row < a.n ? (int64_t)row * a.groups + (t & (HALF - 1)) : -1;
+    const int row = wr * 32 + pg + 8 * r;
+    const int64_t at = (int64_t)min(n0 + row, a.n - 1) * a.groups;
+    sc_at[r] = S::S_AT + row * S::S_PITCH + (int)((reinterpret_cast<uintptr_t>(a.s) + at * s_bytes) & 3) + wk * HALF * s_bytes;
+    z_mis[r] = reinterpret_cast<uintptr_t>(a.z) + at;
   }
-  auto scale_load = [&](int s) {
-    const int grp = s * GROUPS + wk * HALF;
-    const bool in = grp + (t & (HALF - 1)) < a.groups;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool take = in && row_at[r] >= 0;
-      sc[r] = take ? raw_of(a.s, row_at[r] + grp, a.s_type) : 0u;
-      zp[r] = take && a.z ? a.z[row_at[r] + grp] : 8u;
-    }
-  };
 
   float sum[2][NT][4];
 #pragma unroll
@@ -193,32 +232,30 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sum[mt][nt][0] = sum[mt][nt][1] = sum[mt][nt][2] = sum[mt][nt][3] = 0.0f;
 
-  if (s0 < s1) {
-    x_load(s0);
-    scale_load(s0);
-    x_store(s0);
-    if (s0 + 1 < s1) x_load(s0 + 1);
-  }
+  uint32_t magic = BF ? 0x43004300u : 0x64006400u;
+  asm volatile("" : "+r"(magic));  // (kept in a register)
+  const Zero eight = zero_of<BF>(8);
+  const bool xs_many = XK >= X_E4M3 && a.xs_groups > 1;
+  __syncthreads();  // the barriers are there
   for (int s = s0; s < s1; ++s) {
-    float scn[4];
-    uint32_t zn[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) scn[r] = value_of(sc[r], a.s_type), zn[r] = zero_of<BF>(zp[r] & 15u);
-    __syncthreads();  // stage s - 1 is read, x of stage s is there (and, at first, the barriers are)
-    if (threadIdx.x == 0 && s + kStages - 1 < s1) issue(s + kStages - 1);
-    if (s + 1 < s1) {
-      x_store(s + 1);
-      if (s + 2 < s1) x_load(s + 2);
-      scale_load(s + 1);
-    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     if (!mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1) && a.status) atomicCAS(a.status, 0, 8);
-    const uint8_t* wst = smem + ((s - s0) % kStages) * kStageBytes + (wr * 32 + pg) * kRowBytes;
-    const uint4* xst = reinterpret_cast<const uint4*>(xbuf + ((s - s0) & 1) * XBYTES) + lane;
+    __syncthreads();  // everybody's copies of stage s are there, and stage s - 1 is read
+    if (s + kStages - 1 < s1) {
+      if (threadIdx.x == 0) issue_q(s + kStages - 1);
+      issue(s + kStages - 1);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const uint8_t* st = smem + (s - s0) % kStages * S::BYTES;
+    const uint8_t *wst = st + (wr * 32 + pg) * kRowBytes, *xst = st + S::X_AT + lane * S::X_CHUNK;
+    const bool tail = (s + 1) * GROUPS > a.groups;  // groups behind the last one count as zero
 #pragma unroll
     for (int gi = 0; gi < HALF; ++gi) {
       const int byte = wk * (kRowBytes / 2) + gi * (G / 2) + t * (G / 8);  // of the row
       const uint8_t* p = wst + ((((byte >> 4) ^ pg) << 4) + (byte & 15));
       uint32_t w[4][WORDS];
+      Zero zero[4];
+      float sg[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (G == 128) {
@@ -230,15 +267,11 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
         } else {
           w[r][0] = *reinterpret_cast<const uint32_t*>(p + r * 8 * kRowBytes);
         }
-      }
-      const int from = (lane & ~3) | gi;
-      float sg[4];
-      uint32_t zg[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        sg[r] = HALF > 1 ? __shfl_sync(0xffffffffu, scn[r], from) : scn[r];
-        zg[r] = zn[r];
-        if (HALF > 1 && a.z) zg[r] = __shfl_sync(0xffffffffu, zn[r], from);
+        const uint8_t* sp = st + sc_at[r] + gi * s_bytes;
+        sg[r] = value_of(a.s_type == IB200_F32 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp), a.s_type);
+        if (tail && s * GROUPS + wk * HALF + gi >= a.groups) sg[r] = 0.0f;
+        zero[r] = eight;
+        if (a.z) zero[r] = zero_of<BF>(st[S::Z_AT + (wr * 32 + pg + 8 * r) * S::Z_PITCH + (int)((z_mis[r] + s * GROUPS) & 3) + wk * HALF + gi] & 15u);
       }
       float acc[2][NT][4];
 #pragma unroll
@@ -249,12 +282,12 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
       for (int k = 0; k < WORDS; ++k) {
         uint4 x[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) x[nt] = xst[(((wk * HALF + gi) * WORDS + k) * NT + nt) * 32];
+        for (int nt = 0; nt < NT; ++nt) x[nt] = x_pairs<XK>(xst + (((wk * HALF + gi) * WORDS + k) * NT + nt) * 32 * S::X_CHUNK);
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           uint32_t va[4], vb[4];
-          weights_of<BF>(w[2 * mt][k], zg[2 * mt], va);
-          weights_of<BF>(w[2 * mt + 1][k], zg[2 * mt + 1], vb);
+          weights_of<BF>(w[2 * mt][k], zero[2 * mt], magic, va);
+          weights_of<BF>(w[2 * mt + 1][k], zero[2 * mt + 1], magic, vb);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             mma<BF>(acc[mt][nt], va[0], vb[0], va[1], vb[1], x[nt].x, x[nt].y);
@@ -265,17 +298,17 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float2 f = make_float2(1.0f, 1.0f);
-        if (a.xs_groups > 1)
-          f = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(xst - lane + NT * 8 * kStageK / 8) + (wk * HALF + gi) * NT * 8 + nt * 8 + 2 * t);
+        if (xs_many) f = *reinterpret_cast<const float2*>(st + S::XS_AT + ((wk * HALF + gi) * NT * 8 + nt * 8 + 2 * t) * 4);
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sum[mt][nt][c] = fmaf(acc[mt][nt][c], a.xs_groups > 1 ? sg[2 * mt + (c >> 1)] * (c & 1 ? f.y : f.x) : sg[2 * mt + (c >> 1)], sum[mt][nt][c]);
+          for (int c = 0; c < 4; ++c) sum[mt][nt][c] = fmaf(acc[mt][nt][c], xs_many ? sg[2 * mt + (c >> 1)] * (c & 1 ? f.y : f.x) : sg[2 * mt + (c >> 1)], sum[mt][nt][c]);
       }
     }
   }
 
   // ---- add up the cluster's slices and write --------------------------------------------------------------
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   float* box = reinterpret_cast<float*>(smem);  // [half of K][NT * 8][128] sums of this CTA
   constexpr int BOX = NT * 8 * kRows;
@@ -303,16 +336,19 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
   if (split > 1) cluster_arrive_wait();  // nobody leaves while its sums are read
 }
 
-template <bool BF, int NT, int G> int run_stream(W4Args a, cudaStream_t s) {
-  auto* kern = w4_stream_kernel<BF, NT, G>;
-  constexpr int SMEM = kStages * kStageBytes + 2 * NT * 8 * (kStageK * 2 + kStageK / G * 4);
+template <int XK, int NT, int G> int run_stream(W4Args a, cudaStream_t s) {
+  auto* kern = w4_stream_kernel<XK, NT, G>;
+  constexpr int SMEM = Stage<XK, NT, G>::kStages * Stage<XK, NT, G>::BYTES;
+  static_assert(SMEM <= 112 * 1024, "two CTAs per SM");
   IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
   // K is split over a cluster so that the CTAs, two per SM at a time, have as few stages one after the other as can be
   const int tiles = (a.n + kRows - 1) / kRows, stages = (a.k + kStageK - 1) / kStageK, mt = (a.m + NT * 8 - 1) / (NT * 8);
+  // CTAs that run at once in clusters of 1 .. 8, two to an SM (cudaOccupancyMaxActiveClusters: clusters stay within a GPC)
+  static const int kAtOnce[9] = {0, 296, 296, 279, 284, 280, 270, 259, 264};
   int split = 1;
   int64_t best = INT64_MAX;
   for (int i = 1; i <= 8 && (i == 1 || i <= stages); ++i) {
-    const int64_t rounds = ((int64_t)tiles * mt * i + 2 * kSmCount - 1) / (2 * kSmCount), cost = rounds * ((stages + i - 1) / i + 2);  // 2: begin and end
+    const int64_t rounds = ((int64_t)tiles * mt * i + kAtOnce[i] - 1) / kAtOnce[i], cost = rounds * ((stages + i - 1) / i + 2);  // 2: begin and end
     if (cost < best) best = cost, split = i;
   }
   CUtensorMap map = {};
@@ -334,15 +370,13 @@ template <bool BF, int NT, int G> int run_stream(W4Args a, cudaStream_t s) {
   IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a, map));
   return IB200_OK;
 }
-template <bool BF, int NT> int run_stream_group(const W4Args& a, cudaStream_t s) {
-  if (a.group == 128) return run_stream<BF, NT, 128>(a, s);
-  if (a.group == 64) return run_stream<BF, NT, 64>(a, s);
-  return run_stream<BF, NT, 32>(a, s);
+template <int XK, int NT> int run_stream_group(const W4Args& a, cudaStream_t s) {
+  if (a.group == 128) return run_stream<XK, NT, 128>(a, s);
+  if (a.group == 64) return run_stream<XK, NT, 64>(a, s);
+  return run_stream<XK, NT, 32>(a, s);
 }
-template <bool BF> int run_stream_rows(const W4Args& a, cudaStream_t s) {
-  if (a.m <= 8) return run_stream_group<BF, 1>(a, s);
-  if (a.m <= 16) return run_stream_group<BF, 2>(a, s);
-  return run_stream_group<BF, 4>(a, s);
+template <int XK> int run_stream_rows(const W4Args& a, cudaStream_t s) {
+  return a.m <= 8 ? run_stream_group<XK, 1>(a, s) : run_stream_group<XK, 2>(a, s);
 }
 
 }  // namespace
@@ -372,8 +406,13 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
   const int e = held ? 1 : 2;
   const bool x_vec = (reinterpret_cast<uintptr_t>(x) & (held ? 7 : 15)) == 0 && (m == 1 || x_stride * e % (held ? 8 : 16) == 0);
   W4Args a{x, static_cast<const uint8_t*>(q), scales, static_cast<const uint8_t*>(zeros), bias, xs, y, x_stride,
-           (int)m, (int)n, (int)k, (int)group, (int)groups, (int)xs_groups, x_dtype, s_dtype, out_dtype, x_vec, 1, status};
-  return x_dtype == IB200_BF16 ? run_stream_rows<true>(a, s) : run_stream_rows<false>(a, s);
+           (int)m, (int)n, (int)k, (int)group, (int)groups, (int)xs_groups, x_dtype, s_dtype, out_dtype, x_vec, 0, 0, 1, status};
+  const int per = kStageK / (int)group;  // groups of a stage
+  a.s_vec = s_dtype != IB200_F32 && groups % per == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * per) == 0;
+  a.z_vec = zeros && per >= 4 && groups % per == 0 && reinterpret_cast<uintptr_t>(zeros) % per == 0;
+  if (x_dtype == IB200_BF16) return run_stream_rows<X_BF16>(a, s);
+  if (x_dtype == IB200_F16) return run_stream_rows<X_F16>(a, s);
+  return x_dtype == IB200_E4M3 ? run_stream_rows<X_E4M3>(a, s) : run_stream_rows<X_I8>(a, s);
 }
 
 }  // namespace ib200
