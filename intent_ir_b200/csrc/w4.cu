@@ -47,8 +47,8 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
 // the G / 4 adjacent k from t * G / 4, one 32-bit word of q (8 k) per two products, which keeps every product inside one
 // group; the group's sum is then scaled in f32.  A word gives pairs (0, 4), (1, 5), (2, 6), (3, 7), so x is laid down in that order, in
 // the order in which the warps read it.  128 + q in bf16 (1024 + q in f16) is q under the exponent of 128 (1024); minus 128 + z it is exact.
-// x, scales and zero points come by cp.async as far ahead as the weights: a load that a warp waits for costs more than a stage's work.
-constexpr int kRows = 128, kThreads = 256, kStageK = 256, kRowBytes = kStageK / 2;
+// A ninth warp brings everything: the weights as said, x, scales and zero points by cp.async; it and the others meet at mbarriers only.
+constexpr int kRows = 128, kThreads = 288, kStageK = 256, kRowBytes = kStageK / 2;
 enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
 template <int XK, int NT, int G> struct Stage {  // bytes of a stage's parts
   static constexpr int kStages = NT == 1 ? 4 : 3, GROUPS = kStageK / G;
@@ -136,85 +136,89 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
   constexpr int GROUPS = S::GROUPS, HALF = GROUPS / 2, WORDS = G / 32;  // groups of a stage, of a warp's half; words of a thread in a group
   constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ uint64_t full[kStages];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wr = warp & 3, wk = warp >> 2, pg = row_of<G>(g);
+  __shared__ uint64_t full[kStages], empty[kStages];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wr = warp & 3, wk = (warp >> 2) & 1, pg = row_of<G>(g);
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kRows, m0 = blockIdx.y * NT * 8;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
-  const uint32_t smem_at = smem_addr(smem);
-
-  auto issue_q = [&](int s) {  // (one thread)
-    const int i = (s - s0) % kStages;
-    mbarrier_expect_tx(&full[i], kRows * kRowBytes);
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(smem_at + i * S::BYTES), "l"(&map), "r"(smem_addr(&full[i])), "r"(s * kRowBytes), "r"(n0) : "memory");
+  const int s_bytes = a.s_type == IB200_F32 ? 4 : 2;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!mbarrier_wait_bounded(bar, parity) && a.status) atomicCAS(a.status, 0, 8);
   };
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1);
+    for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 8);
     mbarrier_init_fence();
-    for (int i = 0; i < kStages - 1; ++i)
-      if (s0 + i < s1) issue_q(s0 + i);
   }
-  // The other operands.  Two threads share a row of scales and zero points and take every other 4 bytes of it, from the 4-byte boundary
-  // in front of the stage's first group to the one behind its last, never beyond the end of the array.
-  const int srow = threadIdx.x >> 1, s_bytes = a.s_type == IB200_F32 ? 4 : 2;
-  const int64_t first = (int64_t)min(n0 + srow, a.n - 1) * a.groups;
-  const uint8_t *sc_row = static_cast<const uint8_t*>(a.s) + first * s_bytes, *sc_end = static_cast<const uint8_t*>(a.s) + (int64_t)a.n * a.groups * s_bytes;
-  const uint8_t *z_row = a.z + first, *z_end = a.z + (int64_t)a.n * a.groups;
-  auto row_pieces = [&](uint32_t dst, const uint8_t* from, int bytes, const uint8_t* end) {
-    const uint8_t *p = from - (reinterpret_cast<uintptr_t>(from) & 3) + (threadIdx.x & 1) * 4, *stop = from + bytes;
-    for (dst += (threadIdx.x & 1) * 4; p < stop; p += 8, dst += 8) {
-      const int left = (int)(end - p);
-      copy4(dst, left > 0 ? p : from - (reinterpret_cast<uintptr_t>(from) & 3), min(4, max(0, left)));
-    }
-  };
-  auto issue = [&](int s) {
-    const uint32_t dst = smem_at + (s - s0) % kStages * S::BYTES;
+  __syncthreads();
+  float sum[2][NT][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      // chunk (8 k) of row m, where the warps read it: [group, word][tile of 8 rows][row][thread of the quad]
-      const int idx = i * kThreads + threadIdx.x, row = idx / (kStageK / 8), k = idx % (kStageK / 8) * 8, in = k % G, th = in / (G / 4), word = in % (G / 4) / 8;
-      const uint32_t to = dst + S::X_AT + ((((k / G * WORDS + word) * NT + row / 8) * 8 + row % 8) * 4 + th) * S::X_CHUNK;
-      const bool take = m0 + row < a.m && s * kStageK + k < a.k;
-      const uint8_t* src = static_cast<const uint8_t*>(a.x) + (take ? ((int64_t)(m0 + row) * a.x_stride + s * kStageK + k) * (S::X_CHUNK / 8) : 0);
-      if (a.x_vec) {
-        if (S::X_CHUNK == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(take ? 16 : 0) : "memory");
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(src), "r"(take ? 8 : 0) : "memory");
-      } else {
-        uint8_t* out = smem + (to - smem_at);
+  for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (S::X_CHUNK == 16) reinterpret_cast<uint16_t*>(out)[e] = take ? reinterpret_cast<const uint16_t*>(src)[e] : (uint16_t)0;
-          else out[e] = take ? src[e] : (uint8_t)0;
+    for (int nt = 0; nt < NT; ++nt) sum[mt][nt][0] = sum[mt][nt][1] = sum[mt][nt][2] = sum[mt][nt][3] = 0.0f;
+
+  if (warp == 8) {
+    // ---- the bringing warp ----------------------------------------------------------------------------------
+    const uint32_t smem_at = smem_addr(smem);
+    // scales and zero points that are not in aligned pieces: 4 bytes at a time, from the 4-byte boundary in front of a row's first group of
+    // the stage to the one behind its last, never beyond the end of the array
+    auto row_pieces = [&](uint32_t dst, const uint8_t* from, int bytes, const uint8_t* end) {
+      const int mis = (int)(reinterpret_cast<uintptr_t>(from) & 3), left = (int)min((int64_t)(bytes + 4), (int64_t)(end - from));
+      for (int i = -mis; i < bytes; i += 4) copy4(dst + mis + i, i < left ? from + i : from - mis, max(0, min(4, left - i)));
+    };
+    for (int s = s0; s < s1; ++s) {
+      const int i = (s - s0) % kStages;
+      if (s - s0 >= kStages) wait(&empty[i], ((s - s0) / kStages - 1) & 1);
+      const uint32_t dst = smem_at + i * S::BYTES;
+      if (lane == 0) {
+        mbarrier_expect_tx(&full[i], kRows * kRowBytes);
+        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(&map), "r"(smem_addr(&full[i])), "r"(s * kRowBytes), "r"(n0) : "memory");
+      }
+      // x: lane l has the chunk (8 k) 8 l of each row, placed where the warps read it: [group, word][tile of 8 rows][row][thread of the quad]
+      const int k = lane * 8, in = k % G, th = in / (G / 4), word = in % (G / 4) / 8;
+      const uint32_t to0 = dst + S::X_AT + ((k / G * WORDS + word) * NT * 32 + th) * S::X_CHUNK;
+      const bool k_in = s * kStageK + k < a.k;
+      const uint8_t* x0 = static_cast<const uint8_t*>(a.x) + (k_in ? ((int64_t)m0 * a.x_stride + s * kStageK + k) * (S::X_CHUNK / 8) : 0);
+#pragma unroll 8
+      for (int row = 0; row < NT * 8; ++row) {
+        const uint32_t to = to0 + row * 4 * S::X_CHUNK;
+        const bool take = k_in && m0 + row < a.m;
+        const uint8_t* src = take ? x0 + (int64_t)row * a.x_stride * (S::X_CHUNK / 8) : static_cast<const uint8_t*>(a.x);
+        if (a.x_vec) {
+          if (S::X_CHUNK == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(take ? 16 : 0) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(src), "r"(take ? 8 : 0) : "memory");
+        } else {
+          uint8_t* out = smem + (to - smem_at);
+          for (int e = 0; e < 8; ++e) {
+            if (S::X_CHUNK == 16) reinterpret_cast<uint16_t*>(out)[e] = take ? reinterpret_cast<const uint16_t*>(src)[e] : (uint16_t)0;
+            else out[e] = take ? src[e] : (uint8_t)0;
+          }
         }
       }
-    }
-    if (XK >= X_E4M3 && a.xs_groups > 1 && threadIdx.x < GROUPS * NT * 8) {
-      const int m = m0 + threadIdx.x % (NT * 8), grp = s * GROUPS + threadIdx.x / (NT * 8);
-      const bool take = m < a.m && grp < a.groups;
-      copy4(dst + S::XS_AT + threadIdx.x * 4, a.xs + (take ? (int64_t)m * a.groups + grp : 0), take ? 4 : 0);
-    }
-    if (a.s_vec) {  // 16-bit scales, every row's stage in one aligned piece
-      if (threadIdx.x < kRows) {
-        const void* from = static_cast<const uint8_t*>(a.s) + ((int64_t)min(n0 + (int)threadIdx.x, a.n - 1) * a.groups + s * GROUPS) * 2;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + S::S_AT + threadIdx.x * S::S_PITCH), "l"(from), "n"(GROUPS * 2) : "memory");
+      if (!a.x_vec) __threadfence_block();
+      if (XK >= X_E4M3 && a.xs_groups > 1) {
+        for (int e = lane; e < GROUPS * NT * 8; e += 32) {
+          const int m = m0 + e % (NT * 8), grp = s * GROUPS + e / (NT * 8);
+          const bool take = m < a.m && grp < a.groups;
+          copy4(dst + S::XS_AT + e * 4, a.xs + (take ? (int64_t)m * a.groups + grp : 0), take ? 4 : 0);
+        }
       }
-    } else {
-      row_pieces(dst + S::S_AT + srow * S::S_PITCH, sc_row + s * (GROUPS * s_bytes), GROUPS * s_bytes, sc_end);
-    }
-    if (a.z_vec) {
-      if (GROUPS >= 4 && threadIdx.x >= kRows) {
-        const void* from = a.z + (int64_t)min(n0 + (int)threadIdx.x - kRows, a.n - 1) * a.groups + s * GROUPS;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + S::Z_AT + (threadIdx.x - kRows) * S::Z_PITCH), "l"(from), "n"(GROUPS >= 4 ? GROUPS : 4) : "memory");
+#pragma unroll
+      for (int j = 0; j < kRows / 32; ++j) {
+        const int r = j * 32 + lane;
+        const int64_t at = (int64_t)min(n0 + r, a.n - 1) * a.groups + s * GROUPS;
+        const uint8_t* from = static_cast<const uint8_t*>(a.s) + at * s_bytes;
+        const uint32_t sdst = dst + S::S_AT + r * S::S_PITCH;
+        if (a.s_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(sdst), "l"(from), "n"(GROUPS * 2) : "memory");
+        else row_pieces(sdst, from, GROUPS * s_bytes, static_cast<const uint8_t*>(a.s) + (int64_t)a.n * a.groups * s_bytes);
+        if (a.z) {
+          const uint32_t zdst = dst + S::Z_AT + r * S::Z_PITCH;
+          if (a.z_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(zdst), "l"(a.z + at), "n"(GROUPS >= 4 ? GROUPS : 4) : "memory");
+          else row_pieces(zdst, a.z + at, GROUPS, a.z + (int64_t)a.n * a.groups);
+        }
       }
-    } else if (a.z) {
-      row_pieces(dst + S::Z_AT + srow * S::Z_PITCH, z_row + s * GROUPS, GROUPS, z_end);
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
     }
-  };
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (s0 + i < s1) issue(s0 + i);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-
+  } else {
   // this thread's rows: 32 * wr + pg, + 8, + 16, + 24; where their scales and zero points lie in a stage
   int sc_at[4];
   uintptr_t z_mis[4];
@@ -226,29 +230,44 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
     z_mis[r] = reinterpret_cast<uintptr_t>(a.z) + at;
   }
 
-  float sum[2][NT][4];
-#pragma unroll
-  for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sum[mt][nt][0] = sum[mt][nt][1] = sum[mt][nt][2] = sum[mt][nt][3] = 0.0f;
-
   uint32_t magic = BF ? 0x43004300u : 0x64006400u;
   asm volatile("" : "+r"(magic));  // (kept in a register)
   const Zero eight = zero_of<BF>(8);
   const bool xs_many = XK >= X_E4M3 && a.xs_groups > 1;
-  __syncthreads();  // the barriers are there
   for (int s = s0; s < s1; ++s) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    if (!mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1) && a.status) atomicCAS(a.status, 0, 8);
-    __syncthreads();  // everybody's copies of stage s are there, and stage s - 1 is read
-    if (s + kStages - 1 < s1) {
-      if (threadIdx.x == 0) issue_q(s + kStages - 1);
-      issue(s + kStages - 1);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    wait(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
     const uint8_t* st = smem + (s - s0) % kStages * S::BYTES;
     const uint8_t *wst = st + (wr * 32 + pg) * kRowBytes, *xst = st + S::X_AT + lane * S::X_CHUNK;
-    const bool tail = (s + 1) * GROUPS > a.groups;  // groups behind the last one count as zero
+    // scales and zero points of the half's groups: one read of a row where they are in aligned pieces; groups behind the last one count as zero
+    uint32_t sraw[4][HALF], zraw[4];  // zero points: a byte each
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint8_t *sp = st + sc_at[r], *zp = st + S::Z_AT + (wr * 32 + pg + 8 * r) * S::Z_PITCH + (int)((z_mis[r] + s * GROUPS) & 3) + wk * HALF;
+      if (a.s_vec) {
+        if (HALF == 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(sp);
+          sraw[r][0] = v.x & 0xffffu, sraw[r][HALF > 1 ? 1 : 0] = v.x >> 16, sraw[r][HALF > 2 ? 2 : 0] = v.y & 0xffffu, sraw[r][HALF > 3 ? 3 : 0] = v.y >> 16;
+        } else if (HALF == 2) {
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(sp);
+          sraw[r][0] = v & 0xffffu, sraw[r][HALF > 1 ? 1 : 0] = v >> 16;
+        } else {
+          sraw[r][0] = *reinterpret_cast<const uint16_t*>(sp);
+        }
+      } else {
+#pragma unroll
+        for (int gi = 0; gi < HALF; ++gi) {
+          sraw[r][gi] = s_bytes == 4 ? *reinterpret_cast<const uint32_t*>(sp + gi * 4) : *reinterpret_cast<const uint16_t*>(sp + gi * 2);
+          if (s * GROUPS + wk * HALF + gi >= a.groups) sraw[r][gi] = 0;
+        }
+      }
+      zraw[r] = 0;
+      if (a.z) {
+#pragma unroll
+        for (int gi = 0; gi < HALF; ++gi)
+          if (!(a.z_vec && HALF == 4)) zraw[r] |= (uint32_t)zp[gi] << (8 * gi);
+        if (a.z_vec && HALF == 4) zraw[r] = *reinterpret_cast<const uint32_t*>(zp);
+      }
+    }
 #pragma unroll
     for (int gi = 0; gi < HALF; ++gi) {
       const int byte = wk * (kRowBytes / 2) + gi * (G / 2) + t * (G / 8);  // of the row
@@ -267,11 +286,8 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
         } else {
           w[r][0] = *reinterpret_cast<const uint32_t*>(p + r * 8 * kRowBytes);
         }
-        const uint8_t* sp = st + sc_at[r] + gi * s_bytes;
-        sg[r] = value_of(a.s_type == IB200_F32 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp), a.s_type);
-        if (tail && s * GROUPS + wk * HALF + gi >= a.groups) sg[r] = 0.0f;
-        zero[r] = eight;
-        if (a.z) zero[r] = zero_of<BF>(st[S::Z_AT + (wr * 32 + pg + 8 * r) * S::Z_PITCH + (int)((z_mis[r] + s * GROUPS) & 3) + wk * HALF + gi] & 15u);
+        sg[r] = value_of(sraw[r][gi], a.s_type);
+        zero[r] = a.z ? zero_of<BF>(zraw[r] >> (8 * gi) & 15u) : eight;
       }
       float acc[2][NT][4];
 #pragma unroll
@@ -305,13 +321,16 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
           for (int c = 0; c < 4; ++c) sum[mt][nt][c] = fmaf(acc[mt][nt][c], xs_many ? sg[2 * mt + (c >> 1)] * (c & 1 ? f.y : f.x) : sg[2 * mt + (c >> 1)], sum[mt][nt][c]);
       }
     }
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&empty[(s - s0) % kStages])) : "memory");
+  }
   }
 
   // ---- add up the cluster's slices and write --------------------------------------------------------------
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   float* box = reinterpret_cast<float*>(smem);  // [half of K][NT * 8][128] sums of this CTA
   constexpr int BOX = NT * 8 * kRows;
+  if (warp < 8)
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
