@@ -3,6 +3,10 @@
 // q is [N, K/2], the even k of a byte in its low half; z is 8 where there are no zero points; xs (the scales of 8-bit
 // activations) is 1, one value per row, or one per row and group.  x * (q - z) is exact in f32 (and in the 16-bit types),
 // sums are f32.
+#include <array>
+#include <map>
+#include <mutex>
+
 #include "async.cuh"
 #include "common.cuh"
 #include "held8.cuh"
@@ -39,6 +43,9 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
+#ifndef W4_STREAM
+#define W4_STREAM 16
+#endif
 // ---- few rows of x: weights stream through shared memory into mma.sync ----------------------------------
 // A CTA has 128 rows of q, four warps of 32 on each half of a stage's 256 k, and a slice of K; the CTAs of a cluster share the rows and split K, and
 // add their sums up through distributed shared memory in a fixed order.  One tensor copy brings a stage of q (128 rows x
@@ -50,6 +57,7 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
 // A ninth warp brings everything: the weights as said, x, scales and zero points by cp.async; it and the others meet at mbarriers only.
 constexpr int kRows = 128, kThreads = 288, kStageK = 256, kRowBytes = kStageK / 2;
 enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
+constexpr int kStreamRows = W4_STREAM;  // rows of x up to which the weights stream into mma.sync
 template <int XK, int NT, int G> struct Stage {  // bytes of a stage's parts
   static constexpr int kStages = NT == 1 ? 4 : 3, GROUPS = kStageK / G;
   static constexpr int X_CHUNK = XK >= X_E4M3 ? 8 : 16;                     // 8 k of a row
@@ -125,6 +133,40 @@ __device__ __forceinline__ float value_of(uint32_t raw, int type) {
   return __uint_as_float(type == IB200_BF16 ? raw << 16 : raw);
 }
 
+__device__ __forceinline__ void tensor_copy(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y) : "memory");
+}
+// A warp's copies of a stage's scales and zero points.  Where they are not in aligned pieces: 4 bytes at a time, from the 4-byte
+// boundary in front of a row's first group of the stage to the one behind its last, never beyond the end of the array.
+__device__ __forceinline__ void copy_row(uint32_t dst, const uint8_t* from, int bytes, const uint8_t* end) {
+  const int mis = (int)(reinterpret_cast<uintptr_t>(from) & 3), left = (int)min((int64_t)(bytes + 4), (int64_t)(end - from));
+  for (int i = -mis; i < bytes; i += 4) copy4(dst + mis + i, i < left ? from + i : from - mis, max(0, min(4, left - i)));
+}
+template <int GROUPS, int ROWS, typename S> __device__ __forceinline__ void bring_scales(const W4Args& a, uint32_t dst, int n0, int s, int lane) {
+  const int s_bytes = a.s_type == IB200_F32 ? 4 : 2;
+#pragma unroll
+  for (int j = 0; j < ROWS / 32; ++j) {
+    const int r = j * 32 + lane;
+    const int64_t at = (int64_t)min(n0 + r, a.n - 1) * a.groups + s * GROUPS;
+    const uint8_t* from = static_cast<const uint8_t*>(a.s) + at * s_bytes;
+    const uint32_t s_dst = dst + S::S_AT + r * S::S_PITCH, z_dst = dst + S::Z_AT + r * S::Z_PITCH;
+    if (a.s_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(s_dst), "l"(from), "n"(GROUPS * 2) : "memory");
+    else copy_row(s_dst, from, GROUPS * s_bytes, static_cast<const uint8_t*>(a.s) + (int64_t)a.n * a.groups * s_bytes);
+    if (a.z_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(z_dst), "l"(a.z + at), "n"(GROUPS >= 4 ? GROUPS : 4) : "memory");
+    else if (a.z) copy_row(z_dst, a.z + at, GROUPS, a.z + (int64_t)a.n * a.groups);
+  }
+}
+__device__ __forceinline__ void write_y(const W4Args& a, int m, int n, float v) {
+  if (n >= a.n) return;
+  if (a.xs_groups == 1) v *= a.xs[m];
+  if (a.bias) v += float_of(a.bias, n, a.y_type);
+  const int64_t at = (int64_t)m * a.n + n;
+  if (a.y_type == IB200_F32) static_cast<float*>(a.y)[at] = v;
+  else if (a.y_type == IB200_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(a.y)[at] = __float2half_rn(v);
+}
+
 // Row of a 16-row tile (below 8) that thread group g reads: with it, and the copy's swizzle (chunk ^ row % 8), eight lanes of a 16-byte
 // read and sixteen of an 8-byte one touch all banks once.
 template <int G> __device__ __forceinline__ int row_of(int g) { return G == 128 ? (g >> 1) + 4 * (g & 1) : G == 64 ? (g & 3) * 2 + (g >> 2) : g; }
@@ -158,20 +200,13 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
   if (warp == 8) {
     // ---- the bringing warp ----------------------------------------------------------------------------------
     const uint32_t smem_at = smem_addr(smem);
-    // scales and zero points that are not in aligned pieces: 4 bytes at a time, from the 4-byte boundary in front of a row's first group of
-    // the stage to the one behind its last, never beyond the end of the array
-    auto row_pieces = [&](uint32_t dst, const uint8_t* from, int bytes, const uint8_t* end) {
-      const int mis = (int)(reinterpret_cast<uintptr_t>(from) & 3), left = (int)min((int64_t)(bytes + 4), (int64_t)(end - from));
-      for (int i = -mis; i < bytes; i += 4) copy4(dst + mis + i, i < left ? from + i : from - mis, max(0, min(4, left - i)));
-    };
     for (int s = s0; s < s1; ++s) {
       const int i = (s - s0) % kStages;
       if (s - s0 >= kStages) wait(&empty[i], ((s - s0) / kStages - 1) & 1);
       const uint32_t dst = smem_at + i * S::BYTES;
       if (lane == 0) {
         mbarrier_expect_tx(&full[i], kRows * kRowBytes);
-        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                     ::"r"(dst), "l"(&map), "r"(smem_addr(&full[i])), "r"(s * kRowBytes), "r"(n0) : "memory");
+        tensor_copy(dst, &map, &full[i], s * kRowBytes, n0);
       }
       // x: lane l has the chunk (8 k) 8 l of each row, placed where the warps read it: [group, word][tile of 8 rows][row][thread of the quad]
       const int k = lane * 8, in = k % G, th = in / (G / 4), word = in % (G / 4) / 8;
@@ -202,20 +237,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
           copy4(dst + S::XS_AT + e * 4, a.xs + (take ? (int64_t)m * a.groups + grp : 0), take ? 4 : 0);
         }
       }
-#pragma unroll
-      for (int j = 0; j < kRows / 32; ++j) {
-        const int r = j * 32 + lane;
-        const int64_t at = (int64_t)min(n0 + r, a.n - 1) * a.groups + s * GROUPS;
-        const uint8_t* from = static_cast<const uint8_t*>(a.s) + at * s_bytes;
-        const uint32_t sdst = dst + S::S_AT + r * S::S_PITCH;
-        if (a.s_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(sdst), "l"(from), "n"(GROUPS * 2) : "memory");
-        else row_pieces(sdst, from, GROUPS * s_bytes, static_cast<const uint8_t*>(a.s) + (int64_t)a.n * a.groups * s_bytes);
-        if (a.z) {
-          const uint32_t zdst = dst + S::Z_AT + r * S::Z_PITCH;
-          if (a.z_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(zdst), "l"(a.z + at), "n"(GROUPS >= 4 ? GROUPS : 4) : "memory");
-          else row_pieces(zdst, a.z + at, GROUPS, a.z + (int64_t)a.n * a.groups);
-        }
-      }
+      bring_scales<GROUPS, kRows, S>(a, dst, n0, s, lane);
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
     }
   } else {
@@ -344,45 +366,67 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
     float v = 0.0f;
     for (int r = 0; r < split; ++r)
       v += split > 1 ? cluster_read(box + idx, r) + cluster_read(box + BOX + idx, r) : box[idx] + box[BOX + idx];
-    if (n >= a.n) continue;
-    if (a.xs_groups == 1) v *= a.xs[m];
-    if (a.bias) v += float_of(a.bias, n, a.y_type);
-    const int64_t at = (int64_t)m * a.n + n;
-    if (a.y_type == IB200_F32) static_cast<float*>(a.y)[at] = v;
-    else if (a.y_type == IB200_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(a.y)[at] = __float2half_rn(v);
+    write_y(a, m, n, v);
   }
   if (split > 1) cluster_arrive_wait();  // nobody leaves while its sums are read
+}
+
+// K is split over a cluster so that the CTAs that run at once (clusters stay within a GPC, so larger ones fill the GPU less) have as
+// few stages one after the other as can be.
+int choose_split(const void* kern, int smem, int threads, int tiles, int mt, int stages, int* split) {
+  static std::mutex lock;
+  static std::map<std::pair<int, const void*>, std::array<int, 9>> known;
+  int dev = 0;
+  IB200_CUDA_OK(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> hold(lock);
+  auto it = known.find({dev, kern});
+  if (it == known.end()) {
+    IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    std::array<int, 9> at_once{};
+    for (int i = 1; i <= 8; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(i * 4 * kSmCount));
+      cfg.blockDim = dim3((unsigned)threads);
+      cfg.dynamicSmemBytes = (size_t)smem;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)i;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      IB200_CUDA_OK(cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg));
+      at_once[i] = clusters * i;
+    }
+    it = known.emplace(std::make_pair(dev, kern), at_once).first;
+  }
+  int64_t best = INT64_MAX;
+  for (int i = 1; i <= 8 && (i == 1 || i <= stages); ++i) {
+    if (it->second[i] <= 0) continue;
+    const int64_t rounds = ((int64_t)tiles * mt * i + it->second[i] - 1) / it->second[i], cost = rounds * ((stages + i - 1) / i + 2);  // 2: begin and end
+    if (cost < best) best = cost, *split = i;
+  }
+  return IB200_OK;
 }
 
 template <int XK, int NT, int G> int run_stream(W4Args a, cudaStream_t s) {
   auto* kern = w4_stream_kernel<XK, NT, G>;
   constexpr int SMEM = Stage<XK, NT, G>::kStages * Stage<XK, NT, G>::BYTES;
   static_assert(SMEM <= 112 * 1024, "two CTAs per SM");
-  IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-  // K is split over a cluster so that the CTAs, two per SM at a time, have as few stages one after the other as can be
   const int tiles = (a.n + kRows - 1) / kRows, stages = (a.k + kStageK - 1) / kStageK, mt = (a.m + NT * 8 - 1) / (NT * 8);
-  // CTAs that run at once in clusters of 1 .. 8, two to an SM (cudaOccupancyMaxActiveClusters: clusters stay within a GPC)
-  static const int kAtOnce[9] = {0, 296, 296, 279, 284, 280, 270, 259, 264};
-  int split = 1;
-  int64_t best = INT64_MAX;
-  for (int i = 1; i <= 8 && (i == 1 || i <= stages); ++i) {
-    const int64_t rounds = ((int64_t)tiles * mt * i + kAtOnce[i] - 1) / kAtOnce[i], cost = rounds * ((stages + i - 1) / i + 2);  // 2: begin and end
-    if (cost < best) best = cost, split = i;
-  }
+  if (int rc = choose_split(reinterpret_cast<const void*>(kern), SMEM, kThreads, tiles, mt, stages, &a.split)) return rc;
   CUtensorMap map = {};
   if (a.k > 0)
     if (int rc = make_byte_map(&map, a.q, a.n, a.k / 2, kRows)) return rc;
-  a.split = split;
-  if ((int64_t)tiles * split > INT32_MAX || mt > 65535) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: too many rows");
+  if ((int64_t)tiles * a.split > INT32_MAX || mt > 65535) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: too many rows");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * split), (unsigned)mt);
+  cfg.gridDim = dim3((unsigned)(tiles * a.split), (unsigned)mt);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.x = a.split;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -398,13 +442,336 @@ template <int XK> int run_stream_rows(const W4Args& a, cudaStream_t s) {
   return a.m <= 8 ? run_stream_group<XK, 1>(a, s) : run_stream_group<XK, 2>(a, s);
 }
 
+// ---- tensor memory ----------------------------------------------------------------------------------------
+template <int N> __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[N]);
+template <> __device__ __forceinline__ void tmem_load<16>(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(at) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+template <> __device__ __forceinline__ void tmem_load<32>(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(at) : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// K-major operand in shared memory, 128-byte swizzled rows, eight rows 1024 bytes apart
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t at) {
+  return (uint64_t)((at & 0x3FFFF) >> 4) | (uint64_t)(16 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// ---- more rows of x: weights widened into tensor memory, tcgen05.mma ----------------------------------------
+// D[128 rows of q, NX rows of x] per group of G, f32 in tensor memory:  A = the 128 x G widened weights (a thread widens its own
+// row and stores it to tensor memory, where the MMA reads it), B = x from shared memory (128-byte swizzle, K-major).  The sums of a group are read back
+// and scaled into f32 registers, one row to a thread, so nothing but x and q - z, both exact, enters the products.  A CTA has
+// two such blocks of 128 rows, so that a stage of x (L2 -> SM traffic) serves 256 rows, and a slice of K; clusters split K as above.
+//   warps 0-7  widen chunk i of their 32 rows, then scale the sums of chunk i - 1 (whose MMA ran meanwhile)
+//   warp 8     brings the operands; x comes permuted and widened by a small launch in front, on which only x's copies wait
+//   warp 9     one thread issues the MMAs
+// Chunk i's widened weights arriving says that chunk i - 2 has been read back, so its buffers need no barrier of their own.
+constexpr int kTcRows = 256, kTcThreads = 320;
+template <int NX, int G> struct TcStage {
+  static constexpr int GROUPS = kStageK / G;
+  static constexpr int X_AT = kTcRows * kRowBytes;                        // after q: x as four [NX rows][64 k]
+  static constexpr int XS_AT = X_AT + NX * kStageK * 2;                   // scales of x: [group][row]
+  static constexpr int S_PITCH = GROUPS * 4, S_AT = XS_AT + GROUPS * NX * 4;
+  static constexpr int Z_PITCH = (GROUPS + 3) / 4 * 4 + (GROUPS == 4 ? 4 : 8), Z_AT = S_AT + kTcRows * S_PITCH;
+  static constexpr int BYTES = (Z_AT + kTcRows * Z_PITCH + 1023) / 1024 * 1024;
+  static constexpr int kStages = 3 * BYTES <= 225 * 1024 ? 3 : 2;
+};
+
+// x as the MMA reads it: rows of k_pad 16-bit values, each eight in the order (0, 4, 1, 5, 2, 6, 3, 7), zero outside x
+template <int XK> __global__ void __launch_bounds__(256) w4_spread_kernel(const W4Args a, uint4* out, int rows, int chunks) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int SIZE = XK >= X_E4M3 ? 1 : 2;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * chunks; i += (int64_t)gridDim.x * 256) {
+    const int row = (int)(i / chunks), k = (int)(i - (int64_t)row * chunks) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < a.m && k < a.k) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.x) + ((int64_t)row * a.x_stride + k) * SIZE;
+      __align__(16) uint8_t e[16];
+      if (a.x_vec) {
+        if (SIZE == 2) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p);
+        else *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (SIZE == 2) reinterpret_cast<uint16_t*>(e)[j] = reinterpret_cast<const uint16_t*>(p)[j];
+          else e[j] = p[j];
+        }
+      }
+      v = x_pairs<XK>(e);
+    }
+    out[i] = v;
+  }
+}
+
+template <bool BF, int NX, int G>
+__global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_x) {
+  using S = TcStage<NX, G>;
+  constexpr int GROUPS = S::GROUPS, kStages = S::kStages, NA = 256 / G, ND = 128 / NX;  // groups of a stage; buffers of A (128 columns a block) and D
+  constexpr int A_AT = 256;                                                              // tensor memory: D of both blocks, then A of both
+  constexpr int LD = NX < 32 ? NX : 32;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint64_t full[kStages], empty[kStages], a_full[2][NA], d_full[2][ND];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int dead;  // a wait ran out: nothing waits any more
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kTcRows, m0 = blockIdx.y * NX;
+  const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
+  const int s_bytes = a.s_type == IB200_F32 ? 4 : 2;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (dead || mbarrier_wait_bounded(bar, parity)) return;
+    dead = 1;
+    if (a.status) atomicCAS(a.status, 0, 8);
+  };
+  auto arrive = [](uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory"); };
+  if (threadIdx.x == 0) {
+    dead = 0;
+    for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 8 + 1);
+    for (int b = 0; b < 2; ++b) {
+      for (int i = 0; i < NA; ++i) mbarrier_init(&a_full[b][i], 4);
+      for (int i = 0; i < ND; ++i) mbarrier_init(&d_full[b][i], 1);
+    }
+    mbarrier_init_fence();
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+
+  float sum[NX];
+#pragma unroll
+  for (int j = 0; j < NX; ++j) sum[j] = 0.0f;
+
+  if (warp == 8) {
+    // ---- the bringing warp ----------------------------------------------------------------------------------
+    const uint32_t smem_at = smem_addr(smem);
+    for (int s = s0; s < s1; ++s) {
+      const int i = (s - s0) % kStages;
+      if (s - s0 >= kStages) wait(&empty[i], ((s - s0) / kStages - 1) & 1);
+      const uint32_t dst = smem_at + i * S::BYTES;
+      if (lane == 0) {
+        mbarrier_expect_tx(&full[i], kTcRows * kRowBytes + NX * kStageK * 2);
+        tensor_copy(dst, &map_q, &full[i], s * kRowBytes, n0);
+      }
+      bring_scales<GROUPS, kTcRows, S>(a, dst, n0, s, lane);
+      if (a.xs_groups > 1) {
+        for (int e = lane; e < GROUPS * NX; e += 32) {
+          const int m = m0 + e % NX, grp = s * GROUPS + e / NX;
+          const bool take = m < a.m && grp < a.groups;
+          copy4(dst + S::XS_AT + e * 4, a.xs + (take ? (int64_t)m * a.groups + grp : 0), take ? 4 : 0);
+        }
+      }
+      if (lane == 0) {
+        if (s == s0) asm volatile("griddepcontrol.wait;\nfence.proxy.async;" ::: "memory");  // the launch that spreads x
+#pragma unroll
+        for (int j = 0; j < kStageK / 64; ++j) tensor_copy(dst + S::X_AT + j * NX * 128, &map_x, &full[i], s * kStageK * 2 + j * 128, m0);
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
+    }
+    if (dead)  // copies that are still on their way land before the CTA ends
+      for (int s = max(s0, s1 - kStages); s < s1; ++s) (void)mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
+  } else if (warp == 9) {
+    // ---- the MMA thread -------------------------------------------------------------------------------------
+    if (lane == 0) {
+      // f32 accumulators, both operands K-major, N = NX, M = 128
+      const uint32_t idesc = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((uint32_t)(NX >> 3) << 17) | ((128u >> 4) << 24);
+      int i = 0;
+      for (int s = s0; s < s1; ++s) {
+        const int st = (s - s0) % kStages;
+        wait(&full[st], ((s - s0) / kStages) & 1);
+        const uint32_t x_at = smem_addr(smem + st * S::BYTES + S::X_AT);
+        for (int c = 0; c < GROUPS; ++c, ++i) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            wait(&a_full[b][i % NA], (i / NA) & 1);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t d = tmem + b * 128 + (i % ND) * NX, w = tmem + A_AT + b * 128 + (i % NA) * (G / 2);
+#pragma unroll
+            for (int k = 0; k < G / 16; ++k) {
+              const int at = c * G + k * 16;  // k of the stage
+              asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                           ::"r"(d), "r"(w + k * 8), "l"(swizzled_desc(x_at + at / 64 * (NX * 128) + at % 64 * 2)), "r"(idesc), "r"(k ? 1 : 0) : "memory");
+            }
+            commit(&d_full[b][i % ND]);
+          }
+        }
+        commit(&empty[st]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- widen and scale ------------------------------------------------------------------------------------
+    const int b = warp >> 2, row = b * 128 + (warp & 3) * 32 + lane;  // the thread's row of q is its lane of tensor memory
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, d_at = tmem + lanes + b * 128, a_at = tmem + lanes + A_AT + b * 128;
+    const int64_t first = (int64_t)min(n0 + row, a.n - 1) * a.groups;
+    const int s_mis = (int)((reinterpret_cast<uintptr_t>(a.s) + first * s_bytes) & 3);
+    uint32_t magic = BF ? 0x43004300u : 0x64006400u;
+    asm volatile("" : "+r"(magic));  // (kept in a register)
+    const Zero eight = zero_of<BF>(8);
+    const bool xs_many = a.xs_groups > 1;
+    int i = 0, old_group = 0;
+    float old_scale = 0.0f;
+    const uint8_t* old_stage = smem;
+    auto scale_sums = [&](int j) {  // chunk j's
+      wait(&d_full[b][j % ND], (j / ND) & 1);
+      __syncwarp();  // (the loads below are the whole warp's)
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < NX / LD; ++c) {
+        uint32_t r[LD];
+        tmem_load<LD>(d_at + (j % ND) * NX + c * LD, r);
+        if (xs_many) {
+          const float4* f = reinterpret_cast<const float4*>(old_stage + S::XS_AT + (old_group * NX + c * LD) * 4);
+#pragma unroll
+          for (int e = 0; e < LD / 4; ++e) {
+            const float4 v = f[e];
+            sum[c * LD + 4 * e] = fmaf(__uint_as_float(r[4 * e]), old_scale * v.x, sum[c * LD + 4 * e]);
+            sum[c * LD + 4 * e + 1] = fmaf(__uint_as_float(r[4 * e + 1]), old_scale * v.y, sum[c * LD + 4 * e + 1]);
+            sum[c * LD + 4 * e + 2] = fmaf(__uint_as_float(r[4 * e + 2]), old_scale * v.z, sum[c * LD + 4 * e + 2]);
+            sum[c * LD + 4 * e + 3] = fmaf(__uint_as_float(r[4 * e + 3]), old_scale * v.w, sum[c * LD + 4 * e + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < LD; ++e) sum[c * LD + e] = fmaf(__uint_as_float(r[e]), old_scale, sum[c * LD + e]);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    };
+    for (int s = s0; s < s1; ++s) {
+      const uint8_t* st = smem + (s - s0) % kStages * S::BYTES;
+      wait(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
+      __syncwarp();
+      const int z_mis = (int)((reinterpret_cast<uintptr_t>(a.z) + first + s * GROUPS) & 3);
+#pragma unroll
+      for (int c = 0; c < GROUPS; ++c, ++i) {
+        const Zero zero = a.z ? zero_of<BF>(st[S::Z_AT + row * S::Z_PITCH + z_mis + c] & 15u) : eight;
+#pragma unroll
+        for (int q = 0; q < G / 32; ++q) {
+          const uint4 v = *reinterpret_cast<const uint4*>(st + row * kRowBytes + (((c * (G / 32) + q) ^ (row & 7)) << 4));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          uint32_t r[16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t p[4];
+            weights_of<BF>(w[k], zero, magic, p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[4 * k + e] = p[e];
+          }
+          tmem_store16(a_at + (i % NA) * (G / 2) + q * 16, r);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(&a_full[b][i % NA]);
+        const uint8_t* sp = st + S::S_AT + row * S::S_PITCH + s_mis + c * s_bytes;
+        float scale = value_of(s_bytes == 4 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp), a.s_type);
+        if (s * GROUPS + c >= a.groups) scale = 0.0f;  // behind the last group
+        if (i > 0) scale_sums(i - 1);
+        if (c == 0 && s > s0) {
+          __syncwarp();
+          if (lane == 0) arrive(&empty[(s - 1 - s0) % kStages]);
+        }
+        old_scale = scale;
+        old_stage = st;
+        old_group = c;
+      }
+    }
+    if (i > 0) scale_sums(i - 1);
+  }
+
+  // ---- add up the cluster's slices and write ----------------------------------------------------------------
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 9) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+  float* box = reinterpret_cast<float*>(smem);  // [NX][256] sums of this CTA
+  if (warp < 8) {
+#pragma unroll
+    for (int j = 0; j < NX; ++j) box[j * kTcRows + threadIdx.x] = sum[j];
+  }
+  if (split > 1) cluster_arrive_wait(); else __syncthreads();
+  const int rows = min(NX, a.m - m0);
+  for (int idx = rank * kTcThreads + threadIdx.x; idx < rows * kTcRows; idx += split * kTcThreads) {
+    const int m = m0 + idx / kTcRows, n = n0 + idx % kTcRows;
+    float v = 0.0f;
+    for (int r = 0; r < split; ++r) v += split > 1 ? cluster_read(box + idx, r) : box[idx];
+    write_y(a, m, n, v);
+  }
+  if (split > 1) cluster_arrive_wait();
+}
+
+int64_t padded(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int tc_columns(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
+
+template <int XK, int NX, int G> int run_tc(W4Args a, void* scratch, cudaStream_t s) {
+  constexpr bool BF = XK == X_BF16;
+  auto* kern = w4_tc_kernel<BF, NX, G>;
+  constexpr int SMEM = TcStage<NX, G>::kStages * TcStage<NX, G>::BYTES;
+  static_assert(SMEM <= 225 * 1024, "one CTA per SM");
+  const int64_t rows = padded(a.m, NX), k_pad = padded(a.k, kStageK);
+  CUtensorMap map_q, map_x;
+  if (int rc = make_byte_map(&map_q, a.q, a.n, a.k / 2, kTcRows)) return rc;
+  if (int rc = make_byte_map(&map_x, scratch, rows, k_pad * 2, NX)) return rc;
+  const int tiles = (a.n + kTcRows - 1) / kTcRows, mt = (int)(rows / NX);
+  if (mt > 65535) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: too many rows");
+  if (int rc = choose_split(reinterpret_cast<const void*>(kern), SMEM, kTcThreads, tiles, mt, (int)(k_pad / kStageK), &a.split)) return rc;
+  const int64_t blocks = (rows * (k_pad / 8) + 255) / 256;
+  w4_spread_kernel<XK><<<(unsigned)(blocks < kSmCount * 8 ? blocks : kSmCount * 8), 256, 0, s>>>(a, static_cast<uint4*>(scratch), (int)rows, (int)(k_pad / 8));
+  if (cudaPeekAtLastError() != cudaSuccess) return cuda_fail(cudaGetLastError(), "w4_matmul launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * a.split), (unsigned)mt);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a, map_q, map_x));
+  return IB200_OK;
+}
+template <int XK, int NX> int run_tc_group(const W4Args& a, void* scratch, cudaStream_t s) {
+  if (a.group == 128) return run_tc<XK, NX, 128>(a, scratch, s);
+  if (a.group == 64) return run_tc<XK, NX, 64>(a, scratch, s);
+  return run_tc<XK, NX, 32>(a, scratch, s);
+}
+template <int XK> int run_tc_rows(const W4Args& a, void* scratch, cudaStream_t s) {
+  const int nx = tc_columns(a.m);
+  if (nx == 16) return run_tc_group<XK, 16>(a, scratch, s);
+  return nx == 32 ? run_tc_group<XK, 32>(a, scratch, s) : run_tc_group<XK, 64>(a, scratch, s);
+}
+
 }  // namespace
 
-size_t w4_scratch_bytes(int, int64_t, int64_t, int64_t, int64_t) { return 0; }
+// room for x as the MMA reads it
+size_t w4_scratch_bytes(int, int64_t m, int64_t n, int64_t k, int64_t) {
+  if (m <= kStreamRows || n <= 0 || k <= 0 || beyond_any_device(m, k) || k > INT32_MAX - 1024) return 0;
+  return (size_t)(padded(m, tc_columns(m)) * padded(k, kStageK) * 2);
+}
 
 int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_groups, const void* q, const void* scales, const void* zeros,
               const void* bias, void* y, int x_dtype, int s_dtype, int out_dtype, int64_t m, int64_t n, int64_t k, int64_t group,
-              void*, size_t, int32_t* status, cudaStream_t s) {
+              void* scratch, size_t scratch_bytes, int32_t* status, cudaStream_t s) {
   if (m < 0 || n < 0 || k < 0) return fail(IB200_ERR_INVALID, "w4_matmul: negative extent");
   if (beyond_any_device(m, k) || beyond_any_device(n, k) || beyond_any_device(m, n)) return fail(IB200_ERR_INVALID, "w4_matmul: more than 2^40 elements");
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX - 1024) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: extents are below 2^31");
@@ -429,6 +796,12 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
   const int per = kStageK / (int)group;  // groups of a stage
   a.s_vec = s_dtype != IB200_F32 && groups % per == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * per) == 0;
   a.z_vec = zeros && per >= 4 && groups % per == 0 && reinterpret_cast<uintptr_t>(zeros) % per == 0;
+  if (m > kStreamRows && k > 0) {
+    if (!scratch || scratch_bytes < w4_scratch_bytes(x_dtype, m, n, k, group)) return fail(IB200_ERR_BUFFER, "w4_matmul: scratch is smaller than ib200_w4_scratch_bytes");
+    if (x_dtype == IB200_BF16) return run_tc_rows<X_BF16>(a, scratch, s);
+    if (x_dtype == IB200_F16) return run_tc_rows<X_F16>(a, scratch, s);
+    return x_dtype == IB200_E4M3 ? run_tc_rows<X_E4M3>(a, scratch, s) : run_tc_rows<X_I8>(a, scratch, s);
+  }
   if (x_dtype == IB200_BF16) return run_stream_rows<X_BF16>(a, s);
   if (x_dtype == IB200_F16) return run_stream_rows<X_F16>(a, s);
   return x_dtype == IB200_E4M3 ? run_stream_rows<X_E4M3>(a, s) : run_stream_rows<X_I8>(a, s);
