@@ -58,14 +58,14 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
 constexpr int kRows = 128, kThreads = 288, kStageK = 256, kRowBytes = kStageK / 2;
 enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
 constexpr int kStreamRows = W4_STREAM;  // rows of x up to which the weights stream into mma.sync
+constexpr int kBlockBytes = 48, kRowScales = 2 * kBlockBytes;  // a row's two blocks of eight scales and zero points
 template <int XK, int NT, int G> struct Stage {  // bytes of a stage's parts
   static constexpr int kStages = NT == 1 ? 4 : 3, GROUPS = kStageK / G;
   static constexpr int X_CHUNK = XK >= X_E4M3 ? 8 : 16;                     // 8 k of a row
   static constexpr int X_AT = kRows * kRowBytes;                              // after q: x in the order of its reads
   static constexpr int XS_AT = X_AT + NT * 8 * (kStageK / 8) * X_CHUNK;       // scales of x: [group][row]
-  static constexpr int S_PITCH = GROUPS * 4, S_AT = XS_AT + GROUPS * NT * 8 * 4;  // scales of a row: f32, or 16 bits and up to 2 bytes of slack
-  static constexpr int Z_PITCH = (GROUPS + 3) / 4 * 4 + (GROUPS == 4 ? 4 : 8), Z_AT = S_AT + kRows * S_PITCH;  // zero points and up to 3 bytes of slack
-  static constexpr int BYTES = (Z_AT + kRows * Z_PITCH + 1023) / 1024 * 1024;
+  static constexpr int BYTES = (XS_AT + GROUPS * NT * 8 * 4 + 1023) / 1024 * 1024;
+  static constexpr int S_AT = kStages * BYTES, SMEM = S_AT + 8 * 32 * kRowScales;  // behind the stages: every warp's rows' scales
 };
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {  // the rest of the 4 is zero
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -137,26 +137,61 @@ __device__ __forceinline__ void tensor_copy(uint32_t dst, const CUtensorMap* map
   asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y) : "memory");
 }
-// A warp's copies of a stage's scales and zero points.  Where they are not in aligned pieces: 4 bytes at a time, from the 4-byte
-// boundary in front of a row's first group of the stage to the one behind its last, never beyond the end of the array.
-__device__ __forceinline__ void copy_row(uint32_t dst, const uint8_t* from, int bytes, const uint8_t* end) {
-  const int mis = (int)(reinterpret_cast<uintptr_t>(from) & 3), left = (int)min((int64_t)(bytes + 4), (int64_t)(end - from));
-  for (int i = -mis; i < bytes; i += 4) copy4(dst + mis + i, i < left ? from + i : from - mis, max(0, min(4, left - i)));
-}
-template <int GROUPS, int ROWS, typename S> __device__ __forceinline__ void bring_scales(const W4Args& a, uint32_t dst, int n0, int s, int lane) {
-  const int s_bytes = a.s_type == IB200_F32 ? 4 : 2;
+// Scales and zero points of a row, eight groups at a time.  A thread reads a block of its row one block ahead of its use, into registers, and
+// leaves it as eight f32 and eight bytes in one of two places in shared memory, from where it is read group by group.  Groups
+// behind the last one, and rows behind the last, have the scale 0.
+struct RowBlock {
+  uint32_t s[8];
+  uint2 z;
+};
+__device__ __forceinline__ RowBlock read_block(const W4Args& a, int row, int block) {
+  RowBlock r;
+  const int g0 = block * 8;
 #pragma unroll
-  for (int j = 0; j < ROWS / 32; ++j) {
-    const int r = j * 32 + lane;
-    const int64_t at = (int64_t)min(n0 + r, a.n - 1) * a.groups + s * GROUPS;
-    const uint8_t* from = static_cast<const uint8_t*>(a.s) + at * s_bytes;
-    const uint32_t s_dst = dst + S::S_AT + r * S::S_PITCH, z_dst = dst + S::Z_AT + r * S::Z_PITCH;
-    if (a.s_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(s_dst), "l"(from), "n"(GROUPS * 2) : "memory");
-    else copy_row(s_dst, from, GROUPS * s_bytes, static_cast<const uint8_t*>(a.s) + (int64_t)a.n * a.groups * s_bytes);
-    if (a.z_vec) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(z_dst), "l"(a.z + at), "n"(GROUPS >= 4 ? GROUPS : 4) : "memory");
-    else if (a.z) copy_row(z_dst, a.z + at, GROUPS, a.z + (int64_t)a.n * a.groups);
+  for (int i = 0; i < 8; ++i) r.s[i] = 0;
+  r.z = make_uint2(0x08080808u, 0x08080808u);
+  if (row >= a.n || g0 >= a.groups) return r;
+  const int64_t at = (int64_t)row * a.groups + g0;
+  if (a.s_vec) {
+    if (a.s_type == IB200_F32) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(a.s) + at);
+      const uint4 u = p[0], v = p[1];
+      r.s[0] = u.x, r.s[1] = u.y, r.s[2] = u.z, r.s[3] = u.w, r.s[4] = v.x, r.s[5] = v.y, r.s[6] = v.z, r.s[7] = v.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.s) + at);
+      r.s[0] = u.x, r.s[1] = u.y, r.s[2] = u.z, r.s[3] = u.w;  // two to a word
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (g0 + i < a.groups) {
+        if (a.s_type == IB200_F32) r.s[i] = static_cast<const uint32_t*>(a.s)[at + i];
+        else r.s[i] = static_cast<const uint16_t*>(a.s)[at + i];
+      }
   }
+  if (a.z_vec) {
+    r.z = *reinterpret_cast<const uint2*>(a.z + at);
+  } else if (a.z) {
+    uint32_t z[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = g0 + i < a.groups ? a.z[at + i] : 8u;
+    r.z = make_uint2(z[0] | z[1] << 8 | z[2] << 16 | z[3] << 24, z[4] | z[5] << 8 | z[6] << 16 | z[7] << 24);
+  }
+  return r;
 }
+__device__ __forceinline__ void leave_block(const W4Args& a, uint8_t* row, int block, const RowBlock& r) {
+  uint8_t* to = row + (block & 1) * kBlockBytes;
+  const bool pairs = a.s_vec && a.s_type != IB200_F32;
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = value_of(pairs ? r.s[(i + e) / 2] >> (e & 1) * 16 & 0xffffu : r.s[i + e], a.s_type);
+    *reinterpret_cast<float4*>(to + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+  *reinterpret_cast<uint2*>(to + 32) = r.z;
+}
+
 __device__ __forceinline__ void write_y(const W4Args& a, int m, int n, float v) {
   if (n >= a.n) return;
   if (a.xs_groups == 1) v *= a.xs[m];
@@ -182,7 +217,6 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wr = warp & 3, wk = (warp >> 2) & 1, pg = row_of<G>(g);
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kRows, m0 = blockIdx.y * NT * 8;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
-  const int s_bytes = a.s_type == IB200_F32 ? 4 : 2;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (!mbarrier_wait_bounded(bar, parity) && a.status) atomicCAS(a.status, 0, 8);
   };
@@ -237,21 +271,17 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
           copy4(dst + S::XS_AT + e * 4, a.xs + (take ? (int64_t)m * a.groups + grp : 0), take ? 4 : 0);
         }
       }
-      bring_scales<GROUPS, kRows, S>(a, dst, n0, s, lane);
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
     }
   } else {
-  // this thread's rows: 32 * wr + pg, + 8, + 16, + 24; where their scales and zero points lie in a stage
-  int sc_at[4];
-  uintptr_t z_mis[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = wr * 32 + pg + 8 * r;
-    const int64_t at = (int64_t)min(n0 + row, a.n - 1) * a.groups;
-    sc_at[r] = S::S_AT + row * S::S_PITCH + (int)((reinterpret_cast<uintptr_t>(a.s) + at * s_bytes) & 3) + wk * HALF * s_bytes;
-    z_mis[r] = reinterpret_cast<uintptr_t>(a.z) + at;
-  }
-
+  // this thread's rows: 32 * wr + pg, + 8, + 16, + 24; lane t of a quad reads the scales of the one at 8 t for all four.  A warp's groups of a
+  // stage lie in one block.
+  uint8_t *scales = smem + S::S_AT + (warp * 32 + pg) * kRowScales, *mine = scales + 8 * t * kRowScales;
+  const int my_row = n0 + wr * 32 + pg + 8 * t;
+  int block = (s0 * GROUPS + wk * HALF) >> 3;
+  leave_block(a, mine, block, read_block(a, my_row, block));
+  RowBlock ahead = read_block(a, my_row, block + 1);
+  __syncwarp();
   uint32_t magic = BF ? 0x43004300u : 0x64006400u;
   asm volatile("" : "+r"(magic));  // (kept in a register)
   const Zero eight = zero_of<BF>(8);
@@ -260,34 +290,29 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
     wait(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
     const uint8_t* st = smem + (s - s0) % kStages * S::BYTES;
     const uint8_t *wst = st + (wr * 32 + pg) * kRowBytes, *xst = st + S::X_AT + lane * S::X_CHUNK;
-    // scales and zero points of the half's groups: one read of a row where they are in aligned pieces; groups behind the last one count as zero
-    uint32_t sraw[4][HALF], zraw[4];  // zero points: a byte each
+    const int group0 = s * GROUPS + wk * HALF;
+    if (group0 >> 3 != block) {
+      block = group0 >> 3;
+      leave_block(a, mine, block, ahead);
+      ahead = read_block(a, my_row, block + 1);
+      __syncwarp();
+    }
+    float sraw[4][HALF];
+    uint32_t zraw[4];  // zero points: a byte each
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint8_t *sp = st + sc_at[r], *zp = st + S::Z_AT + (wr * 32 + pg + 8 * r) * S::Z_PITCH + (int)((z_mis[r] + s * GROUPS) & 3) + wk * HALF;
-      if (a.s_vec) {
-        if (HALF == 4) {
-          const uint2 v = *reinterpret_cast<const uint2*>(sp);
-          sraw[r][0] = v.x & 0xffffu, sraw[r][HALF > 1 ? 1 : 0] = v.x >> 16, sraw[r][HALF > 2 ? 2 : 0] = v.y & 0xffffu, sraw[r][HALF > 3 ? 3 : 0] = v.y >> 16;
-        } else if (HALF == 2) {
-          const uint32_t v = *reinterpret_cast<const uint32_t*>(sp);
-          sraw[r][0] = v & 0xffffu, sraw[r][HALF > 1 ? 1 : 0] = v >> 16;
-        } else {
-          sraw[r][0] = *reinterpret_cast<const uint16_t*>(sp);
-        }
+      const uint8_t* from = scales + 8 * r * kRowScales + (block & 1) * kBlockBytes;
+      if (HALF == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(from + (group0 & 7) * 4);
+        sraw[r][0] = v.x, sraw[r][HALF > 1 ? 1 : 0] = v.y, sraw[r][HALF > 2 ? 2 : 0] = v.z, sraw[r][HALF > 3 ? 3 : 0] = v.w;
+        zraw[r] = *reinterpret_cast<const uint32_t*>(from + 32 + (group0 & 7));
+      } else if (HALF == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(from + (group0 & 7) * 4);
+        sraw[r][0] = v.x, sraw[r][HALF > 1 ? 1 : 0] = v.y;
+        zraw[r] = *reinterpret_cast<const uint16_t*>(from + 32 + (group0 & 7));
       } else {
-#pragma unroll
-        for (int gi = 0; gi < HALF; ++gi) {
-          sraw[r][gi] = s_bytes == 4 ? *reinterpret_cast<const uint32_t*>(sp + gi * 4) : *reinterpret_cast<const uint16_t*>(sp + gi * 2);
-          if (s * GROUPS + wk * HALF + gi >= a.groups) sraw[r][gi] = 0;
-        }
-      }
-      zraw[r] = 0;
-      if (a.z) {
-#pragma unroll
-        for (int gi = 0; gi < HALF; ++gi)
-          if (!(a.z_vec && HALF == 4)) zraw[r] |= (uint32_t)zp[gi] << (8 * gi);
-        if (a.z_vec && HALF == 4) zraw[r] = *reinterpret_cast<const uint32_t*>(zp);
+        sraw[r][0] = *reinterpret_cast<const float*>(from + (group0 & 7) * 4);
+        zraw[r] = from[32 + (group0 & 7)];
       }
     }
 #pragma unroll
@@ -308,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
         } else {
           w[r][0] = *reinterpret_cast<const uint32_t*>(p + r * 8 * kRowBytes);
         }
-        sg[r] = value_of(sraw[r][gi], a.s_type);
+        sg[r] = sraw[r][gi];
         zero[r] = a.z ? zero_of<BF>(zraw[r] >> (8 * gi) & 15u) : eight;
       }
       float acc[2][NT][4];
@@ -411,7 +436,7 @@ int choose_split(const void* kern, int smem, int threads, int tiles, int mt, int
 
 template <int XK, int NT, int G> int run_stream(W4Args a, cudaStream_t s) {
   auto* kern = w4_stream_kernel<XK, NT, G>;
-  constexpr int SMEM = Stage<XK, NT, G>::kStages * Stage<XK, NT, G>::BYTES;
+  constexpr int SMEM = Stage<XK, NT, G>::SMEM;
   static_assert(SMEM <= 112 * 1024, "two CTAs per SM");
   const int tiles = (a.n + kRows - 1) / kRows, stages = (a.k + kStageK - 1) / kStageK, mt = (a.m + NT * 8 - 1) / (NT * 8);
   if (int rc = choose_split(reinterpret_cast<const void*>(kern), SMEM, kThreads, tiles, mt, stages, &a.split)) return rc;
@@ -448,13 +473,11 @@ template <> __device__ __forceinline__ void tmem_load<16>(uint32_t at, uint32_t 
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(at) : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 template <> __device__ __forceinline__ void tmem_load<32>(uint32_t at, uint32_t (&r)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                : "r"(at) : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -475,17 +498,15 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t at) {
 // two such blocks of 128 rows, so that a stage of x (L2 -> SM traffic) serves 256 rows, and a slice of K; clusters split K as above.
 //   warps 0-7  widen chunk i of their 32 rows, then scale the sums of chunk i - 1 (whose MMA ran meanwhile)
 //   warp 8     brings the operands; x comes permuted and widened by a small launch in front, on which only x's copies wait
-//   warp 9     one thread issues the MMAs
+//   warps 9-10 one thread each issues the MMAs of a block
 // Chunk i's widened weights arriving says that chunk i - 2 has been read back, so its buffers need no barrier of their own.
-constexpr int kTcRows = 256, kTcThreads = 320;
+constexpr int kTcRows = 256, kTcThreads = 352;
 template <int NX, int G> struct TcStage {
   static constexpr int GROUPS = kStageK / G;
   static constexpr int X_AT = kTcRows * kRowBytes;                        // after q: x as four [NX rows][64 k]
   static constexpr int XS_AT = X_AT + NX * kStageK * 2;                   // scales of x: [group][row]
-  static constexpr int S_PITCH = GROUPS * 4, S_AT = XS_AT + GROUPS * NX * 4;
-  static constexpr int Z_PITCH = (GROUPS + 3) / 4 * 4 + (GROUPS == 4 ? 4 : 8), Z_AT = S_AT + kTcRows * S_PITCH;
-  static constexpr int BYTES = (Z_AT + kTcRows * Z_PITCH + 1023) / 1024 * 1024;
-  static constexpr int kStages = 3 * BYTES <= 225 * 1024 ? 3 : 2;
+  static constexpr int BYTES = (XS_AT + GROUPS * NX * 4 + 1023) / 1024 * 1024, kStages = 3;
+  static constexpr int S_AT = kStages * BYTES, SMEM = S_AT + kTcRows * kRowScales;  // behind the stages: the rows' scales
 };
 
 // x as the MMA reads it: rows of k_pad 16-bit values, each eight in the order (0, 4, 1, 5, 2, 6, 3, 7), zero outside x
@@ -527,7 +548,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kTcRows, m0 = blockIdx.y * NX;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
-  const int s_bytes = a.s_type == IB200_F32 ? 4 : 2;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (dead || mbarrier_wait_bounded(bar, parity)) return;
     dead = 1;
@@ -536,7 +556,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   auto arrive = [](uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory"); };
   if (threadIdx.x == 0) {
     dead = 0;
-    for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 8 + 1);
+    for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 8 + 2);
     for (int b = 0; b < 2; ++b) {
       for (int i = 0; i < NA; ++i) mbarrier_init(&a_full[b][i], 4);
       for (int i = 0; i < ND; ++i) mbarrier_init(&d_full[b][i], 1);
@@ -567,7 +587,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
         mbarrier_expect_tx(&full[i], kTcRows * kRowBytes + NX * kStageK * 2);
         tensor_copy(dst, &map_q, &full[i], s * kRowBytes, n0);
       }
-      bring_scales<GROUPS, kTcRows, S>(a, dst, n0, s, lane);
       if (a.xs_groups > 1) {
         for (int e = lane; e < GROUPS * NX; e += 32) {
           const int m = m0 + e % NX, grp = s * GROUPS + e / NX;
@@ -584,30 +603,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
     }
     if (dead)  // copies that are still on their way land before the CTA ends
       for (int s = max(s0, s1 - kStages); s < s1; ++s) (void)mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
-  } else if (warp == 9) {
-    // ---- the MMA thread -------------------------------------------------------------------------------------
+  } else if (warp >= 9) {
+    // ---- the MMA threads, one for each block of rows: everything but the waits and the instructions themselves is a constant, because one
+    // thread's arithmetic between two MMAs costs more than the MMA (with descriptors made in the loop one took 120 cycles of its thread)
     if (lane == 0) {
+      const int b = warp - 9;
       // f32 accumulators, both operands K-major, N = NX, M = 128
-      const uint32_t idesc = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((uint32_t)(NX >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t idesc = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((uint32_t)(NX >> 3) << 17) | ((128u >> 4) << 24);
       int i = 0;
       for (int s = s0; s < s1; ++s) {
         const int st = (s - s0) % kStages;
         wait(&full[st], ((s - s0) / kStages) & 1);
-        const uint32_t x_at = smem_addr(smem + st * S::BYTES + S::X_AT);
+        const uint64_t x = swizzled_desc(smem_addr(smem + st * S::BYTES + S::X_AT));
+#pragma unroll
         for (int c = 0; c < GROUPS; ++c, ++i) {
+          const uint32_t d = tmem + b * 128 + (i % ND) * NX, w = tmem + A_AT + b * 128 + (i % NA) * (G / 2);
+          wait(&a_full[b][i % NA], (i / NA) & 1);
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            wait(&a_full[b][i % NA], (i / NA) & 1);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t d = tmem + b * 128 + (i % ND) * NX, w = tmem + A_AT + b * 128 + (i % NA) * (G / 2);
-#pragma unroll
-            for (int k = 0; k < G / 16; ++k) {
-              const int at = c * G + k * 16;  // k of the stage
-              asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-                           ::"r"(d), "r"(w + k * 8), "l"(swizzled_desc(x_at + at / 64 * (NX * 128) + at % 64 * 2)), "r"(idesc), "r"(k ? 1 : 0) : "memory");
-            }
-            commit(&d_full[b][i % ND]);
+          for (int k = 0; k < G / 16; ++k) {
+            const int at = c * G + k * 16;  // k of the stage
+            const uint64_t xk = x + ((at / 64 * (NX * 128) + at % 64 * 2) >> 4);
+            if (k == 0)
+              asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(w), "l"(xk), "r"(idesc) : "memory");
+            else
+              asm volatile("{\n .reg .pred p;\n setp.eq.b32 p, 0, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                           ::"r"(d), "r"(w + k * 8), "l"(xk), "r"(idesc) : "memory");
           }
+          commit(&d_full[b][i % ND]);
         }
         commit(&empty[st]);
       }
@@ -617,8 +640,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
     // ---- widen and scale ------------------------------------------------------------------------------------
     const int b = warp >> 2, row = b * 128 + (warp & 3) * 32 + lane;  // the thread's row of q is its lane of tensor memory
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, d_at = tmem + lanes + b * 128, a_at = tmem + lanes + A_AT + b * 128;
-    const int64_t first = (int64_t)min(n0 + row, a.n - 1) * a.groups;
-    const int s_mis = (int)((reinterpret_cast<uintptr_t>(a.s) + first * s_bytes) & 3);
+    uint8_t* scales = smem + S::S_AT + row * kRowScales;
+    int block = s0 * GROUPS >> 3;
+    leave_block(a, scales, block, read_block(a, n0 + row, block));
+    RowBlock ahead = read_block(a, n0 + row, block + 1);
     uint32_t magic = BF ? 0x43004300u : 0x64006400u;
     asm volatile("" : "+r"(magic));  // (kept in a register)
     const Zero eight = zero_of<BF>(8);
@@ -630,24 +655,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
       wait(&d_full[b][j % ND], (j / ND) & 1);
       __syncwarp();  // (the loads below are the whole warp's)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      uint32_t r[NX / LD][LD];
 #pragma unroll
-      for (int c = 0; c < NX / LD; ++c) {
-        uint32_t r[LD];
-        tmem_load<LD>(d_at + (j % ND) * NX + c * LD, r);
-        if (xs_many) {
-          const float4* f = reinterpret_cast<const float4*>(old_stage + S::XS_AT + (old_group * NX + c * LD) * 4);
+      for (int c = 0; c < NX / LD; ++c) tmem_load<LD>(d_at + (j % ND) * NX + c * LD, r[c]);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int e = 0; e < LD / 4; ++e) {
-            const float4 v = f[e];
-            sum[c * LD + 4 * e] = fmaf(__uint_as_float(r[4 * e]), old_scale * v.x, sum[c * LD + 4 * e]);
-            sum[c * LD + 4 * e + 1] = fmaf(__uint_as_float(r[4 * e + 1]), old_scale * v.y, sum[c * LD + 4 * e + 1]);
-            sum[c * LD + 4 * e + 2] = fmaf(__uint_as_float(r[4 * e + 2]), old_scale * v.z, sum[c * LD + 4 * e + 2]);
-            sum[c * LD + 4 * e + 3] = fmaf(__uint_as_float(r[4 * e + 3]), old_scale * v.w, sum[c * LD + 4 * e + 3]);
-          }
-        } else {
+      for (int c = 0; c < NX / LD; ++c)
 #pragma unroll
-          for (int e = 0; e < LD; ++e) sum[c * LD + e] = fmaf(__uint_as_float(r[e]), old_scale, sum[c * LD + e]);
+        for (int e = 0; e < LD; ++e) asm volatile("" : "+r"(r[c][e]));  // (values are there from here on)
+      if (xs_many) {
+        const float4* f = reinterpret_cast<const float4*>(old_stage + S::XS_AT + old_group * NX * 4);
+#pragma unroll
+        for (int e = 0; e < NX / 4; ++e) {
+          const float4 v = f[e];
+          sum[4 * e] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD]), old_scale * v.x, sum[4 * e]);
+          sum[4 * e + 1] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD + 1]), old_scale * v.y, sum[4 * e + 1]);
+          sum[4 * e + 2] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD + 2]), old_scale * v.z, sum[4 * e + 2]);
+          sum[4 * e + 3] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD + 3]), old_scale * v.w, sum[4 * e + 3]);
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < NX; ++e) sum[e] = fmaf(__uint_as_float(r[e / LD][e % LD]), old_scale, sum[e]);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     };
@@ -655,10 +683,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
       const uint8_t* st = smem + (s - s0) % kStages * S::BYTES;
       wait(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
       __syncwarp();
-      const int z_mis = (int)((reinterpret_cast<uintptr_t>(a.z) + first + s * GROUPS) & 3);
+      if (s * GROUPS >> 3 != block) {  // (a thread leaves blocks for itself)
+        block = s * GROUPS >> 3;
+        leave_block(a, scales, block, ahead);
+        ahead = read_block(a, n0 + row, block + 1);
+      }
+      const uint8_t* from = scales + (block & 1) * kBlockBytes;
 #pragma unroll
       for (int c = 0; c < GROUPS; ++c, ++i) {
-        const Zero zero = a.z ? zero_of<BF>(st[S::Z_AT + row * S::Z_PITCH + z_mis + c] & 15u) : eight;
+        const Zero zero = a.z ? zero_of<BF>(from[32 + (s * GROUPS & 7) + c] & 15u) : eight;
+        const float scale = *reinterpret_cast<const float*>(from + ((s * GROUPS & 7) + c) * 4);
 #pragma unroll
         for (int q = 0; q < G / 32; ++q) {
           const uint4 v = *reinterpret_cast<const uint4*>(st + row * kRowBytes + (((c * (G / 32) + q) ^ (row & 7)) << 4));
@@ -677,9 +711,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) arrive(&a_full[b][i % NA]);
-        const uint8_t* sp = st + S::S_AT + row * S::S_PITCH + s_mis + c * s_bytes;
-        float scale = value_of(s_bytes == 4 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp), a.s_type);
-        if (s * GROUPS + c >= a.groups) scale = 0.0f;  // behind the last group
         if (i > 0) scale_sums(i - 1);
         if (c == 0 && s > s0) {
           __syncwarp();
@@ -722,8 +753,8 @@ int tc_columns(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
 template <int XK, int NX, int G> int run_tc(W4Args a, void* scratch, cudaStream_t s) {
   constexpr bool BF = XK == X_BF16;
   auto* kern = w4_tc_kernel<BF, NX, G>;
-  constexpr int SMEM = TcStage<NX, G>::kStages * TcStage<NX, G>::BYTES;
-  static_assert(SMEM <= 225 * 1024, "one CTA per SM");
+  constexpr int SMEM = TcStage<NX, G>::SMEM;
+  static_assert(SMEM <= 226 * 1024, "one CTA per SM");
   const int64_t rows = padded(a.m, NX), k_pad = padded(a.k, kStageK);
   CUtensorMap map_q, map_x;
   if (int rc = make_byte_map(&map_q, a.q, a.n, a.k / 2, kTcRows)) return rc;
@@ -793,9 +824,8 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
   const bool x_vec = (reinterpret_cast<uintptr_t>(x) & (held ? 7 : 15)) == 0 && (m == 1 || x_stride * e % (held ? 8 : 16) == 0);
   W4Args a{x, static_cast<const uint8_t*>(q), scales, static_cast<const uint8_t*>(zeros), bias, xs, y, x_stride,
            (int)m, (int)n, (int)k, (int)group, (int)groups, (int)xs_groups, x_dtype, s_dtype, out_dtype, x_vec, 0, 0, 1, status};
-  const int per = kStageK / (int)group;  // groups of a stage
-  a.s_vec = s_dtype != IB200_F32 && groups % per == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * per) == 0;
-  a.z_vec = zeros && per >= 4 && groups % per == 0 && reinterpret_cast<uintptr_t>(zeros) % per == 0;
+  a.s_vec = groups % 8 == 0 && aligned16(scales);
+  a.z_vec = zeros && groups % 8 == 0 && (reinterpret_cast<uintptr_t>(zeros) & 7) == 0;
   if (m > kStreamRows && k > 0) {
     if (!scratch || scratch_bytes < w4_scratch_bytes(x_dtype, m, n, k, group)) return fail(IB200_ERR_BUFFER, "w4_matmul: scratch is smaller than ib200_w4_scratch_bytes");
     if (x_dtype == IB200_BF16) return run_tc_rows<X_BF16>(a, scratch, s);
