@@ -469,6 +469,11 @@ template <int XK> int run_stream_rows(const W4Args& a, cudaStream_t s) {
 
 // ---- tensor memory ----------------------------------------------------------------------------------------
 template <int N> __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[N]);
+template <> __device__ __forceinline__ void tmem_load<8>(uint32_t at, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(at) : "memory");
+}
 template <> __device__ __forceinline__ void tmem_load<16>(uint32_t at, uint32_t (&r)[16]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
@@ -479,7 +484,12 @@ template <> __device__ __forceinline__ void tmem_load<32>(uint32_t at, uint32_t 
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                : "r"(at) : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16]) {
+template <int N> __device__ __forceinline__ void tmem_store(uint32_t at, const uint32_t (&r)[N]);
+template <> __device__ __forceinline__ void tmem_store<8>(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+template <> __device__ __forceinline__ void tmem_store<16>(uint32_t at, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
@@ -496,11 +506,12 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t at) {
 // row and stores it to tensor memory, where the MMA reads it), B = x from shared memory (128-byte swizzle, K-major).  The sums of a group are read back
 // and scaled into f32 registers, one row to a thread, so nothing but x and q - z, both exact, enters the products.  A CTA has
 // two such blocks of 128 rows, so that a stage of x (L2 -> SM traffic) serves 256 rows, and a slice of K; clusters split K as above.
-//   warps 0-7  widen chunk i of their 32 rows, then scale the sums of chunk i - 1 (whose MMA ran meanwhile)
-//   warp 8     brings the operands; x comes permuted and widened by a small launch in front, on which only x's copies wait
-//   warps 9-10 one thread each issues the MMAs of a block
+//   warps 0-15  widen chunk i of their 32 rows (two warps to 32 rows, half of k each), then scale the sums of chunk i - 1, whose MMA ran
+//               meanwhile (half of the columns each)
+//   warp 16     brings the operands; x comes permuted and widened by a small launch in front, on which only x's copies wait
+//   warps 17-18 one thread each issues the MMAs of a block
 // Chunk i's widened weights arriving says that chunk i - 2 has been read back, so its buffers need no barrier of their own.
-constexpr int kTcRows = 256, kTcThreads = 352;
+constexpr int kTcRows = 256, kTcThreads = 608;
 template <int NX, int G> struct TcStage {
   static constexpr int GROUPS = kStageK / G;
   static constexpr int X_AT = kTcRows * kRowBytes;                        // after q: x as four [NX rows][64 k]
@@ -540,12 +551,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   using S = TcStage<NX, G>;
   constexpr int GROUPS = S::GROUPS, kStages = S::kStages, NA = 256 / G, ND = 128 / NX;  // groups of a stage; buffers of A (128 columns a block) and D
   constexpr int A_AT = 256;                                                              // tensor memory: D of both blocks, then A of both
-  constexpr int LD = NX < 32 ? NX : 32;
+  constexpr int COLS = NX / 2, KS = G / 2;  // of a thread: columns of D that it scales, k of a chunk that it widens
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[kStages], empty[kStages], a_full[2][NA], d_full[2][ND];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int dead;  // a wait ran out: nothing waits any more
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be the same for a warp)
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kTcRows, m0 = blockIdx.y * NX;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -556,27 +567,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   auto arrive = [](uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory"); };
   if (threadIdx.x == 0) {
     dead = 0;
-    for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 8 + 2);
+    for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 16 + 2);
     for (int b = 0; b < 2; ++b) {
-      for (int i = 0; i < NA; ++i) mbarrier_init(&a_full[b][i], 4);
+      for (int i = 0; i < NA; ++i) mbarrier_init(&a_full[b][i], 8);
       for (int i = 0; i < ND; ++i) mbarrier_init(&d_full[b][i], 1);
     }
     mbarrier_init_fence();
   }
-  if (warp == 9) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
-  float sum[NX];
+  float sum[COLS];
 #pragma unroll
-  for (int j = 0; j < NX; ++j) sum[j] = 0.0f;
+  for (int j = 0; j < COLS; ++j) sum[j] = 0.0f;
 
-  if (warp == 8) {
+  if (warp == 16) {
     // ---- the bringing warp ----------------------------------------------------------------------------------
     const uint32_t smem_at = smem_addr(smem);
     for (int s = s0; s < s1; ++s) {
@@ -603,23 +614,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
     }
     if (dead)  // copies that are still on their way land before the CTA ends
       for (int s = max(s0, s1 - kStages); s < s1; ++s) (void)mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
-  } else if (warp >= 9) {
-    // ---- the MMA threads, one for each block of rows: everything but the waits and the instructions themselves is a constant, because one
-    // thread's arithmetic between two MMAs costs more than the MMA (with descriptors made in the loop one took 120 cycles of its thread)
-    if (lane == 0) {
-      const int b = warp - 9;
-      // f32 accumulators, both operands K-major, N = NX, M = 128
-      constexpr uint32_t idesc = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((uint32_t)(NX >> 3) << 17) | ((128u >> 4) << 24);
-      int i = 0;
-      for (int s = s0; s < s1; ++s) {
-        const int st = (s - s0) % kStages;
-        wait(&full[st], ((s - s0) / kStages) & 1);
-        const uint64_t x = swizzled_desc(smem_addr(smem + st * S::BYTES + S::X_AT));
+  } else if (warp >= 17) {
+    // ---- the MMA warps, one for each block of rows.  All lanes walk the loop, so that its values stay in uniform registers, and one issues: moved there
+    // from one thread's registers they took 100 cycles an MMA, three times its own time.
+    // f32 accumulators, both operands K-major, N = NX, M = 128
+    constexpr uint32_t idesc = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((uint32_t)(NX >> 3) << 17) | ((128u >> 4) << 24);
+    const int b = warp - 17;
+    uint32_t chosen;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(chosen));
+    int i = 0;
+    for (int s = s0; s < s1; ++s) {
+      const int st = (s - s0) % kStages;
+      wait(&full[st], ((s - s0) / kStages) & 1);
+      const uint64_t x = swizzled_desc(smem_addr(smem) + st * S::BYTES + S::X_AT);
 #pragma unroll
-        for (int c = 0; c < GROUPS; ++c, ++i) {
-          const uint32_t d = tmem + b * 128 + (i % ND) * NX, w = tmem + A_AT + b * 128 + (i % NA) * (G / 2);
-          wait(&a_full[b][i % NA], (i / NA) & 1);
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (int c = 0; c < GROUPS; ++c, ++i) {
+        const uint32_t d = tmem + b * 128 + (i % ND) * NX, w = tmem + A_AT + b * 128 + (i % NA) * (G / 2);
+        wait(&a_full[b][i % NA], (i / NA) & 1);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (chosen) {
 #pragma unroll
           for (int k = 0; k < G / 16; ++k) {
             const int at = c * G + k * 16;  // k of the stage
@@ -632,18 +646,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
           }
           commit(&d_full[b][i % ND]);
         }
-        commit(&empty[st]);
       }
+      if (chosen) commit(&empty[st]);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // ---- widen and scale ------------------------------------------------------------------------------------
-    const int b = warp >> 2, row = b * 128 + (warp & 3) * 32 + lane;  // the thread's row of q is its lane of tensor memory
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, d_at = tmem + lanes + b * 128, a_at = tmem + lanes + A_AT + b * 128;
+    const int b = warp >> 2 & 1, half = warp >> 3, row = b * 128 + (warp & 3) * 32 + lane;  // the thread's row of q is its lane of tensor memory
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, d_at = tmem + lanes + b * 128 + half * COLS, a_at = tmem + lanes + A_AT + b * 128 + half * (KS / 2);
     uint8_t* scales = smem + S::S_AT + row * kRowScales;
     int block = s0 * GROUPS >> 3;
-    leave_block(a, scales, block, read_block(a, n0 + row, block));
-    RowBlock ahead = read_block(a, n0 + row, block + 1);
+    RowBlock ahead = {};
+    auto next_block = [&] {  // the first of the two warps reads the rows' scales for both
+      if (half == 0) {
+        leave_block(a, scales, block, ahead);
+        ahead = read_block(a, n0 + row, block + 1);
+      }
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 7)) : "memory");
+    };
+    if (half == 0) ahead = read_block(a, n0 + row, block);
+    next_block();
     uint32_t magic = BF ? 0x43004300u : 0x64006400u;
     asm volatile("" : "+r"(magic));  // (kept in a register)
     const Zero eight = zero_of<BF>(8);
@@ -655,27 +677,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
       wait(&d_full[b][j % ND], (j / ND) & 1);
       __syncwarp();  // (the loads below are the whole warp's)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      uint32_t r[NX / LD][LD];
-#pragma unroll
-      for (int c = 0; c < NX / LD; ++c) tmem_load<LD>(d_at + (j % ND) * NX + c * LD, r[c]);
+      uint32_t r[COLS];
+      tmem_load<COLS>(d_at + (j % ND) * NX, r);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-      for (int c = 0; c < NX / LD; ++c)
-#pragma unroll
-        for (int e = 0; e < LD; ++e) asm volatile("" : "+r"(r[c][e]));  // (values are there from here on)
+      for (int e = 0; e < COLS; ++e) asm volatile("" : "+r"(r[e]));  // (values are there from here on)
       if (xs_many) {
-        const float4* f = reinterpret_cast<const float4*>(old_stage + S::XS_AT + old_group * NX * 4);
+        const float4* f = reinterpret_cast<const float4*>(old_stage + S::XS_AT + (old_group * NX + half * COLS) * 4);
 #pragma unroll
-        for (int e = 0; e < NX / 4; ++e) {
-          const float4 v = f[e];
-          sum[4 * e] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD]), old_scale * v.x, sum[4 * e]);
-          sum[4 * e + 1] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD + 1]), old_scale * v.y, sum[4 * e + 1]);
-          sum[4 * e + 2] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD + 2]), old_scale * v.z, sum[4 * e + 2]);
-          sum[4 * e + 3] = fmaf(__uint_as_float(r[4 * e / LD][4 * e % LD + 3]), old_scale * v.w, sum[4 * e + 3]);
+        for (int e = 0; e < COLS; e += 4) {
+          const float4 v = f[e / 4];
+          sum[e] = fmaf(__uint_as_float(r[e]), old_scale * v.x, sum[e]);
+          sum[e + 1] = fmaf(__uint_as_float(r[e + 1]), old_scale * v.y, sum[e + 1]);
+          sum[e + 2] = fmaf(__uint_as_float(r[e + 2]), old_scale * v.z, sum[e + 2]);
+          sum[e + 3] = fmaf(__uint_as_float(r[e + 3]), old_scale * v.w, sum[e + 3]);
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < NX; ++e) sum[e] = fmaf(__uint_as_float(r[e / LD][e % LD]), old_scale, sum[e]);
+        for (int e = 0; e < COLS; ++e) sum[e] = fmaf(__uint_as_float(r[e]), old_scale, sum[e]);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     };
@@ -683,29 +702,36 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
       const uint8_t* st = smem + (s - s0) % kStages * S::BYTES;
       wait(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
       __syncwarp();
-      if (s * GROUPS >> 3 != block) {  // (a thread leaves blocks for itself)
+      if (s * GROUPS >> 3 != block) {
         block = s * GROUPS >> 3;
-        leave_block(a, scales, block, ahead);
-        ahead = read_block(a, n0 + row, block + 1);
+        next_block();
       }
       const uint8_t* from = scales + (block & 1) * kBlockBytes;
 #pragma unroll
       for (int c = 0; c < GROUPS; ++c, ++i) {
         const Zero zero = a.z ? zero_of<BF>(from[32 + (s * GROUPS & 7) + c] & 15u) : eight;
         const float scale = *reinterpret_cast<const float*>(from + ((s * GROUPS & 7) + c) * 4);
+        constexpr int WORDS = KS >= 32 ? 4 : 2;  // of q a time
 #pragma unroll
-        for (int q = 0; q < G / 32; ++q) {
-          const uint4 v = *reinterpret_cast<const uint4*>(st + row * kRowBytes + (((c * (G / 32) + q) ^ (row & 7)) << 4));
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          uint32_t r[16];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t p[4];
-            weights_of<BF>(w[k], zero, magic, p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r[4 * k + e] = p[e];
+        for (int q = 0; q < KS / (8 * WORDS); ++q) {
+          const int byte = c * (G / 2) + half * (KS / 2) + q * 16;  // of the row
+          const uint8_t* p = st + row * kRowBytes + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
+          uint32_t w[4], r[4 * WORDS];
+          if (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x, w[1] = v.y;
           }
-          tmem_store16(a_at + (i % NA) * (G / 2) + q * 16, r);
+#pragma unroll
+          for (int k = 0; k < WORDS; ++k) {
+            uint32_t pairs[4];
+            weights_of<BF>(w[k], zero, magic, pairs);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[4 * k + e] = pairs[e];
+          }
+          tmem_store<4 * WORDS>(a_at + (i % NA) * (G / 2) + q * 16, r);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -727,14 +753,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   // ---- add up the cluster's slices and write ----------------------------------------------------------------
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
   float* box = reinterpret_cast<float*>(smem);  // [NX][256] sums of this CTA
-  if (warp < 8) {
+  if (warp < 16) {
 #pragma unroll
-    for (int j = 0; j < NX; ++j) box[j * kTcRows + threadIdx.x] = sum[j];
+    for (int j = 0; j < COLS; ++j) box[((warp >> 3) * COLS + j) * kTcRows + threadIdx.x % kTcRows] = sum[j];
   }
   if (split > 1) cluster_arrive_wait(); else __syncthreads();
   const int rows = min(NX, a.m - m0);
