@@ -13,9 +13,8 @@ namespace {
 // ---- append -----------------------------------------------------------------------------------------
 // A unit is the new tokens of one block: for a head, one warp (few tokens) or CTA for the keys and one for the values.
 //   s' = max(s, max|new| / Q), s = 0 for a block that begins here; held values become round(q * s / s') where s' > s, new ones round(x / s')
-// Divisions are IEEE divisions: the held values then depend on nothing but their definition.  The new values are read once
-// into registers (up to KEEP vectors of 8 a thread, blocks of 64 tokens of 128; more are read again) and written 8 bytes at a time.
-constexpr int KEEP = 8;
+// Quotients round as IEEE divisions do: the held values depend on nothing but their definition.  The new values are read once
+// into registers (up to KEEP vectors of 8 a thread: 16 tokens of 128 in a warp, 64 in a CTA; more are read again) and written 8 bytes at a time.
 template <typename T> __device__ __forceinline__ uint4 read_new(const T* p, bool vec) {
   if (vec) return __ldcs(reinterpret_cast<const uint4*>(p));
   const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
@@ -26,18 +25,39 @@ template <typename T> __device__ __forceinline__ void floats_of(const uint4& r, 
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = to_f32(p[i]);
 }
-template <int HELD> __device__ __forceinline__ uint2 hold_quotients(const float (&v)[8], float div) {
-  return make_uint2(hold4<HELD>(v[0] / div, v[1] / div, v[2] / div, v[3] / div), hold4<HELD>(v[4] / div, v[5] / div, v[6] / div, v[7] / div));
+// round(v / div) of eight values to the held type.  v * (1 / div) is within 2 ulp of the f32 quotient, so it rounds alike unless it lies that close to
+// the middle between two held values (or, in e4m3, in the subnormals, whose middles lie elsewhere).  One test over the eight finds that, one vector in some
+// thousand is divided; all are where 1 / div overflows, and those with a NaN.
+template <int HELD> __device__ __forceinline__ uint2 hold_quotients(const float (&v)[8], float div, float inv) {
+  float q[8], least = INFINITY, most = 0.0f;
+  int nearest = INT32_MAX;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    q[i] = v[i] * inv;
+    if (HELD == HELD_E4M3) {  // 3 of 23 mantissa bits stay: the other 20, as a signed distance from their middle
+      nearest = min(nearest, abs((int)(__float_as_uint(q[i]) * 4096u + 0x80000000u)));
+      least = fminf(least, fabsf(q[i]));
+    } else {  // |q| < 2^7, so 2 ulp are below 2^-15
+      const float whole = (q[i] + 0x1.8p23f) - 0x1.8p23f;
+      most = fmaxf(most, fabsf(q[i] - whole));
+    }
+  }
+  const bool sure = HELD == HELD_E4M3 ? nearest > 16 * 4096 && least >= 0x1.01p-6f && inv <= 0x1p127f : most < 0.49993f && inv <= 0x1p127f;
+  if (!sure) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = v[i] / div;
+  }
+  return make_uint2(hold4<HELD>(q[0], q[1], q[2], q[3]), hold4<HELD>(q[4], q[5], q[6], q[7]));
 }
 
 template <typename T, int HELD, int D, int THREADS>
 __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, const int vec) {
-  constexpr int PER = D / 8;  // vectors of a token
+  constexpr int PER = D / 8, KEEP = THREADS == 32 ? 8 : 4;  // vectors of a token, of a thread
   __shared__ float slots[32];
   const int head = blockIdx.y, tid = threadIdx.x, block = (int)a.block;
   // Unit u: with offsets, sequence b has the units from cu[b] / block + 2 b, which leaves room for (its new tokens) / block + 2; without,
   // the same number for each.
-  const int64_t u = blockIdx.x;
+  const int u = (int)blockIdx.x;
   int b, first, count, j;
   if (a.cu) {
     int lo = 0, hi = (int)a.batch;
@@ -51,26 +71,20 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, cons
     j = (int)(u - (first / block + 2 * (int64_t)b));
     if (first < 0 || count <= 0 || j < 0 || (int64_t)first + count > a.tokens) return;
   } else {
-    b = (int)(u / a.per);
-    j = (int)(u - (int64_t)b * a.per);
+    b = u / a.per;
+    j = u - b * a.per;
     first = b * a.each;
     count = a.each;
   }
-  const int64_t start = (int64_t)a.lens[b] - count, end = start + count;  // places of the new tokens
-  const int64_t blk = max((int64_t)0, start) / block + j;
-  const int64_t from = max(max((int64_t)0, start), blk * block), to = min(end, (blk + 1) * block);
+  const int end = a.lens[b], start = max(end, -1) - count;  // places of the new tokens: start .. end - 1; those below 0 have none
+  const int64_t blk = max(0, start) / block + j;
+  const int from = (int)max((int64_t)max(0, start), min(blk * block, (int64_t)INT32_MAX)), to = (int)min((int64_t)end, (blk + 1) * block);
   if (from >= to || blk >= a.table_blocks) return;
-  const int page = a.table[(int64_t)b * a.table_blocks + blk];
-  if ((unsigned)page >= (unsigned)a.pages) return;
+  const int page = a.table[(int64_t)b * a.table_blocks + blk];  // (looked at when the new values are on their way)
   const bool is_v = blockIdx.z;
-  const int slot = (int)(from - blk * block), fresh = (int)(to - from), vectors = fresh * PER;
+  const int slot = (int)(from - blk * block), vectors = (to - from) * PER;
   const int64_t x_token = is_v ? a.v_token : a.k_token;
-  const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (first + (from - start)) * x_token + (int64_t)head * (is_v ? a.v_head : a.k_head);
-  const int64_t at = (int64_t)page * a.heads + head;
-  uint8_t* cache = (is_v ? a.v_cache : a.k_cache) + at * block * D;
-  float* scale = (is_v ? a.v_scale : a.k_scale) + at;
-  const float before = slot ? *scale : 0.0f;
-
+  const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (int64_t)(first + (from - start)) * x_token + (int64_t)head * (is_v ? a.v_head : a.k_head);
   auto source = [&](int i) { return x + (i / PER) * x_token + i % PER * 8; };
   uint4 keep[KEEP];
   float top = 0.0f;
@@ -83,12 +97,18 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, cons
 #pragma unroll
   for (int k = 0; k < KEEP; ++k)
     if (tid + k * THREADS < vectors) keep[k] = read_new(source(tid + k * THREADS), vec);
+  if ((unsigned)page >= (unsigned)a.pages) return;
+  const int64_t at = (int64_t)page * a.heads + head;
+  uint8_t* cache = (is_v ? a.v_cache : a.k_cache) + at * block * D;
+  float* scale = (is_v ? a.v_scale : a.k_scale) + at;
+  const float before = slot ? *scale : 0.0f;
+
 #pragma unroll
   for (int k = 0; k < KEEP; ++k)
     if (tid + k * THREADS < vectors) enter(keep[k]);
   for (int i = tid + KEEP * THREADS; i < vectors; i += THREADS) enter(read_new(source(i), vec));
   top = THREADS == 32 ? warp_reduce<MaxOp>(top) : block_reduce<MaxOp>(top, slots);  // (the barrier: every thread has read the old scale)
-  const float after = max_nan(before, top / held_top<HELD>()), div = after == 0.0f ? 1.0f : after;
+  const float after = max_nan(before, top / held_top<HELD>()), div = after == 0.0f ? 1.0f : after, inv = 1.0f / div;
   if (THREADS == 32) __syncwarp();
   if (tid == 0) *scale = after;
   if (!(after == before)) {
@@ -97,14 +117,14 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, cons
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = held_value<HELD>((uint8_t)((e < 4 ? old.x : old.y) >> (8 * (e & 3)))) * before;
-      *reinterpret_cast<uint2*>(cache + i * 8) = hold_quotients<HELD>(v, div);
+      *reinterpret_cast<uint2*>(cache + i * 8) = hold_quotients<HELD>(v, div, inv);
     }
   }
   uint8_t* out = cache + slot * D;
   auto leave = [&](int i, const uint4& r) {
     float v[8];
     floats_of<T>(r, v);
-    *reinterpret_cast<uint2*>(out + i * 8) = hold_quotients<HELD>(v, div);
+    *reinterpret_cast<uint2*>(out + i * 8) = hold_quotients<HELD>(v, div, inv);
   };
 #pragma unroll
   for (int k = 0; k < KEEP; ++k)
@@ -119,8 +139,8 @@ template <typename T, int HELD, int D> int run_append(const Kv8Append& a, cudaSt
   const dim3 grid((unsigned)units, (unsigned)a.heads, 2);
   // a warp holds 16 tokens of 128 in its registers; where a block takes more, a CTA
   const int64_t expect = (a.tokens + a.batch - 1) / a.batch;
-  if ((expect < a.block ? expect : a.block) * D <= 32 * KEEP * 8) append_kernel<T, HELD, D, 32><<<grid, 32, 0, s>>>(a, vec);
-  else append_kernel<T, HELD, D, 128><<<grid, 128, 0, s>>>(a, vec);
+  if ((expect < a.block ? expect : a.block) * D <= 16 * 128) append_kernel<T, HELD, D, 32><<<grid, 32, 0, s>>>(a, vec);
+  else append_kernel<T, HELD, D, 256><<<grid, 256, 0, s>>>(a, vec);
   return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "kv8_append launch");
 }
 template <typename T, int HELD> int run_append_dim(const Kv8Append& a, cudaStream_t s) {

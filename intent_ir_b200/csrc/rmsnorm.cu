@@ -56,6 +56,15 @@ template <typename T> __device__ __forceinline__ float load_w(const RmsArgs& a, 
 __device__ __forceinline__ float top_of(int type) { return type == IB200_E4M3 ? held_top<HELD_E4M3>() : held_top<HELD_I8>(); }
 __device__ __forceinline__ float inverse_of(int type, float top) { return type == IB200_E4M3 ? held_inverse<HELD_E4M3>(top) : held_inverse<HELD_I8>(top); }
 
+// The same to 2 ulp without divisions, for the scales of groups, of which there are many
+__device__ __forceinline__ float top_inverse(int type) { return type == IB200_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f; }
+__device__ __forceinline__ float inverse_fast(int type, float top) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
+  r *= type == IB200_E4M3 ? 448.0f : 127.0f;
+  return top == 0.0f || isinf(r) ? 0.0f : r;
+}
+
 // ---- rows that fit the registers of a warp or a CTA -------------------------------------------------------
 // One read of x and the residual, one write of everything: HBM-bound.  With VEC a thread has vectors of 8 adjacent columns, 8 * 32
 // or 8 * THREADS apart (16-byte accesses).  Rows that do not begin on 16-byte boundaries are read element by
@@ -181,7 +190,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
     for (int i = 0; i < VE; ++i) {
       e[k][i] *= rstd;
       if (a.w && col(k, VEC ? 0 : i) < cols) e[k][i] *= w[i];
-      if (HELD) top = max_nan(top, fabsf(e[k][i]));
+      if (HELD && a.group == 0) top = max_nan(top, fabsf(e[k][i]));
     }
   }
   if constexpr (!HELD) {
@@ -204,18 +213,27 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
       if (tid == 0) a.scale[row] = top / top_of(a.out_type);
       inv = inverse_of(a.out_type, top);
     }
-    const int lanes = a.group / VE, steps = a.group / 32;  // of a scale: lanes with VEC, elements of a lane without
+    const int lanes = a.group / VE, steps = a.group / 32, shift = __ffs(a.group) - 1;  // of a scale: lanes with VEC, elements of a lane without
+    float tops[NV];
+    if (VEC && a.group) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        tops[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) tops[k] = max_nan(tops[k], fabsf(e[k][i]));
+      }
+      for (int o = lanes >> 1; o; o >>= 1) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) tops[k] = max_nan(tops[k], __shfl_xor_sync(0xffffffffu, tops[k], o));
+      }
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if (VEC) {
         if (a.group) {
-          float m = 0.0f;
-#pragma unroll
-          for (int i = 0; i < VE; ++i) m = max_nan(m, fabsf(e[k][i]));
-          for (int o = lanes >> 1; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
           const int c = col(k, 0);
-          if (c < cols && (tid & (lanes - 1)) == 0) a.scale[row * a.groups + c / a.group] = m / top_of(a.out_type);
-          inv = inverse_of(a.out_type, m);
+          if (c < cols && (tid & (lanes - 1)) == 0) a.scale[row * a.groups + (c >> shift)] = tops[k] * top_inverse(a.out_type);
+          inv = inverse_fast(a.out_type, tops[k]);
         }
         if (col(k, 0) < cols) {
           if (a.out_type == IB200_E4M3) hold8<HELD_E4M3>(y + col(k, 0), e[k], inv, true, VE);
@@ -240,8 +258,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
         for (int i = 0; i < VE; ++i) {
           const int c = col(k, i);
           if (a.group) {
-            inv = inverse_of(a.out_type, m[i]);
-            if (c < cols && lane == 0 && i % steps == 0) a.scale[row * a.groups + c / a.group] = m[i] / top_of(a.out_type);
+            inv = inverse_fast(a.out_type, m[i]);
+            if (c < cols && lane == 0 && i % steps == 0) a.scale[row * a.groups + (c >> shift)] = m[i] * top_inverse(a.out_type);
           }
           if (c < cols) y[c] = (uint8_t)(a.out_type == IB200_E4M3 ? hold1<HELD_E4M3>(e[k][i] * inv) : hold1<HELD_I8>(e[k][i] * inv));
         }

@@ -300,6 +300,15 @@ def _address(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _dense_empty(shape: Tuple[int, ...], dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+    # of the ways to allocate without another tensor as a pattern this is the fastest (1.5 us; new_empty 2.1 - 2.5, empty 2.5)
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=dev)
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=dev)
+    return torch.empty(shape, dtype=dtype, device=dev)
+
+
 def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
             out_dtype: Optional[torch.dtype] = None, group: int = 0, residual_out: Optional[torch.Tensor] = None):
     """``h = x + residual`` and ``y = h / sqrt(mean(h * h) + eps) * w`` over the last axis, in f32 from the unrounded sum; returns
@@ -326,7 +335,7 @@ def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optiona
             raise B200RuntimeError(f"residual must be on cuda:{index} with the shape and dtype of x")
         res_stride = _row_stride("residual", residual)
         if h is None:
-            h = torch.empty_like(x) if stride == cols else x.new_empty(shape)
+            h = torch.empty_like(x) if stride == cols else _dense_empty(shape, dtype, x.device)
             h_stride = cols
         else:
             if not isinstance(h, torch.Tensor) or h.get_device() != index or h.shape != shape or h.dtype != dtype:
@@ -337,13 +346,13 @@ def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optiona
     scale = None
     out_code = code
     if out_dtype is None or out_dtype == dtype:
-        y = torch.empty_like(x) if stride == cols else x.new_empty(shape)
+        y = torch.empty_like(x) if stride == cols else _dense_empty(shape, dtype, x.device)
     else:
         out_code = _HELD_CODE.get(out_dtype)
         if out_code is None:
             raise B200LoweringError(f"rmsnorm: the result is {dtype}, float8_e4m3fn or int8, not {out_dtype}")
-        y = x.new_empty(shape, dtype=out_dtype)
-        scale = x.new_empty(shape[:-1] + ((cols + group - 1) // group if group > 0 else 1,), dtype=torch.float32)
+        y = torch.empty_like(x, dtype=out_dtype) if stride == cols else _dense_empty(shape, out_dtype, x.device)
+        scale = _dense_empty(shape[:-1] + ((cols + group - 1) // group if group > 0 else 1,), torch.float32, x.device)
     args = _lib.RMSNORM_ARGS.pack(x.data_ptr(), _address(residual), _address(w), y.data_ptr(), _address(h), _address(scale), stride, res_stride, h_stride,
                                   code, w_code, out_code, shape[:-1].numel(), cols, group, eps)
     rc = _lib.load().ib200_rmsnorm(args, _stream())
@@ -393,12 +402,12 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
         out_dtype = torch.bfloat16 if x_groups else x.dtype
     elif out_dtype not in _FLOAT_CODE:
         raise B200LoweringError(f"w4_matmul: the result is float32, bfloat16 or float16, not {out_dtype}")
-    y = x.new_empty(front + (n,), dtype=out_dtype)
+    y = _dense_empty(front + (n,), out_dtype, x.device)
     if bias is not None:
         _dense("bias", bias, (n,), out_dtype)
     m = front.numel()
     need = _w4_scratch(x_code, m, n, k, group)
-    scratch = x.new_empty(need, dtype=torch.uint8) if need else None
+    scratch = _dense_empty((need,), torch.uint8, x.device) if need else None
     args = _lib.W4_ARGS.pack(x.data_ptr(), _address(x_scale), q.data_ptr(), scales.data_ptr(), _address(zeros), _address(bias), y.data_ptr(), _address(scratch),
                              _status_address(index), stride, x_groups, x_code, _code("scales", scales, _FLOAT_CODE), _FLOAT_CODE[out_dtype], m, n, k, group, need)
     rc = _lib.load().ib200_w4_matmul(args, _stream())
@@ -509,13 +518,13 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     held, pages, heads, block, dim, batch, table_blocks = _cache_extents(index, "q", q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
     tokens, q_heads, _ = shape = q.shape
     if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+        out = torch.empty_like(q) if q.is_contiguous() else _dense_empty(shape, q.dtype, q.device)
     else:
         _on_device(index, out=out)
         _dense("out", out, shape, q.dtype)
-    lse = q.new_empty((tokens, q_heads), dtype=torch.float32) if return_lse else None
+    lse = _dense_empty((tokens, q_heads), torch.float32, q.device) if return_lse else None
     need = _attention_scratch(tokens, batch, q_heads, heads, dim, block, table_blocks)
-    scratch = q.new_empty(need, dtype=torch.uint8) if need else None
+    scratch = _dense_empty((need,), torch.uint8, q.device) if need else None
     q_token, q_head, _ = q.stride()
     args = _lib.ATTENTION_KV8_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
                                         seq_lens.data_ptr(), _address(cu_new), out.data_ptr(), _address(lse), _address(scratch), q_token, q_head,
