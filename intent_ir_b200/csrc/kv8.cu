@@ -5,6 +5,8 @@
 //   cu     [sequences + 1]: where each sequence's new tokens lie in k, v, q and o (null: the same number for every sequence)
 // What a table says is not trusted: a page outside the cache, and a token outside the table, is never read or written.  The
 // append leaves such tokens out, attention that would have to read them answers NaN.
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace ib200 {
@@ -29,7 +31,7 @@ template <typename T> __device__ __forceinline__ void floats_of(const uint4& r, 
 // the middle between two held values (or, in e4m3, in the subnormals, whose middles lie elsewhere).  One test over the eight finds that, one vector in some
 // thousand is divided; all are where 1 / div overflows, and those with a NaN.
 template <int HELD> __device__ __forceinline__ uint2 hold_quotients(const float (&v)[8], float div, float inv) {
-  float q[8], least = INFINITY, most = 0.0f;
+  float q[8], whole[8], least = INFINITY, most = 0.0f;
   int nearest = INT32_MAX;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -37,12 +39,18 @@ template <int HELD> __device__ __forceinline__ uint2 hold_quotients(const float 
     if (HELD == HELD_E4M3) {  // 3 of 23 mantissa bits stay: the other 20, as a signed distance from their middle
       nearest = min(nearest, abs((int)(__float_as_uint(q[i]) * 4096u + 0x80000000u)));
       least = fminf(least, fabsf(q[i]));
-    } else {  // |q| < 2^7, so 2 ulp are below 2^-15
-      const float whole = (q[i] + 0x1.8p23f) - 0x1.8p23f;
-      most = fmaxf(most, fabsf(q[i] - whole));
+    } else {  // |q| < 2^7, so 2 ulp are below 2^-15; the sum's low byte is round(q)
+      whole[i] = q[i] + 0x1.8p23f;
+      most = fmaxf(most, fabsf(q[i] - (whole[i] - 0x1.8p23f)));
     }
   }
-  const bool sure = HELD == HELD_E4M3 ? nearest > 16 * 4096 && least >= 0x1.01p-6f && inv <= 0x1p127f : most < 0.49993f && inv <= 0x1p127f;
+  const bool sure = (HELD == HELD_E4M3 ? nearest > 16 * 4096 && least >= 0x1.01p-6f : most < 0.49993f) && inv > 0.0f && inv <= 0x1p127f;
+  if (HELD == HELD_I8 && sure) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __byte_perm(__float_as_uint(whole[2 * i]), __float_as_uint(whole[2 * i + 1]), 0x0040);
+    return make_uint2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410));
+  }
   if (!sure) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = v[i] / div;
@@ -52,6 +60,7 @@ template <int HELD> __device__ __forceinline__ uint2 hold_quotients(const float 
 
 template <typename T, int HELD, int D, int THREADS>
 __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, const int vec) {
+  using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
   constexpr int PER = D / 8, KEEP = THREADS == 32 ? 8 : 4;  // vectors of a token, of a thread
   __shared__ float slots[32];
   const int head = blockIdx.y, tid = threadIdx.x, block = (int)a.block;
@@ -87,12 +96,14 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, cons
   const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (int64_t)(first + (from - start)) * x_token + (int64_t)head * (is_v ? a.v_head : a.k_head);
   auto source = [&](int i) { return x + (i / PER) * x_token + i % PER * 8; };
   uint4 keep[KEEP];
-  float top = 0.0f;
+  Pair largest = {};  // two values at a time, in their own type
   auto enter = [&](const uint4& r) {
-    float v[8];
-    floats_of<T>(r, v);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(v[e]));
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t size = w[e] & 0x7fff7fffu;
+      largest = __hmax2_nan(largest, *reinterpret_cast<const Pair*>(&size));
+    }
   };
 #pragma unroll
   for (int k = 0; k < KEEP; ++k)
@@ -107,6 +118,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, cons
   for (int k = 0; k < KEEP; ++k)
     if (tid + k * THREADS < vectors) enter(keep[k]);
   for (int i = tid + KEEP * THREADS; i < vectors; i += THREADS) enter(read_new(source(i), vec));
+  float top = max_nan(to_f32(largest.x), to_f32(largest.y));
   top = THREADS == 32 ? warp_reduce<MaxOp>(top) : block_reduce<MaxOp>(top, slots);  // (the barrier: every thread has read the old scale)
   const float after = max_nan(before, top / held_top<HELD>()), div = after == 0.0f ? 1.0f : after, inv = 1.0f / div;
   if (THREADS == 32) __syncwarp();
