@@ -70,20 +70,22 @@ struct Seq {  // what a sequence asks for
   int first, n, len, keys, tile0, tiles, units_per_head;  // keys: those that the table has room for
   int64_t unit_work, work;  // a unit's, all units' (0 where there are no tiles)
 };
-__device__ __forceinline__ int first_key(const Kv8Attention& a, int64_t pos) {  // that the token at `pos` sees
-  return a.window > 0 ? (int)max((int64_t)0, pos - a.window + 1) : 0;
+__device__ __forceinline__ int first_key(const Kv8Attention& a, int pos) {  // that the token at `pos` sees
+  return a.window > 0 && pos >= a.window ? pos - (int)a.window + 1 : 0;
 }
-__device__ __forceinline__ Seq seq_of(const Kv8Attention& a, int b, int rows) {
+struct Divisors {
+  FastDiv group, block;
+};
+__device__ __forceinline__ Seq seq_of(const Kv8Attention& a, int group, int b, int rows) {
   Seq s;
   s.first = a.cu ? a.cu[b] : b * a.each;
   s.n = a.cu ? a.cu[b + 1] - s.first : a.each;
   s.len = a.lens[b];
-  const int64_t group = a.q_heads / a.heads;
   if (s.n <= 0 || s.len <= 0 || s.first < 0 || (int64_t)s.first + s.n > a.tokens) s.n = 0, s.len = 0;  // nothing to do, or offsets that cannot be
   s.keys = (int)min((int64_t)s.len, a.table_blocks * a.block);
-  s.tile0 = first_key(a, (int64_t)s.len - s.n) / kTile;
+  s.tile0 = first_key(a, s.len - s.n) / kTile;
   s.tiles = s.keys > 0 ? max(0, (s.keys - 1) / kTile + 1 - s.tile0) : 0;
-  s.units_per_head = (int)((s.n * group + rows - 1) / rows);
+  s.units_per_head = (int)(((int64_t)s.n * group + rows - 1) / rows);
   s.unit_work = s.tiles ? s.tiles + kStart : 0;
   s.work = a.heads * s.units_per_head * s.unit_work;
   return s;
@@ -109,7 +111,7 @@ template <typename V> __device__ __forceinline__ V scan_warp(V v, int lane) {  /
 }
 
 template <typename T, int HELD, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kCtas - 1) attention_kernel(const Kv8Attention a, const Scratch sc, const int q_vec) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kCtas - 1) attention_kernel(const Kv8Attention a, const Scratch sc, const Divisors by, const int q_vec) {
   using C = Cfg<D>;
   constexpr int ROWS = 8 * NT, HALVES = D / 64, MT = D / 16, CH = D / 16;  // CH: 16-byte chunks of a token
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
   __shared__ int found;
   __shared__ float stat[kWarps][ROWS][2], top_v[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int batch = (int)a.batch, group = (int)(a.q_heads / a.heads);
+  const int batch = (int)a.batch, group = (int)by.group.d;
 
   // ---- this CTA's range of tiles -------------------------------------------------------------------
   if (threadIdx.x == 0) found = -1;
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
   };
   if (batch > kThreads) {
     int64_t mine = 0;
-    for (int b = threadIdx.x; b < batch; b += kThreads) mine += seq_of(a, b, ROWS).work;
+    for (int b = threadIdx.x; b < batch; b += kThreads) mine += seq_of(a, group, b, ROWS).work;
 #pragma unroll
     for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) sums[warp] = mine;
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
   for (int base = 0; base < batch; base += kThreads) {
     __syncthreads();
     const int b = base + threadIdx.x;
-    const int64_t v = b < batch ? seq_of(a, b, ROWS).work : 0;
+    const int64_t v = b < batch ? seq_of(a, group, b, ROWS).work : 0;
     const int64_t upto = scan_warp(v, lane);
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
   const uint32_t stages_at = (uint32_t)__cvta_generic_to_shared(stages);
   int b = found;
   int64_t front = found_before;
-  Seq s = seq_of(a, b, ROWS);
+  Seq s = seq_of(a, group, b, ROWS);
   const int64_t w_start = w;
 
   while (w < w_end) {
@@ -180,10 +182,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
     const int unit = (int)unit64, from = (int)max((int64_t)0, in - kStart), to = (int)min((int64_t)s.tiles, in + (w_end - w) - kStart);
     w = min(w_end, front + (unit64 + 1) * s.unit_work);
     if (to > from) {
-    const int head = unit / s.units_per_head, r0 = (unit - head * s.units_per_head) * ROWS;
+    const int head = s.units_per_head == 1 ? unit : unit / s.units_per_head, r0 = (unit - head * s.units_per_head) * ROWS;
     const int rows = (int)min((int64_t)ROWS, (int64_t)s.n * group - r0);
     const int start = s.len - s.n;  // place of the first new token (negative: fewer tokens than new ones)
-    const int pos_min = start + r0 / group, pos_max = start + (r0 + rows - 1) / group;
+    const int pos_min = start + (int)by.group.div(r0), pos_max = start + (int)by.group.div(r0 + rows - 1);
     const int lo_min = first_key(a, pos_min), lo_max = first_key(a, pos_max);
     // this warp's steps: 32 keys from 128 * tile + 32 * warp, those with a key that any row sees
     const int off = warp * kStep;
@@ -197,10 +199,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
     auto look_up = [&](int step0) {
       Meta x{-1, 0, NAN, NAN};
       const int step = step0 + (lane >> 1);
-      const unsigned key = (unsigned)(j0 + step) * kTile + off + (lane & 1) * 16, block = (unsigned)a.block;  // (32-bit division)
+      const unsigned key = (unsigned)(j0 + step) * kTile + off + (lane & 1) * 16;
       if (step < steps && key < (unsigned)s.keys) {
-        const unsigned blk = key / block;
-        x.slot = (int)(key - blk * block);
+        unsigned blk, slot;
+        by.block.divmod(key, blk, slot);
+        x.slot = (int)slot;
         const int page = a.table[(int64_t)b * a.table_blocks + blk];
         if ((unsigned)page < (unsigned)a.pages) x.page = page * (int)a.heads + head;
       }
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
     for (int nt = 0; nt < NT; ++nt) {
       const int row = r0 + nt * 8 + g;
       const bool real = nt * 8 + g < rows;
-      const int i = real ? row / group : 0, jq = real ? row - i * group : 0;
+      const int i = real ? (int)by.group.div(row) : 0, jq = real ? row - i * group : 0;
       const T* q = static_cast<const T*>(a.q) + (int64_t)(s.first + i) * a.q_token + (int64_t)(head * group + jq) * a.q_head;
       float v[HALVES * 4][4], top = 0.0f;
 #pragma unroll
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
       for (int c = 0; c < 2; ++c) {
         mult[nt][c] = __shfl_sync(0xffffffffu, m, (2 * t + c) * 4);
         const int rr = nt * 8 + 2 * t + c;
-        hi[nt][c] = rr < rows ? start + (r0 + rr) / group : -1;
+        hi[nt][c] = rr < rows ? start + (int)by.group.div(r0 + rr) : -1;
         low[nt][c] = first_key(a, hi[nt][c]);
       }
     }
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
         v[0] += x.x * fv, v[1] += x.y * fv, v[2] += x.z * fv, v[3] += x.w * fv;
       }
       if (whole) {
-        const int i = (r0 + row) / group;
+        const int i = (int)by.group.div(r0 + row);
         const int64_t out = (int64_t)(s.first + i) * a.q_heads + head * group + (r0 + row - i * group);
         const bool empty = start + i < 0;
         if (start + i >= s.keys) sum = NAN;  // its own key is outside the table
@@ -540,32 +543,33 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
     }
     if (w < w_end && w == front + s.work) {
       front = w;
-      do s = seq_of(a, ++b, ROWS); while (s.work == 0);  // w < total: there is one
+      do s = seq_of(a, group, ++b, ROWS); while (s.work == 0);  // w < total: there is one
     }
   }
 }
 
-// One CTA per row: a row whose unit was cut is joined from its pieces, four at a time, one without keys is zero.
+// A row whose unit was cut is joined from its pieces, one without keys is zero.  WARPS warps to a row take every WARPS-th piece.
 constexpr int kJoin = 128;
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const Scratch sc, const int grid) {
-  constexpr int ROWS = 8 * NT, PER = D / 32, WARPS = kJoin / 32;
-  __shared__ float slots[2][32], weight[kJoin], box[WARPS][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x;
-  const int64_t u = blockIdx.x;
-  const int t = (int)(u / a.q_heads), qh = (int)(u - (int64_t)t * a.q_heads), group = (int)(a.q_heads / a.heads);
+template <typename T, int D, int NT, int WARPS>
+__global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const Scratch sc, const Divisors by, const int grid) {
+  constexpr int ROWS = 8 * NT, PER = D / 32;
+  __shared__ float box[kJoin / 32][D];
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS;
+  const int64_t u = (int64_t)blockIdx.x * (kJoin / 32 / WARPS) + (threadIdx.x >> 5) / WARPS;
+  if (u >= a.tokens * a.q_heads) return;  // (warps of one row leave together, here and below)
+  const int t = (int)(u / a.q_heads), qh = (int)(u - (int64_t)t * a.q_heads), group = (int)by.group.d;
   int b, first, count;
   if (!find_sequence(a.cu, (int)a.batch, a.each, t, b, first, count)) return;
-  const Seq s = seq_of(a, b, ROWS);
+  const Seq s = seq_of(a, group, b, ROWS);
   const int64_t pos = (int64_t)a.lens[b] - count + (t - first);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   T* o = static_cast<T*>(a.o) + u * D;
   if (pos < 0 || pos >= s.keys || s.tiles == 0) {  // no keys; or its own key is outside the table (or offsets that cannot be)
-    for (int d = tid; d < D; d += kJoin) o[d] = from_f32<T>(pos < 0 ? 0.0f : NAN);
-    if (a.lse && tid == 0) a.lse[u] = pos < 0 ? -INFINITY : NAN;
+    for (int d = warp * 32 + lane; d < D; d += WARPS * 32) o[d] = from_f32<T>(pos < 0 ? 0.0f : NAN);
+    if (a.lse && warp == 0 && lane == 0) a.lse[u] = pos < 0 ? -INFINITY : NAN;
     return;
   }
-  const int head = qh / group, r = (t - first) * group + (qh - head * group), row = r % ROWS;
+  const int head = (int)by.group.div(qh), r = (t - first) * group + (qh - head * group), row = r % ROWS;
   // the CTAs whose ranges hold the unit's first and last tile
   const int64_t total = sc.before[a.batch], unit = sc.before[b] + ((int64_t)head * s.units_per_head + r / ROWS) * s.unit_work;
   const int64_t ctas = min((int64_t)grid, total), lo = unit + kStart, hi = unit + s.unit_work - 1;
@@ -577,20 +581,19 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const
   float m = -INFINITY, sum = 0.0f, v[PER];
 #pragma unroll
   for (int e = 0; e < PER; ++e) v[e] = 0.0f;
-  for (int base = c0; base <= c1; base += kJoin) {  // kJoin pieces at a time
-    const int c = base + tid, n = min(kJoin, c1 - base + 1);
+  for (int base = c0; base <= c1; base += 32) {  // every warp has the weights of 32 pieces, a lane each
+    const int c = base + lane, n = min(32, c1 - base + 1);
     const float pm = c <= c1 ? piece(c)[ROWS * D + row] : -INFINITY, pl = c <= c1 ? piece(c)[ROWS * D + ROWS + row] : 0.0f;
-    const float now = fmaxf(m, block_reduce<MaxOp>(pm, slots[0])), from = now == -INFINITY ? 0.0f : now;
+    const float now = fmaxf(m, warp_reduce<MaxOp>(pm)), from = now == -INFINITY ? 0.0f : now;
     const float keep = exp2_fast(m - from), f = exp2_fast(pm - from);
-    weight[tid] = f;
-    sum = sum * keep + block_reduce<SumOp>(c <= c1 ? pl * f : 0.0f, slots[1]);
+    sum = sum * keep + warp_reduce<SumOp>(c <= c1 ? pl * f : 0.0f);
 #pragma unroll
     for (int e = 0; e < PER; ++e) v[e] *= keep;
     m = now;
-#pragma unroll 8
+#pragma unroll 4
     for (int i = warp; i < n; i += WARPS) {
       const float* p = piece(base + i) + row * D + lane * PER;
-      const float g = weight[i];
+      const float g = __shfl_sync(0xffffffffu, f, i);
       if (PER == 4) {
         const float4 x = *reinterpret_cast<const float4*>(p);
         v[0] += x.x * g, v[1] += x.y * g, v[PER - 2] += x.z * g, v[PER - 1] += x.w * g;
@@ -599,18 +602,20 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const
         v[0] += x.x * g, v[1] += x.y * g;
       }
     }
+  }
+  if (WARPS > 1) {  // (one row to the CTA)
+#pragma unroll
+    for (int e = 0; e < PER; ++e) box[warp][lane * PER + e] = v[e];
     __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) v[e] += box[i][lane * PER + e];
   }
 #pragma unroll
-  for (int e = 0; e < PER; ++e) box[warp][lane * PER + e] = v[e];
-  __syncthreads();
-  for (int d = tid; d < D; d += kJoin) {
-    float x = 0.0f;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) x += box[i][d];
-    o[d] = from_f32<T>(x / sum);
-  }
-  if (a.lse && tid == 0) a.lse[u] = (m + log2f(sum)) * 0.6931471805599453f;
+  for (int e = 0; e < PER; ++e) o[lane * PER + e] = from_f32<T>(v[e] / sum);
+  if (a.lse && lane == 0) a.lse[u] = (m + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Rows of a unit, in eights: one where 8 rows suffice, two where a sequence has more (several new tokens, many heads to a group) so
@@ -631,10 +636,14 @@ template <typename T, int HELD, int D, int NT> int run_attention(const Kv8Attent
   IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
   const Scratch sc = carve(scratch, a.batch);
   const int q_vec = (reinterpret_cast<uintptr_t>(a.q) & 7) == 0 && a.q_token % 4 == 0 && a.q_head % 4 == 0;
-  kern<<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, q_vec);
+  const Divisors by{FastDiv((uint32_t)(a.q_heads / a.heads)), FastDiv((uint32_t)a.block)};
+  kern<<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, by, q_vec);
   if (cudaPeekAtLastError() != cudaSuccess) return cuda_fail(cudaGetLastError(), "attention_kv8 launch");
+  // few rows have many pieces each: a CTA for a row; many rows have few: a warp
+  const int64_t rows = a.tokens * a.q_heads;
+  const bool many = rows > 4 * kSmCount;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.tokens * a.q_heads));
+  cfg.gridDim = dim3((unsigned)(many ? (rows + 3) / 4 : rows));
   cfg.blockDim = dim3(kJoin);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -642,7 +651,7 @@ template <typename T, int HELD, int D, int NT> int run_attention(const Kv8Attent
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, a, sc, grid));
+  IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, many ? join_kernel<T, D, NT, 1> : join_kernel<T, D, NT, 4>, a, sc, by, grid));
   return IB200_OK;
 }
 template <typename T, int HELD, int D> int run_nt(const Kv8Attention& a, int nt, int grid, void* scratch, cudaStream_t s) {
