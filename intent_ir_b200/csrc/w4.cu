@@ -43,10 +43,7 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
-#ifndef W4_STREAM
-#define W4_STREAM 16
-#endif
-// ---- few rows of x: weights stream through shared memory into mma.sync ----------------------------------
+// ---- few rows of x: weights stream through shared memory into mma.sync -----------------------------------
 // A CTA has 128 rows of q, four warps of 32 on each half of a stage's 256 k, and a slice of K; the CTAs of a cluster share the rows and split K, and
 // add their sums up through distributed shared memory in a fixed order.  One tensor copy brings a stage of q (128 rows x
 // 128 bytes, zeros outside the matrix).  Weights are the 16 rows of m16n8k16, 8 rows of x its
@@ -57,15 +54,14 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
 // A ninth warp brings everything: the weights as said, x, scales and zero points by cp.async; it and the others meet at mbarriers only.
 constexpr int kRows = 128, kThreads = 288, kStageK = 256, kRowBytes = kStageK / 2;
 enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
-constexpr int kStreamRows = W4_STREAM;  // rows of x up to which the weights stream into mma.sync
-constexpr int kBlockBytes = 48, kRowScales = 2 * kBlockBytes;  // a row's two blocks of eight scales and zero points
+constexpr int kRowScales = 144;  // a row's two blocks of eight scales, then of eight zero points' patterns; 16 bytes keep rows in different banks
 template <int XK, int NT, int G> struct Stage {  // bytes of a stage's parts
   static constexpr int kStages = NT == 1 ? 4 : 3, GROUPS = kStageK / G;
   static constexpr int X_CHUNK = XK >= X_E4M3 ? 8 : 16;                     // 8 k of a row
   static constexpr int X_AT = kRows * kRowBytes;                              // after q: x in the order of its reads
   static constexpr int XS_AT = X_AT + NT * 8 * (kStageK / 8) * X_CHUNK;       // scales of x: [group][row]
   static constexpr int BYTES = (XS_AT + GROUPS * NT * 8 * 4 + 1023) / 1024 * 1024;
-  static constexpr int S_AT = kStages * BYTES, SMEM = S_AT + 8 * 32 * kRowScales;  // behind the stages: every warp's rows' scales
+  static constexpr int S_AT = kStages * BYTES, SMEM = S_AT + kRows * kRowScales;  // behind the stages: the rows' scales
 };
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {  // the rest of the 4 is zero
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -89,11 +85,8 @@ template <uint32_t MASK> __device__ __forceinline__ uint32_t under(uint32_t x, u
 struct Zero {
   uint32_t lo, hi;
 };
-template <bool BF> __device__ __forceinline__ Zero zero_of(uint32_t z) {
-  const uint32_t zz = z * 0x10001u;
-  if (BF) return {0x43004300u | zz, 0};
-  return {0x64006400u | zz, 0xD400D400u | zz << 4};
-}
+template <bool BF> __device__ __forceinline__ uint32_t pattern_of(uint32_t z) { return (BF ? 0x43004300u : 0x64006400u) | z * 0x10001u; }
+template <bool BF> __device__ __forceinline__ Zero zero_of(uint32_t pattern) { return {pattern, BF ? 0u : (pattern << 4 & 0x00f000f0u) | 0xD400D400u}; }
 template <typename H> __device__ __forceinline__ H as_pair(uint32_t x) { return *reinterpret_cast<const H*>(&x); }
 // the pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's eight q - z; `magic`: the exponent, in a register
 template <bool BF> __device__ __forceinline__ void weights_of(uint32_t w, const Zero& z, uint32_t magic, uint32_t (&v)[4]) {
@@ -137,59 +130,62 @@ __device__ __forceinline__ void tensor_copy(uint32_t dst, const CUtensorMap* map
   asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(dst), "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(y) : "memory");
 }
-// Scales and zero points of a row, eight groups at a time.  A thread reads a block of its row one block ahead of its use, into registers, and
-// leaves it as eight f32 and eight bytes in one of two places in shared memory, from where it is read group by group.  Groups
-// behind the last one, and rows behind the last, have the scale 0.
+// Scales and zero points of a row, eight groups at a time.  Of two warps that share 32 rows one reads the scales, a row to a lane, the other the zero
+// points, one block ahead of its use, into registers; the block is left in one of two places in shared memory, as f32 and as patterns, when
+// the warps come to it.  Groups behind the last one, and rows behind the last, have the scale 0.
 struct RowBlock {
-  uint32_t s[8];
-  uint2 z;
+  uint32_t v[8];
 };
-__device__ __forceinline__ RowBlock read_block(const W4Args& a, int row, int block) {
+__device__ __forceinline__ RowBlock read_block(const W4Args& a, bool zeros, int row, int block) {
   RowBlock r;
   const int g0 = block * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.s[i] = 0;
-  r.z = make_uint2(0x08080808u, 0x08080808u);
-  if (row >= a.n || g0 >= a.groups) return r;
+  for (int i = 0; i < 8; ++i) r.v[i] = 0;
+  if (row >= a.n || g0 >= a.groups || (zeros && !a.z)) return r;
   const int64_t at = (int64_t)row * a.groups + g0;
-  if (a.s_vec) {
+  if (zeros) {
+    if (a.z_vec) {
+      const uint2 u = *reinterpret_cast<const uint2*>(a.z + at);
+      r.v[0] = u.x, r.v[1] = u.y;  // four to a word
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (g0 + i < a.groups) r.v[i] = a.z[at + i];
+    }
+  } else if (a.s_vec) {
     if (a.s_type == IB200_F32) {
       const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(a.s) + at);
       const uint4 u = p[0], v = p[1];
-      r.s[0] = u.x, r.s[1] = u.y, r.s[2] = u.z, r.s[3] = u.w, r.s[4] = v.x, r.s[5] = v.y, r.s[6] = v.z, r.s[7] = v.w;
+      r.v[0] = u.x, r.v[1] = u.y, r.v[2] = u.z, r.v[3] = u.w, r.v[4] = v.x, r.v[5] = v.y, r.v[6] = v.z, r.v[7] = v.w;
     } else {
       const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.s) + at);
-      r.s[0] = u.x, r.s[1] = u.y, r.s[2] = u.z, r.s[3] = u.w;  // two to a word
+      r.v[0] = u.x, r.v[1] = u.y, r.v[2] = u.z, r.v[3] = u.w;  // two to a word
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (g0 + i < a.groups) {
-        if (a.s_type == IB200_F32) r.s[i] = static_cast<const uint32_t*>(a.s)[at + i];
-        else r.s[i] = static_cast<const uint16_t*>(a.s)[at + i];
+        if (a.s_type == IB200_F32) r.v[i] = static_cast<const uint32_t*>(a.s)[at + i];
+        else r.v[i] = static_cast<const uint16_t*>(a.s)[at + i];
       }
-  }
-  if (a.z_vec) {
-    r.z = *reinterpret_cast<const uint2*>(a.z + at);
-  } else if (a.z) {
-    uint32_t z[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) z[i] = g0 + i < a.groups ? a.z[at + i] : 8u;
-    r.z = make_uint2(z[0] | z[1] << 8 | z[2] << 16 | z[3] << 24, z[4] | z[5] << 8 | z[6] << 16 | z[7] << 24);
   }
   return r;
 }
-__device__ __forceinline__ void leave_block(const W4Args& a, uint8_t* row, int block, const RowBlock& r) {
-  uint8_t* to = row + (block & 1) * kBlockBytes;
-  const bool pairs = a.s_vec && a.s_type != IB200_F32;
+__device__ __forceinline__ float scale_of(const W4Args& a, const RowBlock& r, int i) {
+  return value_of(a.s_vec && a.s_type != IB200_F32 ? r.v[i / 2] >> (i & 1) * 16 & 0xffffu : r.v[i], a.s_type);
+}
+template <bool BF> __device__ __forceinline__ void leave_block(const W4Args& a, bool zeros, uint8_t* row, int block, const RowBlock& r) {
+  uint4* to = reinterpret_cast<uint4*>(row + (zeros ? 64 : 0) + (block & 1) * 32);
 #pragma unroll
   for (int i = 0; i < 8; i += 4) {
-    float v[4];
+    uint32_t v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = value_of(pairs ? r.s[(i + e) / 2] >> (e & 1) * 16 & 0xffffu : r.s[i + e], a.s_type);
-    *reinterpret_cast<float4*>(to + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
+    for (int e = 0; e < 4; ++e) {
+      if (zeros) v[e] = pattern_of<BF>((a.z_vec ? r.v[(i + e) / 4] >> (e * 8) : r.v[i + e]) & 15u);
+      else v[e] = __float_as_uint(scale_of(a, r, i + e));
+    }
+    to[i / 4] = make_uint4(v[0], v[1], v[2], v[3]);
   }
-  *reinterpret_cast<uint2*>(to + 32) = r.z;
 }
 
 __device__ __forceinline__ void write_y(const W4Args& a, int m, int n, float v) {
@@ -214,13 +210,17 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
   constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[kStages], empty[kStages];
+  __shared__ volatile int dead;  // a wait ran out: nothing waits any more
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wr = warp & 3, wk = (warp >> 2) & 1, pg = row_of<G>(g);
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kRows, m0 = blockIdx.y * NT * 8;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!mbarrier_wait_bounded(bar, parity) && a.status) atomicCAS(a.status, 0, 8);
+    if (mbarrier_try_wait(bar, parity) || dead || mbarrier_wait_bounded(bar, parity)) return;
+    dead = 1;
+    if (a.status) atomicCAS(a.status, 0, 8);
   };
   if (threadIdx.x == 0) {
+    dead = 0;
     for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 8);
     mbarrier_init_fence();
   }
@@ -274,45 +274,54 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
     }
   } else {
-  // this thread's rows: 32 * wr + pg, + 8, + 16, + 24; lane t of a quad reads the scales of the one at 8 t for all four.  A warp's groups of a
-  // stage lie in one block.
-  uint8_t *scales = smem + S::S_AT + (warp * 32 + pg) * kRowScales, *mine = scales + 8 * t * kRowScales;
-  const int my_row = n0 + wr * 32 + pg + 8 * t;
-  int block = (s0 * GROUPS + wk * HALF) >> 3;
-  leave_block(a, mine, block, read_block(a, my_row, block));
-  RowBlock ahead = read_block(a, my_row, block + 1);
-  __syncwarp();
+  // this thread's rows: 32 * wr + pg, + 8, + 16, + 24.  A stage's groups lie in one block.
+  const uint8_t* scales = smem + S::S_AT + (wr * 32 + pg) * kRowScales;
+  uint8_t* mine = smem + S::S_AT + (wr * 32 + lane) * kRowScales;  // the row whose blocks this lane reads
+  const int my_row = n0 + wr * 32 + lane;
+  int block = s0 * GROUPS >> 3;
+  RowBlock ahead = read_block(a, wk, my_row, block);
+  auto next_block = [&] {
+    leave_block<BF>(a, wk, mine, block, ahead);
+    ahead = read_block(a, wk, my_row, block + 1);
+    asm volatile("bar.sync %0, 64;" ::"r"(1 + wr) : "memory");
+  };
+  next_block();
   uint32_t magic = BF ? 0x43004300u : 0x64006400u;
   asm volatile("" : "+r"(magic));  // (kept in a register)
-  const Zero eight = zero_of<BF>(8);
+  const Zero eight = zero_of<BF>(pattern_of<BF>(8));
   const bool xs_many = XK >= X_E4M3 && a.xs_groups > 1;
   for (int s = s0; s < s1; ++s) {
     wait(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
     const uint8_t* st = smem + (s - s0) % kStages * S::BYTES;
     const uint8_t *wst = st + (wr * 32 + pg) * kRowBytes, *xst = st + S::X_AT + lane * S::X_CHUNK;
-    const int group0 = s * GROUPS + wk * HALF;
-    if (group0 >> 3 != block) {
-      block = group0 >> 3;
-      leave_block(a, mine, block, ahead);
-      ahead = read_block(a, my_row, block + 1);
-      __syncwarp();
+    if (s * GROUPS >> 3 != block) {
+      block = s * GROUPS >> 3;
+      next_block();
     }
-    float sraw[4][HALF];
-    uint32_t zraw[4];  // zero points: a byte each
+    const uint8_t* from = scales + (block & 1) * 32 + ((s * GROUPS & 7) + wk * HALF) * 4;
+    uint32_t sraw[4][HALF], zraw[4][HALF];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint8_t* from = scales + 8 * r * kRowScales + (block & 1) * kBlockBytes;
+      const uint8_t* p = from + 8 * r * kRowScales;
       if (HALF == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(from + (group0 & 7) * 4);
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
         sraw[r][0] = v.x, sraw[r][HALF > 1 ? 1 : 0] = v.y, sraw[r][HALF > 2 ? 2 : 0] = v.z, sraw[r][HALF > 3 ? 3 : 0] = v.w;
-        zraw[r] = *reinterpret_cast<const uint32_t*>(from + 32 + (group0 & 7));
       } else if (HALF == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(from + (group0 & 7) * 4);
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
         sraw[r][0] = v.x, sraw[r][HALF > 1 ? 1 : 0] = v.y;
-        zraw[r] = *reinterpret_cast<const uint16_t*>(from + 32 + (group0 & 7));
       } else {
-        sraw[r][0] = *reinterpret_cast<const float*>(from + (group0 & 7) * 4);
-        zraw[r] = from[32 + (group0 & 7)];
+        sraw[r][0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+      if (a.z) {
+        if (HALF == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p + 64);
+          zraw[r][0] = v.x, zraw[r][HALF > 1 ? 1 : 0] = v.y, zraw[r][HALF > 2 ? 2 : 0] = v.z, zraw[r][HALF > 3 ? 3 : 0] = v.w;
+        } else if (HALF == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p + 64);
+          zraw[r][0] = v.x, zraw[r][HALF > 1 ? 1 : 0] = v.y;
+        } else {
+          zraw[r][0] = *reinterpret_cast<const uint32_t*>(p + 64);
+        }
       }
     }
 #pragma unroll
@@ -333,8 +342,8 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
         } else {
           w[r][0] = *reinterpret_cast<const uint32_t*>(p + r * 8 * kRowBytes);
         }
-        sg[r] = sraw[r][gi];
-        zero[r] = a.z ? zero_of<BF>(zraw[r] >> (8 * gi) & 15u) : eight;
+        sg[r] = __uint_as_float(sraw[r][gi]);
+        zero[r] = a.z ? zero_of<BF>(zraw[r][gi]) : eight;
       }
       float acc[2][NT][4];
 #pragma unroll
@@ -511,13 +520,15 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t at) {
 //   warp 16     brings the operands; x comes permuted and widened by a small launch in front, on which only x's copies wait
 //   warps 17-18 one thread each issues the MMAs of a block
 // Chunk i's widened weights arriving says that chunk i - 2 has been read back, so its buffers need no barrier of their own.
+constexpr int kTcRowScales = 84;  // a row's two blocks of eight scales, then of eight zero points as bytes; 21 words, so that rows lie in different banks
 constexpr int kTcRows = 256, kTcThreads = 608;
 template <int NX, int G> struct TcStage {
   static constexpr int GROUPS = kStageK / G;
   static constexpr int X_AT = kTcRows * kRowBytes;                        // after q: x as four [NX rows][64 k]
   static constexpr int XS_AT = X_AT + NX * kStageK * 2;                   // scales of x: [group][row]
-  static constexpr int BYTES = (XS_AT + GROUPS * NX * 4 + 1023) / 1024 * 1024, kStages = 3;
-  static constexpr int S_AT = kStages * BYTES, SMEM = S_AT + kTcRows * kRowScales;  // behind the stages: the rows' scales
+  static constexpr int BYTES = (XS_AT + GROUPS * NX * 4 + 1023) / 1024 * 1024;
+  static constexpr int kStages = 3;
+  static constexpr int S_AT = kStages * BYTES, SMEM = S_AT + kTcRows * kTcRowScales;  // behind the stages: the rows' scales
 };
 
 // x as the MMA reads it: rows of k_pad 16-bit values, each eight in the order (0, 4, 1, 5, 2, 6, 3, 7), zero outside x
@@ -560,7 +571,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kTcRows, m0 = blockIdx.y * NX;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (dead || mbarrier_wait_bounded(bar, parity)) return;
+    if (mbarrier_try_wait(bar, parity) || dead || mbarrier_wait_bounded(bar, parity)) return;
     dead = 1;
     if (a.status) atomicCAS(a.status, 0, 8);
   };
@@ -654,21 +665,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
     // ---- widen and scale ------------------------------------------------------------------------------------
     const int b = warp >> 2 & 1, half = warp >> 3, row = b * 128 + (warp & 3) * 32 + lane;  // the thread's row of q is its lane of tensor memory
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, d_at = tmem + lanes + b * 128 + half * COLS, a_at = tmem + lanes + A_AT + b * 128 + half * (KS / 2);
-    uint8_t* scales = smem + S::S_AT + row * kRowScales;
+    uint8_t* scales = smem + S::S_AT + row * kTcRowScales;
     int block = s0 * GROUPS >> 3;
-    RowBlock ahead = {};
-    auto next_block = [&] {  // the first of the two warps reads the rows' scales for both
-      if (half == 0) {
-        leave_block(a, scales, block, ahead);
-        ahead = read_block(a, n0 + row, block + 1);
+    RowBlock ahead = read_block(a, half, n0 + row, block);
+    auto next_block = [&] {
+      uint32_t* to = reinterpret_cast<uint32_t*>(scales + (half ? 64 + (block & 1) * 8 : (block & 1) * 32));
+      if (half) {
+        to[0] = a.z_vec ? ahead.v[0] : ahead.v[0] | ahead.v[1] << 8 | ahead.v[2] << 16 | ahead.v[3] << 24;
+        to[1] = a.z_vec ? ahead.v[1] : ahead.v[4] | ahead.v[5] << 8 | ahead.v[6] << 16 | ahead.v[7] << 24;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = __float_as_uint(scale_of(a, ahead, e));
       }
+      ahead = read_block(a, half, n0 + row, block + 1);
       asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 7)) : "memory");
     };
-    if (half == 0) ahead = read_block(a, n0 + row, block);
     next_block();
     uint32_t magic = BF ? 0x43004300u : 0x64006400u;
     asm volatile("" : "+r"(magic));  // (kept in a register)
-    const Zero eight = zero_of<BF>(8);
+    const Zero eight = zero_of<BF>(pattern_of<BF>(8));
     const bool xs_many = a.xs_groups > 1;
     int i = 0, old_group = 0;
     float old_scale = 0.0f;
@@ -706,11 +721,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
         block = s * GROUPS >> 3;
         next_block();
       }
-      const uint8_t* from = scales + (block & 1) * kBlockBytes;
+      const float* scales_of = reinterpret_cast<const float*>(scales + (block & 1) * 32) + (s * GROUPS & 7);
+      const uint8_t* zeros_of = scales + 64 + (block & 1) * 8 + (s * GROUPS & 7);
 #pragma unroll
       for (int c = 0; c < GROUPS; ++c, ++i) {
-        const Zero zero = a.z ? zero_of<BF>(from[32 + (s * GROUPS & 7) + c] & 15u) : eight;
-        const float scale = *reinterpret_cast<const float*>(from + ((s * GROUPS & 7) + c) * 4);
+        const Zero zero = a.z ? zero_of<BF>(pattern_of<BF>(zeros_of[c] & 15u)) : eight;
+        const float scale = scales_of[c];
         constexpr int WORDS = KS >= 32 ? 4 : 2;  // of q a time
 #pragma unroll
         for (int q = 0; q < KS / (8 * WORDS); ++q) {
@@ -820,9 +836,16 @@ template <int XK> int run_tc_rows(const W4Args& a, void* scratch, cudaStream_t s
 
 }  // namespace
 
+// Which kernel: up to 8 rows of x the weights stream into mma.sync (8192 x 8192, groups of 128, bf16: 16.4 us against 16.7 through tensor memory, and
+// 4096 x 4096 7.2 against 9.9), above 16 they go through tensor memory.  Between, mma.sync takes two column tiles: 10.2 against 10.4 us at 4096 x 4096, but 22.7
+// against 17.2 at 8192 x 8192, and 11.2 against 16.7 with groups of 32, whose sums come back four times as often.
+static bool through_tensor_memory(int64_t m, int64_t n, int64_t k, int64_t group) {
+  return k > 0 && (m > 16 || (m > 8 && group == 128 && n * k >= (int64_t)1 << 26));
+}
+
 // room for x as the MMA reads it
-size_t w4_scratch_bytes(int, int64_t m, int64_t n, int64_t k, int64_t) {
-  if (m <= kStreamRows || n <= 0 || k <= 0 || beyond_any_device(m, k) || k > INT32_MAX - 1024) return 0;
+size_t w4_scratch_bytes(int, int64_t m, int64_t n, int64_t k, int64_t group) {
+  if (m <= 0 || n <= 0 || k <= 0 || beyond_any_device(m, k) || beyond_any_device(n, k) || k > INT32_MAX - 1024 || !through_tensor_memory(m, n, k, group)) return 0;
   return (size_t)(padded(m, tc_columns(m)) * padded(k, kStageK) * 2);
 }
 
@@ -852,7 +875,7 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
            (int)m, (int)n, (int)k, (int)group, (int)groups, (int)xs_groups, x_dtype, s_dtype, out_dtype, x_vec, 0, 0, 1, status};
   a.s_vec = groups % 8 == 0 && aligned16(scales);
   a.z_vec = zeros && groups % 8 == 0 && (reinterpret_cast<uintptr_t>(zeros) & 7) == 0;
-  if (m > kStreamRows && k > 0) {
+  if (through_tensor_memory(m, n, k, group)) {
     if (!scratch || scratch_bytes < w4_scratch_bytes(x_dtype, m, n, k, group)) return fail(IB200_ERR_BUFFER, "w4_matmul: scratch is smaller than ib200_w4_scratch_bytes");
     if (x_dtype == IB200_BF16) return run_tc_rows<X_BF16>(a, scratch, s);
     if (x_dtype == IB200_F16) return run_tc_rows<X_F16>(a, scratch, s);
