@@ -287,7 +287,7 @@ IB200_API int ib200_transpose2d(const void* x, void* out, int elem_bytes, int64_
  * h = x + residual;  y = h / sqrt(mean(h^2) + eps) * w  over rows of `cols` elements, computed from the unrounded sum.
  * residual may be NULL (h = x); h (its rounded value, row stride h_stride) may be NULL, and may be the memory of x or
  * residual.  dtype (x, residual, h): IB200_F32, IB200_BF16 or IB200_F16; w (NULL: ones) has dtype or IB200_F32.  out_dtype:
- * dtype, or IB200_E4M3 / IB200_I8 with scale[rows, groups] (f32):  s = max|y| / Q over a group, y / s rounded to nearest even,
+ * dtype, or IB200_E4M3 / IB200_I8 with scale[rows, groups] (f32):  s = max|y| * (1/Q) over a group, y / s rounded to nearest even,
  * Q = 448 / 127.  group: 32, 64, 128 or 256 columns (the last one may be shorter), 0: the row.  A group of zeros (or below
  * 2^-119) holds zeros; one with a NaN or an infinity has a NaN or infinite scale and stands for NaN.  y is dense. */
 typedef struct ib200_rmsnorm_args {
@@ -328,7 +328,7 @@ IB200_API size_t ib200_w4_scratch_bytes(int x_dtype, int64_t m, int64_t n, int64
  * 16 up to 1024; dim 64 or 128; dtype (k, v, q, o) bf16 or f16; caches 16-byte aligned.  The contents of table, lens and cu
  * are not trusted: pages outside the cache and tokens outside the table are neither read nor written.  Tokens behind cu[batch] are left alone.
  *
- * append: the block of a head gets the scale s' = max(s, max|new| / Q), s = 0 where the block begins with a new token; values held before are
+ * append: the block of a head gets the scale s' = max(s, max|new| * (1/Q)), s = 0 where the block begins with a new token; values held before are
  * rounded again to q * s / s' where s' > s, new ones to x / s' (nearest even).  Slots behind a sequence's end are left as they are.
  * No two sequences may append to one page in the same call. */
 typedef struct ib200_kv8_append_args {

@@ -11,6 +11,8 @@ enum : int { HELD_NONE = 0, HELD_E4M3 = 1, HELD_I8 = 2 };
 
 #ifdef __CUDACC__
 template <int HELD> __device__ __forceinline__ constexpr float held_top() { return HELD == HELD_E4M3 ? 448.0f : 127.0f; }
+// 1 / Q in f32: a scale is the largest magnitude times this
+template <int HELD> __device__ __forceinline__ constexpr float held_unit() { return HELD == HELD_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f; }
 // What a value is multiplied by before it is rounded: Q / max|y|, 0 for a group of zeros (which then holds zeros) and where the
 // quotient overflows (max|y| below 2^-119: the group is held as zeros).  A NaN stays a NaN; an infinite maximum gives 0.
 template <int HELD> __device__ __forceinline__ float held_inverse(float top) {

@@ -14,7 +14,7 @@ namespace {
 
 // ---- append -----------------------------------------------------------------------------------------
 // A unit is the new tokens of one block: for a head, one warp (few tokens) or CTA for the keys and one for the values.
-//   s' = max(s, max|new| / Q), s = 0 for a block that begins here; held values become round(q * s / s') where s' > s, new ones round(x / s')
+//   s' = max(s, max|new| * (1 / Q)), s = 0 for a block that begins here; held values become round(q * s / s') where s' > s, new ones round(x / s')
 // Quotients round as IEEE divisions do: the held values depend on nothing but their definition.  The new values are read once
 // into registers (up to KEEP vectors of 8 a thread: 16 tokens of 128 in a warp, 64 in a CTA; more are read again) and written 8 bytes at a time.
 template <typename T> __device__ __forceinline__ uint4 read_new(const T* p, bool vec) {
@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Kv8Append a, cons
   for (int i = tid + KEEP * THREADS; i < vectors; i += THREADS) enter(read_new(source(i), vec));
   float top = max_nan(to_f32(largest.x), to_f32(largest.y));
   top = THREADS == 32 ? warp_reduce<MaxOp>(top) : block_reduce<MaxOp>(top, slots);  // (the barrier: every thread has read the old scale)
-  const float after = max_nan(before, top / held_top<HELD>()), div = after == 0.0f ? 1.0f : after, inv = 1.0f / div;
+  const float after = max_nan(before, top * held_unit<HELD>()), div = after == 0.0f ? 1.0f : after, inv = 1.0f / div;
   if (THREADS == 32) __syncwarp();
   if (tid == 0) *scale = after;
   if (!(after == before)) {

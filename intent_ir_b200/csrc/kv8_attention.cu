@@ -114,6 +114,8 @@ template <typename T, int HELD, int D, int NT>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kCtas - 1) attention_kernel(const Kv8Attention a, const Scratch sc, const Divisors by, const int q_vec) {
   using C = Cfg<D>;
   constexpr int ROWS = 8 * NT, HALVES = D / 64, MT = D / 16, CH = D / 16;  // CH: 16-byte chunks of a token
+  // An f16 result is off by 2^-12 of itself, no more than p rounded to f16 once: there p is multiplied in two parts.  (bf16's 2^-9 hides it.)
+  constexpr bool kTwice = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t sums[kWarps], found_before;
   __shared__ int found;
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
         vtop = up;
       }
       const float vf[2] = {vs[0] * (0x1p14f / vtop), vs[1] * (0x1p14f / vtop)};
-      uint32_t pf[NT][2][2];
+      uint32_t pf[NT][2][2], pl[NT][2][2];  // p, and what its rounding left
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float top[2] = {-INFINITY, -INFINITY};
@@ -390,8 +392,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
               if (key > hi[nt][c & 1] || key < low[nt][c & 1]) p[mt][c] = 0.0f;
             }
           }
-          pf[nt][mt][0] = transpose8x8(pack16(p[mt][0], p[mt][1]));
-          pf[nt][mt][1] = transpose8x8(pack16(p[mt][2], p[mt][3]));
+          const uint32_t p0 = pack16(p[mt][0], p[mt][1]), p1 = pack16(p[mt][2], p[mt][3]);
+          pf[nt][mt][0] = transpose8x8(p0);
+          pf[nt][mt][1] = transpose8x8(p1);
+          if constexpr (kTwice) {
+            const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&p0)), h1 = __half22float2(*reinterpret_cast<const __half2*>(&p1));
+            pl[nt][mt][0] = transpose8x8(pack16(p[mt][0] - h0.x, p[mt][1] - h0.y));
+            pl[nt][mt][1] = transpose8x8(pack16(p[mt][2] - h1.x, p[mt][3] - h1.y));
+          }
         }
         const float k0 = keep[0] * grow, k1 = keep[1] * grow;
 #pragma unroll
@@ -439,7 +447,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) mma16816(o[nt][2 * k + i], f[i][0], f[i][1], f[i][2], f[i][3], pf[nt][mt][0], pf[nt][mt][1]);
+              for (int i = 0; i < 2; ++i) {
+                mma16816(o[nt][2 * k + i], f[i][0], f[i][1], f[i][2], f[i][3], pf[nt][mt][0], pf[nt][mt][1]);
+                if constexpr (kTwice) mma16816(o[nt][2 * k + i], f[i][0], f[i][1], f[i][2], f[i][3], pl[nt][mt][0], pl[nt][mt][1]);
+              }
           } else {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -453,9 +464,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
                   keep[e] = (key <= last && key >= begin ? 0xffffu : 0u) | (key + 1 <= last && key + 1 >= begin ? 0xffff0000u : 0u);
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i) {
                   mma16816(o[nt][2 * k + i], f[i][0] & keep[0], f[i][1] & keep[0], f[i][2] & keep[1], f[i][3] & keep[1], g == col ? pf[nt][mt][0] : 0u,
                            g == col ? pf[nt][mt][1] : 0u);
+                  if constexpr (kTwice)
+                    mma16816(o[nt][2 * k + i], f[i][0] & keep[0], f[i][1] & keep[0], f[i][2] & keep[1], f[i][3] & keep[1], g == col ? pl[nt][mt][0] : 0u,
+                             g == col ? pl[nt][mt][1] : 0u);
+                }
               }
           }
         }

@@ -1,5 +1,5 @@
 // Root-mean-square norm with the residual's addition in front and, on request, an 8-bit result with scales:
-//   h = x + residual;  y = h / sqrt(mean(h^2) + eps) * w;  per group of columns  s = max|y| / Q,  q = round(y * Q / max|y|)
+//   h = x + residual;  y = h / sqrt(mean(h^2) + eps) * w;  per group of columns  s = max|y| * (1 / Q),  q = round(y * Q / max|y|)
 // with Q = 448 (e4m3) or 127 (int8).  h is stored rounded to the row type; everything else is computed from the unrounded
 // f32 sum, so the stored rounding of h does not enter y.
 #include "common.cuh"
@@ -53,11 +53,10 @@ template <typename T> __device__ __forceinline__ void load_w8(const RmsArgs& a, 
 template <typename T> __device__ __forceinline__ float load_w(const RmsArgs& a, int64_t at) {
   return a.wide_w ? static_cast<const float*>(a.w)[at] : to_f32(static_cast<const T*>(a.w)[at]);
 }
-__device__ __forceinline__ float top_of(int type) { return type == IB200_E4M3 ? held_top<HELD_E4M3>() : held_top<HELD_I8>(); }
+__device__ __forceinline__ float top_inverse(int type) { return type == IB200_E4M3 ? held_unit<HELD_E4M3>() : held_unit<HELD_I8>(); }
 __device__ __forceinline__ float inverse_of(int type, float top) { return type == IB200_E4M3 ? held_inverse<HELD_E4M3>(top) : held_inverse<HELD_I8>(top); }
 
-// The same to 2 ulp without divisions, for the scales of groups, of which there are many
-__device__ __forceinline__ float top_inverse(int type) { return type == IB200_E4M3 ? 1.0f / 448.0f : 1.0f / 127.0f; }
+// The same to 2 ulp without a division, for the scales of groups, of which there are many
 __device__ __forceinline__ float inverse_fast(int type, float top) {
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
@@ -210,7 +209,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
     float inv = 0.0f;
     if (a.group == 0) {
       top = THREADS == 32 ? warp_reduce<MaxOp>(top) : block_reduce<MaxOp>(top, slots[1]);
-      if (tid == 0) a.scale[row] = top / top_of(a.out_type);
+      if (tid == 0) a.scale[row] = top * top_inverse(a.out_type);
       inv = inverse_of(a.out_type, top);
     }
     const int lanes = a.group / VE, steps = a.group / 32, shift = __ffs(a.group) - 1;  // of a scale: lanes with VEC, elements of a lane without
@@ -322,7 +321,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
         for (int i = 0; i < VE; ++i) row_max = max_nan(row_max, fabsf(e[i]));
       }
       row_max = block_reduce<MaxOp>(row_max, slots[1]);
-      if (threadIdx.x == 0) a.scale[row] = row_max / top_of(a.out_type);
+      if (threadIdx.x == 0) a.scale[row] = row_max * top_inverse(a.out_type);
     }
     for (int64_t v = threadIdx.x; v < nv_warp; v += THREADS) {
       float e[VE];
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
 #pragma unroll
           for (int i = 0; i < VE; ++i) top = max_nan(top, fabsf(e[i]));
           for (int o = lanes >> 1; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (v < nv && (v % lanes) == 0) a.scale[row * a.groups + v / lanes] = top / top_of(a.out_type);
+          if (v < nv && (v % lanes) == 0) a.scale[row * a.groups + v / lanes] = top * top_inverse(a.out_type);
         }
         if (v < nv) {
           uint8_t* y = static_cast<uint8_t*>(a.y) + row * a.cols + v * VE;

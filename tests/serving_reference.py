@@ -87,7 +87,8 @@ def hold(x, dtype):
 
 
 def append(k, v, k_cache, v_cache, k_scale, v_scale, table, lens, cu):
-    """In place on CPU tensors, sequence by sequence and block by block, with the f32 divisions of the definition."""
+    """In place on CPU tensors, sequence by sequence and block by block, with the f32 arithmetic of the definition: a scale is the largest
+    magnitude times 1 / Q, a held value the rounded quotient."""
     pages, heads, block, dim = k_cache.shape
     for b in range(len(lens)):
         n = int(cu[b + 1] - cu[b])
@@ -102,7 +103,7 @@ def append(k, v, k_cache, v_cache, k_scale, v_scale, table, lens, cu):
                     new = x[int(cu[b]) + lo - start:int(cu[b]) + hi - start, h].float().numpy()
                     top = np.float32(TOP[cache.dtype])
                     before = np.float32(scale[page, h]) if lo > blk * block else np.float32(0)
-                    after = np.maximum(before, np.abs(new).max() / top)
+                    after = np.maximum(before, np.abs(new).max() * (np.float32(1) / top))
                     div = after if after != 0 else np.float32(1)
                     with np.errstate(invalid="ignore", divide="ignore"):
                         if not after == before:
