@@ -23,6 +23,16 @@ int cuda_fail(cudaError_t err, const char* what) {
 
 using namespace ib200;
 
+static int code(int64_t v) { return v >= 0 && v < 256 ? (int)v : -1; }
+// no exception (an allocation that failed, for a message or a map) leaves a C entry
+template <typename F> static int guarded(F f) noexcept {
+  try {
+    return f();
+  } catch (...) {
+    return IB200_ERR_CUDA;
+  }
+}
+
 extern "C" {
 
 const char* ib200_last_error(void) { return g_last_error.c_str(); }
@@ -139,37 +149,43 @@ int ib200_transpose2d(const void* x, void* out, int elem_bytes, int64_t rows, in
   return launch_transpose2d(x, out, elem_bytes, rows, cols, static_cast<cudaStream_t>(stream));
 }
 
-static int code(int64_t v) { return v >= 0 && v < 256 ? (int)v : -1; }
-
 int ib200_rmsnorm(const ib200_rmsnorm_args* a, void* stream) {
-  if (!a) return fail(IB200_ERR_INVALID, "rmsnorm: no arguments");
-  return launch_rmsnorm(a->x, a->x_stride, a->residual, a->residual_stride, a->w, a->y, a->h, a->h_stride, a->scale, code(a->dtype),
-                        code(a->w_dtype), code(a->out_dtype), a->rows, a->cols, a->group, (float)a->eps, static_cast<cudaStream_t>(stream));
+  return guarded([&] {
+    if (!a) return fail(IB200_ERR_INVALID, "rmsnorm: no arguments");
+    return launch_rmsnorm(a->x, a->x_stride, a->residual, a->residual_stride, a->w, a->y, a->h, a->h_stride, a->scale, code(a->dtype),
+                          code(a->w_dtype), code(a->out_dtype), a->rows, a->cols, a->group, (float)a->eps, static_cast<cudaStream_t>(stream));
+  });
 }
 
 int ib200_w4_matmul(const ib200_w4_args* a, void* stream) {
-  if (!a) return fail(IB200_ERR_INVALID, "w4_matmul: no arguments");
-  if (reinterpret_cast<uintptr_t>(a->scratch) & 255u) return fail(IB200_ERR_INVALID, "w4_matmul: scratch must be 256-byte aligned");
-  return launch_w4(a->x, a->x_stride, a->x_scale, a->x_scale_groups, a->q, a->scales, a->zeros, a->bias, a->y, code(a->x_dtype), code(a->s_dtype),
-                   code(a->out_dtype), a->m, a->n, a->k, a->group, a->scratch, (size_t)a->scratch_bytes, a->status, static_cast<cudaStream_t>(stream));
+  return guarded([&] {
+    if (!a) return fail(IB200_ERR_INVALID, "w4_matmul: no arguments");
+    if (reinterpret_cast<uintptr_t>(a->scratch) & 255u) return fail(IB200_ERR_INVALID, "w4_matmul: scratch must be 256-byte aligned");
+    return launch_w4(a->x, a->x_stride, a->x_scale, a->x_scale_groups, a->q, a->scales, a->zeros, a->bias, a->y, code(a->x_dtype), code(a->s_dtype),
+                     code(a->out_dtype), a->m, a->n, a->k, a->group, a->scratch, (size_t)a->scratch_bytes, a->status, static_cast<cudaStream_t>(stream));
+  });
 }
 size_t ib200_w4_scratch_bytes(int x_dtype, int64_t m, int64_t n, int64_t k, int64_t group) { return w4_scratch_bytes(x_dtype, m, n, k, group); }
 
 int ib200_kv8_append(const ib200_kv8_append_args* a, void* stream) {
-  if (!a) return fail(IB200_ERR_INVALID, "kv8_append: no arguments");
-  Kv8Append k{a->k, a->v, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, static_cast<uint8_t*>(a->k_cache),
-              static_cast<uint8_t*>(a->v_cache), a->k_scale, a->v_scale, a->table, a->lens, a->cu, a->pages, a->heads, a->block, a->dim, a->batch,
-              a->table_blocks, a->tokens, 0, 0};
-  return launch_kv8_append(k, code(a->dtype), code(a->held), static_cast<cudaStream_t>(stream));
+  return guarded([&] {
+    if (!a) return fail(IB200_ERR_INVALID, "kv8_append: no arguments");
+    Kv8Append k{a->k, a->v, a->k_token_stride, a->k_head_stride, a->v_token_stride, a->v_head_stride, static_cast<uint8_t*>(a->k_cache),
+                static_cast<uint8_t*>(a->v_cache), a->k_scale, a->v_scale, a->table, a->lens, a->cu, a->pages, a->heads, a->block, a->dim, a->batch,
+                a->table_blocks, a->tokens, 0, 0};
+    return launch_kv8_append(k, code(a->dtype), code(a->held), static_cast<cudaStream_t>(stream));
+  });
 }
 
 int ib200_attention_kv8(const ib200_attention_kv8_args* a, void* stream) {
-  if (!a) return fail(IB200_ERR_INVALID, "attention_kv8: no arguments");
-  if (reinterpret_cast<uintptr_t>(a->scratch) & 255u) return fail(IB200_ERR_INVALID, "attention_kv8: scratch must be 256-byte aligned");
-  Kv8Attention k{a->q, a->q_token_stride, a->q_head_stride, static_cast<const uint8_t*>(a->k_cache), static_cast<const uint8_t*>(a->v_cache),
-                 a->k_scale, a->v_scale, a->table, a->lens, a->cu, a->o, a->lse, a->pages, a->heads, a->block, a->dim, a->batch, a->table_blocks,
-                 a->tokens, a->q_heads, a->window, (float)a->scale, 0};
-  return launch_kv8_attention(k, code(a->dtype), code(a->held), a->scratch, (size_t)a->scratch_bytes, static_cast<cudaStream_t>(stream));
+  return guarded([&] {
+    if (!a) return fail(IB200_ERR_INVALID, "attention_kv8: no arguments");
+    if (reinterpret_cast<uintptr_t>(a->scratch) & 255u) return fail(IB200_ERR_INVALID, "attention_kv8: scratch must be 256-byte aligned");
+    Kv8Attention k{a->q, a->q_token_stride, a->q_head_stride, static_cast<const uint8_t*>(a->k_cache), static_cast<const uint8_t*>(a->v_cache),
+                   a->k_scale, a->v_scale, a->table, a->lens, a->cu, a->o, a->lse, a->pages, a->heads, a->block, a->dim, a->batch, a->table_blocks,
+                   a->tokens, a->q_heads, a->window, (float)a->scale, 0};
+    return launch_kv8_attention(k, code(a->dtype), code(a->held), a->scratch, (size_t)a->scratch_bytes, static_cast<cudaStream_t>(stream));
+  });
 }
 size_t ib200_attention_kv8_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block,
                                          int64_t table_blocks) {

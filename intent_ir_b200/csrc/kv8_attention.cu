@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
         vtop = up;
       }
       const float vf[2] = {vs[0] * (0x1p14f / vtop), vs[1] * (0x1p14f / vtop)};
-      uint32_t pf[NT][2][2], pl[NT][2][2];  // p, and what its rounding left
+      uint32_t pf[NT][2][2];
+      [[maybe_unused]] uint32_t pl[NT][2][2];  // what p's rounding left
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float top[2] = {-INFINITY, -INFINITY};

@@ -140,6 +140,16 @@ def test_rmsnorm_refusals(ops):
         ops.rmsnorm(x.cpu())
 
 
+def test_rmsnorm_beyond_two_billion_elements(ops):
+    rows, cols = 140000, 16384
+    x = torch.empty(rows, cols, dtype=BF16, device="cuda")
+    x[:] = torch.randn(cols, device="cuda").to(BF16)
+    x[-3:] = torch.randn(3, cols, device="cuda").to(BF16)
+    y, scale, _ = ops.rmsnorm(x, out_dtype=E4M3, group=128)
+    _, want = ref.rmsnorm(x[-4:].cpu(), None, None, 1e-6)
+    ref.check_held(y[-4:].cpu(), scale[-4:].cpu(), want, 128, (cols / 16 + 16) * 2.0**-24)
+
+
 # ---- products with 4-bit weights --------------------------------------------------------------------
 
 def _w4_case(m, n, k, dtype, group, zeros, bias, x_groups, scale_dtype, seed=0, out_dtype=None):
@@ -222,6 +232,41 @@ def test_w4_strides_axes_large_values_and_empty(ops):
     empty = ops.w4_matmul(torch.empty(2, 0, dtype=BF16, device="cuda"), torch.empty(7, 0, dtype=torch.uint8, device="cuda"),
                           torch.empty(7, 0, dtype=BF16, device="cuda"), bias=bias)
     assert torch.equal(empty, bias.expand(2, 7))
+
+
+@pytest.mark.parametrize("m", [1, 12, 40])
+def test_w4_scales_and_zero_points_off_their_boundaries(ops, m):
+    """Groups that fill their blocks of eight or not, in arrays that begin anywhere."""
+    for k, group in ((2048, 128), (2048, 32), (1056, 32), (1152, 128)):
+        for scale_dtype in (BF16, F32):
+            d, out = _w4_case(m, 150, k, F16, group, True, True, 0, scale_dtype)
+            want = _check_w4(ops, d, out)
+            e = {n: v.cuda() if isinstance(v, torch.Tensor) else v for n, v in d.items()}
+            for name in ("scales", "zeros", "bias"):
+                box = torch.empty(e[name].numel() + 3, dtype=e[name].dtype, device="cuda")
+                for off in (1, 3):
+                    view = box[off:off + e[name].numel()].view(e[name].shape)
+                    view.copy_(e[name])
+                    assert torch.equal(ops.w4_matmul(**{**e, name: view}, out_dtype=out), want), (k, group, name, off)
+
+
+@pytest.mark.parametrize("m", [9, 16])
+def test_w4_larger_matrices_with_a_few_rows(ops, m):
+    d, out = _w4_case(m, 8200, 8192, BF16, 128, m == 9, False, 0, BF16)
+    _check_w4(ops, d, out)
+
+
+@pytest.mark.parametrize("m", [1, 20])
+def test_w4_weights_beyond_two_gigabytes(ops, m):
+    n, k, group = 66000, 65536, 128
+    q = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda")
+    scales = (torch.rand(n, k // group, device="cuda") * 0.01).to(BF16)
+    x = torch.randn(m, k, device="cuda").to(BF16)
+    got = ops.w4_matmul(x, q, scales, group=group)
+    for at in (0, 65520, n - 40):
+        part = {"x": x.cpu(), "q": q[at:at + 40].cpu(), "scales": scales[at:at + 40].cpu(), "zeros": None, "bias": None, "x_scale": None, "group": group}
+        want, size = ref.w4_matmul(**part)
+        assert ((got[:, at:at + 40].cpu().double() - want).abs() <= ref.w4_bound(want, size, k, BF16)).all()
 
 
 def test_w4_refusals(ops):
@@ -366,6 +411,35 @@ def test_append_zeros_and_non_finite_values(ops, held):
     assert torch.isnan(o[6:]).all()
 
 
+@pytest.mark.parametrize("held", [E4M3, I8])
+def test_append_and_attention_in_a_cache_beyond_two_billion_values(ops, held):
+    d = _paged(14, [3, 40], [70, 300], 8, 128, 16, BF16, held)
+    q = torch.randn(43, 8, 128, generator=_gen(2)).to(BF16)
+    small = _cuda(d)
+    pages, used = 140000, d["k_cache"].shape[0]
+    big = dict(small, block_table=torch.where(small["block_table"] >= 0, small["block_table"] + (pages - used), small["block_table"]))
+    for c in CACHE:
+        big[c] = torch.zeros((pages,) + tuple(small[c].shape[1:]), dtype=small[c].dtype, device="cuda")
+        big[c][pages - used:].view(torch.uint8).copy_(small[c].view(torch.uint8))
+    out = []
+    for s in (small, big):
+        args = [s[c] for c in CACHE] + [s["block_table"], s["seq_lens"]]
+        ops.kv8_append(s["k"], s["v"], *args, cu_new=s["cu_new"])
+        out.append(ops.attention_kv8(q.cuda(), *args, cu_new=s["cu_new"]))
+    assert torch.equal(*out) and torch.isfinite(out[0]).all()
+    for c in CACHE:
+        assert torch.equal(big[c][pages - used:].view(torch.uint8), small[c].view(torch.uint8))
+        assert not big[c][:pages - used].view(torch.uint8).any()
+
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+def test_append_a_padded_batch(ops, held):
+    """Sequences of length 0 with a place among the new tokens: nothing is written for them."""
+    d = _paged(15, [1] * 5, [40, 0, 17, 0, 0], 2, 64, 16, BF16, held)
+    _check_append(ops, d, uniform=True)
+    _check_attention(ops, {**d}, 4, uniform=True)
+
+
 def test_append_strided_inputs(ops):
     d = _paged(13, [2, 7], [20, 39], 3, 64, 16, BF16, E4M3)
     fused = torch.randn(9, 5 * 3, 64, generator=_gen(3)).to(BF16)
@@ -420,6 +494,19 @@ def test_attention_several_tokens_and_windows(ops, held, heads, group, dim, bloc
 def test_attention_long_sequences_beside_short_ones(ops, held):
     _check_attention(ops, _paged(24, [1] * 5, [20000, 3, 700, 1, 9001], 2, 128, 32, BF16, held), 8, uniform=True)
     _check_attention(ops, _paged(25, [2, 1, 2], [30001, 1, 77], 1, 64, 16, F16, held), 4)
+
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+def test_attention_many_sequences(ops, held):
+    """More sequences than a CTA has threads, and pages that several of them share."""
+    lens = [(i * 37) % 200 for i in range(300)]
+    d = _paged(31, [1] * 300, lens, 1, 64, 16, BF16, held)
+    _check_attention(ops, d, 4, uniform=True)
+    news = [i % 3 for i in range(290)]
+    d = _paged(32, news, [max(n, x) for n, x in zip(news, lens)], 2, 64, 16, F16, held)
+    d["block_table"][5:40] = d["block_table"][4]  # read by all: nobody appends here
+    d["seq_lens"][5:40] = d["seq_lens"][4]
+    _check_attention(ops, d, 2, window=50)
 
 
 @pytest.mark.parametrize("held", [E4M3, I8])
@@ -530,6 +617,20 @@ def test_the_step_together(ops, held, out8):
     again = _cuda(_layer_inputs(held))
     for a, b in zip(_layer(ops, again, held, out8), (y, scale, h)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))  # the same inputs, the same bits
+
+
+def test_two_steps_at_once_on_two_streams(ops):
+    want = [t.clone() for t in _layer(ops, _cuda(_layer_inputs(E4M3)), E4M3, I8)]
+    states = [_cuda(_layer_inputs(E4M3)) for _ in range(8)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, s in enumerate(states):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(_layer(ops, s, E4M3, I8))
+    torch.cuda.synchronize()
+    for out in got:
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(out, want))
 
 
 def test_the_step_on_another_stream_and_in_a_graph(ops):
