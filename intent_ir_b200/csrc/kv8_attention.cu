@@ -12,6 +12,7 @@
 // O' = V' P', so that 8 queries fill a fragment where queries as rows would need 16.  Bytes are widened to f16, which
 // is exact for both types; scales are applied to the scores and to p.  q is scaled by a power of two to below 2 (exact), p * vs
 // by another one to below 2^15, so that f16 holds them to 2^-12 over 2^39.
+#include <atomic>
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -649,7 +650,13 @@ int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int
 
 template <typename T, int HELD, int D, int NT> int run_attention(const Kv8Attention& a, int grid, void* scratch, cudaStream_t s) {
   auto* kern = attention_kernel<T, HELD, D, NT>;
-  IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
+  static std::atomic<uint64_t> ready{0};  // devices that have been told of the shared memory
+  int dev = 0;
+  IB200_CUDA_OK(cudaGetDevice(&dev));
+  if (dev > 63 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    IB200_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem));
+    if (dev <= 63) ready.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+  }
   const Scratch sc = carve(scratch, a.batch);
   const int q_vec = (reinterpret_cast<uintptr_t>(a.q) & 7) == 0 && a.q_token % 4 == 0 && a.q_head % 4 == 0;
   const Divisors by{FastDiv((uint32_t)(a.q_heads / a.heads)), FastDiv((uint32_t)a.block)};

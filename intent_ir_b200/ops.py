@@ -260,6 +260,10 @@ _HALF_CODE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _HELD_CODE = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.I8}
 
 
+_current_device = torch._C._cuda_getDevice  # what torch.cuda.current_device asks, once CUDA is up; there is a CUDA tensor by then
+_stream_of = torch._C._cuda_getCurrentRawStream  # the handle of torch.cuda.current_stream(device)
+
+
 def _on_device(index: int, **tensors: Optional[torch.Tensor]) -> None:
     for name, t in tensors.items():
         if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index):
@@ -268,10 +272,11 @@ def _on_device(index: int, **tensors: Optional[torch.Tensor]) -> None:
 
 def _first(name: str, t) -> int:
     """The device of a call's first tensor."""
-    index = t.get_device() if isinstance(t, torch.Tensor) else -1
-    if index < 0:
-        raise B200RuntimeError(f"{name} must be a CUDA tensor")
-    return index
+    if isinstance(t, torch.Tensor):
+        index = t.get_device()
+        if index >= 0:
+            return index
+    raise B200RuntimeError(f"{name} must be a CUDA tensor")
 
 
 def _dense(name: str, t: torch.Tensor, shape: Sequence[int], dtype: torch.dtype) -> None:
@@ -317,7 +322,7 @@ def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optiona
     with one f32 scale for each row (``group`` 0) or for each 32, 64, 128 or 256 columns; otherwise y has the type of x and
     scale is None.  x is f32, bf16 or f16; w has its type or f32; x, residual and residual_out may be matrices of spaced rows."""
     index = _first("x", x)
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
             return rmsnorm(x, w, residual, eps, out_dtype, group, residual_out)
     stride = _row_stride("x", x)
@@ -355,7 +360,7 @@ def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optiona
         scale = _dense_empty(shape[:-1] + ((cols + group - 1) // group if group > 0 else 1,), torch.float32, x.device)
     args = _lib.RMSNORM_ARGS.pack(x.data_ptr(), _address(residual), _address(w), y.data_ptr(), _address(h), _address(scale), stride, res_stride, h_stride,
                                   code, w_code, out_code, shape[:-1].numel(), cols, group, eps)
-    rc = _lib.load().ib200_rmsnorm(args, _stream())
+    rc = _lib.load().ib200_rmsnorm(args, _stream_of(index))
     if rc:
         _check(rc, "rmsnorm")
     return y, scale, h
@@ -370,10 +375,12 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
     [.., ceil(K / group)], as ``rmsnorm`` returns them.  ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.
     K is a multiple of 32, the group 32, 64 or 128."""
     index = _first("x", x)
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
             return w4_matmul(x, q, scales, zeros, bias, x_scale, group, out_dtype)
-    _on_device(index, q=q, scales=scales, zeros=zeros, bias=bias, x_scale=x_scale)
+    for t in (q, scales, zeros, bias, x_scale):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != index):
+            _on_device(index, q=q, scales=scales, zeros=zeros, bias=bias, x_scale=x_scale)
     if q is None or scales is None or q.dim() != 2 or group not in (32, 64, 128):
         raise B200LoweringError("w4_matmul: q is a matrix, the group 32, 64 or 128")
     stride = _row_stride("x", x)
@@ -410,7 +417,7 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
     scratch = _dense_empty((need,), torch.uint8, x.device) if need else None
     args = _lib.W4_ARGS.pack(x.data_ptr(), _address(x_scale), q.data_ptr(), scales.data_ptr(), _address(zeros), _address(bias), y.data_ptr(), _address(scratch),
                              _status_address(index), stride, x_groups, x_code, _code("scales", scales, _FLOAT_CODE), _FLOAT_CODE[out_dtype], m, n, k, group, need)
-    rc = _lib.load().ib200_w4_matmul(args, _stream())
+    rc = _lib.load().ib200_w4_matmul(args, _stream_of(index))
     if rc:
         _check(rc, "w4_matmul")
     return y
@@ -485,7 +492,7 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     grows with its block's largest value, and the values held before are rounded again; slots behind the end, tokens behind
     ``cu_new[-1]``, and pages or tokens outside the cache and the table are left alone.  No two sequences may append to one page."""
     index = _first("k", k)
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
             return kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
     held, pages, heads, block, dim, batch, table_blocks = _cache_extents(index, "k", k, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
@@ -497,7 +504,7 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     args = _lib.KV8_APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                      block_table.data_ptr(), seq_lens.data_ptr(), _address(cu_new), k_token, k_head, v_token, v_head,
                                      _code("k", k, _HALF_CODE), held, k.shape[0], batch, heads, dim, pages, block, table_blocks)
-    rc = _lib.load().ib200_kv8_append(args, _stream())
+    rc = _lib.load().ib200_kv8_append(args, _stream_of(index))
     if rc:
         _check(rc, "kv8_append")
 
@@ -512,7 +519,7 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     the softmax's denominators.  Rows without keys are 0 (lse -inf); rows that need a page outside the cache or a token outside the
     table are NaN; tokens behind ``cu_new[-1]`` are not written."""
     index = _first("q", q)
-    if index != torch.cuda.current_device():
+    if index != _current_device():
         with torch.cuda.device(index):
             return attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new, scale, window, return_lse, out)
     held, pages, heads, block, dim, batch, table_blocks = _cache_extents(index, "q", q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_new)
@@ -522,15 +529,16 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     else:
         _on_device(index, out=out)
         _dense("out", out, shape, q.dtype)
-    lse = _dense_empty((tokens, q_heads), torch.float32, q.device) if return_lse else None
+    dev = q.device
+    lse = torch.empty_strided((tokens, q_heads), (q_heads, 1), dtype=torch.float32, device=dev) if return_lse else None
     need = _attention_scratch(tokens, batch, q_heads, heads, dim, block, table_blocks)
-    scratch = _dense_empty((need,), torch.uint8, q.device) if need else None
+    scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev) if need else None
     q_token, q_head, _ = q.stride()
     args = _lib.ATTENTION_KV8_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
                                         seq_lens.data_ptr(), _address(cu_new), out.data_ptr(), _address(lse), _address(scratch), q_token, q_head,
                                         _code("q", q, _HALF_CODE), held, tokens, batch, q_heads, heads, dim, pages, block, table_blocks, window, need,
                                         dim ** -0.5 if scale is None else scale)
-    rc = _lib.load().ib200_attention_kv8(args, _stream())
+    rc = _lib.load().ib200_attention_kv8(args, _stream_of(index))
     if rc:
         _check(rc, "attention_kv8")
     return (out, lse) if return_lse else out
