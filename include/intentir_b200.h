@@ -363,7 +363,7 @@ typedef struct ib200_attention_kv8_args {
 } ib200_attention_kv8_args;
 IB200_API int ib200_attention_kv8(const ib200_attention_kv8_args* args, void* stream);
 IB200_API size_t ib200_attention_kv8_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block,
-                                         int64_t table_blocks);
+                                         int64_t table_blocks, int uniform /* whether cu is NULL */);
 
 #ifdef __cplusplus
 }

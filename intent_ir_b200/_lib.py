@@ -76,7 +76,7 @@ SIGNATURES = {
     "ib200_w4_scratch_bytes": (_sz, [_i, _i64, _i64, _i64, _i64]),
     "ib200_kv8_append": (_i, [_cp, _vp]),
     "ib200_attention_kv8": (_i, [_cp, _vp]),
-    "ib200_attention_kv8_scratch_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "ib200_attention_kv8_scratch_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i]),
 }
 
 # the argument structs of the serving entries (every field 8 bytes: pointers, int64, double), in the header's order; a bytes

@@ -188,8 +188,8 @@ int ib200_attention_kv8(const ib200_attention_kv8_args* a, void* stream) {
   });
 }
 size_t ib200_attention_kv8_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block,
-                                         int64_t table_blocks) {
-  return kv8_attention_scratch_bytes(tokens, batch, q_heads, heads, dim, block, table_blocks);
+                                         int64_t table_blocks, int uniform) {
+  return kv8_attention_scratch_bytes(tokens, batch, q_heads, heads, dim, block, table_blocks, uniform != 0);
 }
 
 }  // extern "C"

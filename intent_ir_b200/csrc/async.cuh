@@ -53,4 +53,21 @@ __device__ __forceinline__ void remote_store_signal(uint32_t remote_addr, float 
                ::"r"(remote_addr), "r"(__float_as_uint(value)), "r"(remote_bar) : "memory");
 }
 
+// all threads of all CTAs of the cluster; what was written to shared memory before is there after it
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// `local` (a shared-memory object of this CTA) as it is in CTA `rank` of the cluster
+__device__ __forceinline__ float cluster_read(const float* local, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_map(local, (uint32_t)rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_read4(const float* local, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_map(local, (uint32_t)rank)) : "memory");
+  return v;
+}
+
 }  // namespace ib200

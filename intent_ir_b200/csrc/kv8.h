@@ -33,6 +33,6 @@ int check_kv8(const char* what, int64_t pages, int64_t heads, int64_t block, int
               int dtype, const int* cu);
 int launch_kv8_append(Kv8Append& a, int dtype, int held, cudaStream_t s);
 int launch_kv8_attention(Kv8Attention& a, int dtype, int held, void* scratch, size_t scratch_bytes, cudaStream_t s);
-size_t kv8_attention_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block, int64_t table_blocks);
+size_t kv8_attention_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block, int64_t table_blocks, bool uniform);
 
 }  // namespace ib200

@@ -6,15 +6,19 @@
 // its keys in tiles of 128.  All tiles of all units, in order, are cut into one equal range per CTA whatever the lengths are (each
 // CTA adds up the lengths itself), so a batch of mixed lengths fills the GPU evenly.  A unit that lies in one range is
 // finished there; the pieces of others go to scratch as (sum, maximum, unnormalised o), and a second launch joins them in order.
+// Where the units and the table are small enough that a cluster of CTAs can take each unit (CLUSTER), its pieces are joined through
+// distributed shared memory instead: one launch, no scratch.
 //
 // Inside a CTA the four warps take 32 keys each of a tile, with copies of their own two stages deep (cp.async) and no
 // barrier between them until the unit ends.  Both products run on mma.sync with the keys as the 16 rows: S' = K Q' and
 // O' = V' P', so that 8 queries fill a fragment where queries as rows would need 16.  Bytes are widened to f16, which
 // is exact for both types; scales are applied to the scores and to p.  q is scaled by a power of two to below 2 (exact), p * vs
 // by another one to below 2^15, so that f16 holds them to 2^-12 over 2^39.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
+#include "async.cuh"
 #include "kv8.cuh"
 
 namespace ib200 {
@@ -76,6 +80,7 @@ __device__ __forceinline__ int first_key(const Kv8Attention& a, int pos) {  // t
 }
 struct Divisors {
   FastDiv group, block;
+  int split, units_per_head;  // CLUSTER: CTAs to a unit; units of every sequence and head
 };
 __device__ __forceinline__ Seq seq_of(const Kv8Attention& a, int group, int b, int rows) {
   Seq s;
@@ -111,7 +116,7 @@ template <typename V> __device__ __forceinline__ V scan_warp(V v, int lane) {  /
   return v;
 }
 
-template <typename T, int HELD, int D, int NT>
+template <typename T, int HELD, int D, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kCtas - 1) attention_kernel(const Kv8Attention a, const Scratch sc, const Divisors by, const int q_vec) {
   using C = Cfg<D>;
   constexpr int ROWS = 8 * NT, HALVES = D / 64, MT = D / 16, CH = D / 16;  // CH: 16-byte chunks of a token
@@ -120,13 +125,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t sums[kWarps], found_before;
   __shared__ int found;
-  __shared__ float stat[kWarps][ROWS][2], top_v[kWarps];
+  __shared__ float stat[kWarps][ROWS][2], top_v[kWarps], joined[ROWS][2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int batch = (int)a.batch, group = (int)by.group.d;
 
   // ---- this CTA's range of tiles -------------------------------------------------------------------
+  int64_t total = 0, w = 0, w_end = 1, front = 0;
+  int b = 0;
+  if constexpr (CLUSTER) {
+    b = (int)(blockIdx.x / by.split) / ((int)a.heads * by.units_per_head);
+  } else {
+  w_end = 0;
   if (threadIdx.x == 0) found = -1;
-  int64_t total = 0, w = 0, w_end = 0;
   auto range = [&] {
     const int ctas = (int)min((int64_t)gridDim.x, total);  // with less work than CTAs, one tile to each
     if (blockIdx.x < ctas) {
@@ -152,42 +162,61 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
     const int64_t upto = scan_warp(v, lane);
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    int64_t front = before;
-    for (int i = 0; i < warp; ++i) front += sums[i];
-    front += upto - v;  // the work in front of sequence b
+    int64_t upfront = before;
+    for (int i = 0; i < warp; ++i) upfront += sums[i];
+    upfront += upto - v;  // the work in front of sequence b
     before += sums[0] + sums[1] + sums[2] + sums[3];
     if (batch <= kThreads) {
       total = before;
       range();
     }
-    if (blockIdx.x == 0 && b < batch) sc.before[b] = front;
-    if (v > 0 && front <= w && w < front + v) {
+    if (blockIdx.x == 0 && b < batch) sc.before[b] = upfront;
+    if (v > 0 && upfront <= w && w < upfront + v) {
       found = b;
-      found_before = front;
+      found_before = upfront;
     }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) sc.before[batch] = total;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the joining launch may line up: it waits for this one's end
   __syncthreads();
   if (w >= w_end) return;
+  b = found;
+  front = found_before;
+  }
 
   uint8_t* stages = smem + warp * kStages * C::kStageBytes;
   const uint32_t stages_at = (uint32_t)__cvta_generic_to_shared(stages);
-  int b = found;
-  int64_t front = found_before;
   Seq s = seq_of(a, group, b, ROWS);
   const int64_t w_start = w;
 
   while (w < w_end) {
     // ---- a piece: one unit's tiles [from, to) -------------------------------------------------------
     // a unit's work is kStart for beginning it, then its tiles; a piece without tiles is nothing
-    const int64_t rel = w - front, unit64 = rel >> 32 ? rel / s.unit_work : (int64_t)((unsigned)rel / (unsigned)s.unit_work), in = rel - unit64 * s.unit_work, piece_start = w;
-    const int unit = (int)unit64, from = (int)max((int64_t)0, in - kStart), to = (int)min((int64_t)s.tiles, in + (w_end - w) - kStart);
-    w = min(w_end, front + (unit64 + 1) * s.unit_work);
-    if (to > from) {
-    const int head = s.units_per_head == 1 ? unit : unit / s.units_per_head, r0 = (unit - head * s.units_per_head) * ROWS;
-    const int rows = (int)min((int64_t)ROWS, (int64_t)s.n * group - r0);
-    const int start = s.len - s.n;  // place of the first new token (negative: fewer tokens than new ones)
+    int head, r0, from, to, rows, start;  // start: place of the first new token (negative: fewer tokens than new ones)
+    const int64_t piece_start = w;
+    if constexpr (CLUSTER) {
+      const int unit = (int)(blockIdx.x / by.split) - b * (int)a.heads * by.units_per_head, rank = blockIdx.x % by.split;
+      head = unit / by.units_per_head;
+      r0 = (unit - head * by.units_per_head) * ROWS;
+      from = (int)((int64_t)s.tiles * rank / by.split);
+      to = (int)((int64_t)s.tiles * (rank + 1) / by.split);
+      rows = min(ROWS, a.each * group - r0);
+      start = max(a.lens[b], -1) - a.each;  // (s counts nothing for a sequence without tokens, whose rows are written all the same)
+      w = w_end;
+    } else {
+      const int64_t rel = w - front, unit64 = rel >> 32 ? rel / s.unit_work : (int64_t)((unsigned)rel / (unsigned)s.unit_work), in = rel - unit64 * s.unit_work;
+      const int unit = (int)unit64;
+      from = (int)max((int64_t)0, in - kStart);
+      to = (int)min((int64_t)s.tiles, in + (w_end - w) - kStart);
+      w = min(w_end, front + (unit64 + 1) * s.unit_work);
+      if (to > from) {
+        head = s.units_per_head == 1 ? unit : unit / s.units_per_head;
+        r0 = (unit - head * s.units_per_head) * ROWS;
+        rows = (int)min((int64_t)ROWS, (int64_t)s.n * group - r0);
+        start = s.len - s.n;
+      }
+    }
+    if (CLUSTER || to > from) {
     const int pos_min = start + (int)by.group.div(r0), pos_max = start + (int)by.group.div(r0 + rows - 1);
     const int lo_min = first_key(a, pos_min), lo_max = first_key(a, pos_max);
     // this warp's steps: 32 keys from 128 * tile + 32 * warp, those with a key that any row sees
@@ -524,7 +553,18 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
     if (lane == 0) top_v[warp] = vtop;
     __syncthreads();
     const bool whole = from == 0 && to == s.tiles;
-    float* part = sc.part + ((int64_t)blockIdx.x * 2 + (piece_start == w_start ? 0 : 1)) * (ROWS * (D + 2));
+    float* part = CLUSTER ? nullptr : sc.part + ((int64_t)blockIdx.x * 2 + (piece_start == w_start ? 0 : 1)) * (ROWS * (D + 2));
+    float* joint = box + kWarps * ROWS * C::kPitch;  // CLUSTER: this CTA's piece
+    auto write = [&](int row, int d, float mm, float sum, float (&v)[4]) {
+      const int i = (int)by.group.div(r0 + row);
+      const int64_t out = (int64_t)(s.first + i) * a.q_heads + head * group + (r0 + row - i * group);
+      const bool empty = start + i < 0;
+      if (start + i >= s.keys) sum = NAN;  // its own key is outside the table
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = empty ? 0.0f : v[e] / sum;
+      store4(static_cast<T*>(a.o) + out * D + d, v);
+      if (a.lse && d == 0) a.lse[out] = empty ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
+    };
     for (int idx = threadIdx.x; idx < ROWS * (D / 4); idx += kThreads) {
       const int row = idx / (D / 4), d = idx % (D / 4) * 4;
       if (row >= rows) break;
@@ -539,15 +579,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
         const float fv = f * (top_v[i] * 0x1p-14f);
         v[0] += x.x * fv, v[1] += x.y * fv, v[2] += x.z * fv, v[3] += x.w * fv;
       }
-      if (whole) {
-        const int i = (int)by.group.div(r0 + row);
-        const int64_t out = (int64_t)(s.first + i) * a.q_heads + head * group + (r0 + row - i * group);
-        const bool empty = start + i < 0;
-        if (start + i >= s.keys) sum = NAN;  // its own key is outside the table
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = empty ? 0.0f : v[e] / sum;
-        store4(static_cast<T*>(a.o) + out * D + d, v);
-        if (a.lse && d == 0) a.lse[out] = empty ? -INFINITY : (mm + log2f(sum)) * 0.6931471805599453f;
+      if constexpr (CLUSTER) {
+        *reinterpret_cast<float4*>(joint + row * C::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
+        if (d == 0) joined[row][0] = mm, joined[row][1] = sum;
+      } else if (whole) {
+        write(row, d, mm, sum, v);
       } else {
         *reinterpret_cast<float4*>(part + row * D + d) = make_float4(v[0], v[1], v[2], v[3]);
         if (d == 0) {
@@ -555,6 +591,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
           part[ROWS * D + ROWS + row] = sum;
         }
       }
+    }
+    if constexpr (CLUSTER) {
+      cluster_sync();
+      for (int idx = (int)(blockIdx.x % by.split) * kThreads + threadIdx.x; idx < rows * (D / 4); idx += by.split * kThreads) {
+        const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+        float mm = -INFINITY, sum = 0.0f, v[4] = {0, 0, 0, 0};
+        for (int r = 0; r < by.split; ++r) mm = fmaxf(mm, cluster_read(&joined[row][0], r));
+        const float base = mm == -INFINITY ? 0.0f : mm;
+        for (int r = 0; r < by.split; ++r) {
+          const float f = exp2_fast(cluster_read(&joined[row][0], r) - base);
+          sum += cluster_read(&joined[row][1], r) * f;
+          const float4 x = cluster_read4(joint + row * C::kPitch + d, r);
+          v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
+        }
+        write(row, d, mm, sum, v);
+      }
+      cluster_sync();  // nobody leaves while its piece is read
+      return;
     }
     __syncthreads();  // the next piece copies over the box
     }
@@ -648,8 +702,20 @@ int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int
   return units > most || units * tiles > most ? most : units * tiles;
 }
 
-template <typename T, int HELD, int D, int NT> int run_attention(const Kv8Attention& a, int grid, void* scratch, cudaStream_t s) {
-  auto* kern = attention_kernel<T, HELD, D, NT>;
+// CTAs of a cluster that takes a unit, 0 where the general form is to be used.  Its CTAs must all run at once and have at most four tiles each, by the
+// room in the table: 1 sequence of 701 tokens, 8 key heads, 9.0 -> 7.1 us on the device and a launch less (see run_attention); longer or more
+// sequences gain from the even split of their tiles.
+int cluster_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, int nt, bool uniform) {
+  if (!uniform) return 0;
+  const int64_t units = batch * heads * ((tokens / batch * group + 8 * nt - 1) / (8 * nt)), tiles = (table_blocks * block + kTile - 1) / kTile;
+  const int64_t most = (int64_t)kSmCount * ((dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas) - (nt > 1));
+  if (units <= 0 || units > most) return 0;
+  const int64_t split = std::min<int64_t>(8, std::max<int64_t>(1, std::min(tiles, most / units)));
+  return tiles <= 4 * split ? (int)split : 0;
+}
+
+template <typename T, int HELD, int D, int NT, bool CLUSTER> int run_attention(const Kv8Attention& a, int grid, int split, void* scratch, cudaStream_t s) {
+  auto* kern = attention_kernel<T, HELD, D, NT, CLUSTER>;
   static std::atomic<uint64_t> ready{0};  // devices that have been told of the shared memory
   int dev = 0;
   IB200_CUDA_OK(cudaGetDevice(&dev));
@@ -659,38 +725,51 @@ template <typename T, int HELD, int D, int NT> int run_attention(const Kv8Attent
   }
   const Scratch sc = carve(scratch, a.batch);
   const int q_vec = (reinterpret_cast<uintptr_t>(a.q) & 7) == 0 && a.q_token % 4 == 0 && a.q_head % 4 == 0;
-  const Divisors by{FastDiv((uint32_t)(a.q_heads / a.heads)), FastDiv((uint32_t)a.block)};
+  const int per_head = (int)(((int64_t)a.each * (a.q_heads / a.heads) + 8 * NT - 1) / (8 * NT));
+  const Divisors by{FastDiv((uint32_t)(a.q_heads / a.heads)), FastDiv((uint32_t)a.block), split, per_head};
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if constexpr (CLUSTER) {
+    cfg.gridDim = dim3((unsigned)(a.batch * a.heads * per_head * split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<D>::kSmem;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, a, sc, by, q_vec));
+    return IB200_OK;
+  }
   kern<<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, by, q_vec);
   if (cudaPeekAtLastError() != cudaSuccess) return cuda_fail(cudaGetLastError(), "attention_kv8 launch");
   // few rows have many pieces each: a CTA for a row; many rows have few: a warp
   const int64_t rows = a.tokens * a.q_heads;
   const bool many = rows > 4 * kSmCount;
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(many ? (rows + 3) / 4 : rows));
   cfg.blockDim = dim3(kJoin);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   IB200_CUDA_OK(cudaLaunchKernelEx(&cfg, many ? join_kernel<T, D, NT, 1> : join_kernel<T, D, NT, 4>, a, sc, by, grid));
   return IB200_OK;
 }
-template <typename T, int HELD, int D> int run_nt(const Kv8Attention& a, int nt, int grid, void* scratch, cudaStream_t s) {
-  return nt == 1 ? run_attention<T, HELD, D, 1>(a, grid, scratch, s) : run_attention<T, HELD, D, 2>(a, grid, scratch, s);
+template <typename T, int HELD, int D> int run_nt(const Kv8Attention& a, int nt, int grid, int split, void* scratch, cudaStream_t s) {
+  if (split) return nt == 1 ? run_attention<T, HELD, D, 1, true>(a, grid, split, scratch, s) : run_attention<T, HELD, D, 2, true>(a, grid, split, scratch, s);
+  return nt == 1 ? run_attention<T, HELD, D, 1, false>(a, grid, split, scratch, s) : run_attention<T, HELD, D, 2, false>(a, grid, split, scratch, s);
 }
-template <typename T, int HELD> int run_dim(const Kv8Attention& a, int nt, int grid, void* scratch, cudaStream_t s) {
-  return a.dim == 128 ? run_nt<T, HELD, 128>(a, nt, grid, scratch, s) : run_nt<T, HELD, 64>(a, nt, grid, scratch, s);
+template <typename T, int HELD> int run_dim(const Kv8Attention& a, int nt, int grid, int split, void* scratch, cudaStream_t s) {
+  return a.dim == 128 ? run_nt<T, HELD, 128>(a, nt, grid, split, scratch, s) : run_nt<T, HELD, 64>(a, nt, grid, split, scratch, s);
 }
 
 }  // namespace
 
-size_t kv8_attention_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block, int64_t table_blocks) {
+size_t kv8_attention_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t heads, int64_t dim, int64_t block, int64_t table_blocks, bool uniform) {
   if (tokens <= 0 || batch <= 0 || heads <= 0 || q_heads < heads || (dim != 64 && dim != 128) || block <= 0 || table_blocks < 0 || batch > INT32_MAX ||
       tokens > INT32_MAX || q_heads > 65535 || beyond_any_device(table_blocks, block))
     return 0;  // the launch refuses these, or does nothing
   const int nt = tiles_of_rows(tokens, batch, q_heads / heads);
+  if (cluster_of(tokens, batch, heads, q_heads / heads, dim, block, table_blocks, nt, uniform)) return 0;
   return prefix_bytes(batch) + (size_t)grid_of(tokens, batch, heads, q_heads / heads, dim, block, table_blocks, nt) * 2 * 8 * nt * (dim + 2) * 4;
 }
 
@@ -705,15 +784,17 @@ int launch_kv8_attention(Kv8Attention& a, int dtype, int held, void* scratch, si
   if (!aligned16(a.k_cache) || !aligned16(a.v_cache)) return fail(IB200_ERR_INVALID, "attention_kv8: caches must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(a.o) & 7) return fail(IB200_ERR_INVALID, "attention_kv8: o must be 8-byte aligned");
   if (a.tokens * a.q_heads >= INT32_MAX || beyond_any_device(a.tokens, a.q_heads, a.dim)) return fail(IB200_ERR_UNSUPPORTED, "attention_kv8: too many rows");
-  if (!scratch || scratch_bytes < kv8_attention_scratch_bytes(a.tokens, a.batch, a.q_heads, a.heads, a.dim, a.block, a.table_blocks))
-    return fail(IB200_ERR_BUFFER, "attention_kv8: scratch is smaller than ib200_attention_kv8_scratch_bytes");
-  if (a.pages == 0) a.k_cache = a.v_cache = static_cast<const uint8_t*>(scratch);  // an address for copies that take nothing
+  const size_t need = kv8_attention_scratch_bytes(a.tokens, a.batch, a.q_heads, a.heads, a.dim, a.block, a.table_blocks, !a.cu);
+  if (need && (!scratch || scratch_bytes < need)) return fail(IB200_ERR_BUFFER, "attention_kv8: scratch is smaller than ib200_attention_kv8_scratch_bytes");
+  // a cache without pages is never read, but copies that take nothing want an aligned address all the same
+  if (a.pages == 0) a.k_cache = a.v_cache = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.lens) & ~(uintptr_t)15);
   a.each = (int)(a.tokens / a.batch);
   const int64_t group = a.q_heads / a.heads;
-  const int nt = tiles_of_rows(a.tokens, a.batch, group), grid = (int)grid_of(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, nt);
+  const int nt = tiles_of_rows(a.tokens, a.batch, group), split = cluster_of(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, nt, !a.cu);
+  const int grid = (int)grid_of(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, nt);
   if (dtype == IB200_BF16)
-    return held == IB200_E4M3 ? run_dim<__nv_bfloat16, HELD_E4M3>(a, nt, grid, scratch, s) : run_dim<__nv_bfloat16, HELD_I8>(a, nt, grid, scratch, s);
-  return held == IB200_E4M3 ? run_dim<__half, HELD_E4M3>(a, nt, grid, scratch, s) : run_dim<__half, HELD_I8>(a, nt, grid, scratch, s);
+    return held == IB200_E4M3 ? run_dim<__nv_bfloat16, HELD_E4M3>(a, nt, grid, split, scratch, s) : run_dim<__nv_bfloat16, HELD_I8>(a, nt, grid, split, scratch, s);
+  return held == IB200_E4M3 ? run_dim<__half, HELD_E4M3>(a, nt, grid, split, scratch, s) : run_dim<__half, HELD_I8>(a, nt, grid, split, scratch, s);
 }
 
 }  // namespace ib200

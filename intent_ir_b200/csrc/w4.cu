@@ -29,14 +29,6 @@ struct W4Args {
   int32_t* status;
 };
 
-__device__ __forceinline__ void cluster_arrive_wait() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float cluster_read(const float* local, int rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_map(local, (uint32_t)rank)) : "memory");
-  return v;
-}
 __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
   if (type == IB200_F32) return static_cast<const float*>(p)[i];
   if (type == IB200_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
@@ -393,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 4; ++c) box[wk * BOX + (nt * 8 + 2 * t + (c & 1)) * kRows + wr * 32 + mt * 16 + pg + 8 * (c >> 1)] = sum[mt][nt][c];
-  if (split > 1) cluster_arrive_wait(); else __syncthreads();
+  if (split > 1) cluster_sync(); else __syncthreads();
   const int rows = min(NT * 8, a.m - m0);
   for (int idx = rank * kThreads + threadIdx.x; idx < rows * kRows; idx += split * kThreads) {
     const int m = m0 + idx / kRows, n = n0 + idx % kRows;
@@ -402,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
       v += split > 1 ? cluster_read(box + idx, r) + cluster_read(box + BOX + idx, r) : box[idx] + box[BOX + idx];
     write_y(a, m, n, v);
   }
-  if (split > 1) cluster_arrive_wait();  // nobody leaves while its sums are read
+  if (split > 1) cluster_sync();  // nobody leaves while its sums are read
 }
 
 // K is split over a cluster so that the CTAs that run at once (clusters stay within a GPC, so larger ones fill the GPU less) have as
@@ -778,7 +770,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
 #pragma unroll
     for (int j = 0; j < COLS; ++j) box[((warp >> 3) * COLS + j) * kTcRows + threadIdx.x % kTcRows] = sum[j];
   }
-  if (split > 1) cluster_arrive_wait(); else __syncthreads();
+  if (split > 1) cluster_sync(); else __syncthreads();
   const int rows = min(NX, a.m - m0);
   for (int idx = rank * kTcThreads + threadIdx.x; idx < rows * kTcRows; idx += split * kTcThreads) {
     const int m = m0 + idx / kTcRows, n = n0 + idx % kTcRows;
@@ -786,7 +778,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
     for (int r = 0; r < split; ++r) v += split > 1 ? cluster_read(box + idx, r) : box[idx];
     write_y(a, m, n, v);
   }
-  if (split > 1) cluster_arrive_wait();
+  if (split > 1) cluster_sync();
 }
 
 int64_t padded(int64_t v, int64_t to) { return (v + to - 1) / to * to; }

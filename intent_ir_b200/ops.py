@@ -531,7 +531,7 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         _dense("out", out, shape, q.dtype)
     dev = q.device
     lse = torch.empty_strided((tokens, q_heads), (q_heads, 1), dtype=torch.float32, device=dev) if return_lse else None
-    need = _attention_scratch(tokens, batch, q_heads, heads, dim, block, table_blocks)
+    need = _attention_scratch(tokens, batch, q_heads, heads, dim, block, table_blocks, cu_new is None)
     scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev) if need else None
     q_token, q_head, _ = q.stride()
     args = _lib.ATTENTION_KV8_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),

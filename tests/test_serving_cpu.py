@@ -73,8 +73,13 @@ def test_what_the_kernels_do_not_cover_is_unsupported(call, bad):
 
 
 def test_scratch_that_is_too_small_is_refused_and_no_arguments_are_invalid():
-    need = _lib.load().ib200_attention_kv8_scratch_bytes(4, 2, 4, 2, 64, 16, 4)
-    assert need > 0 and _attention(bytes=need - 1) == _lib.ERR_BUFFER and _attention(scratch=None) == _lib.ERR_BUFFER
+    size = _lib.load().ib200_attention_kv8_scratch_bytes
+    need = size(4, 2, 4, 2, 64, 16, 4, 0)
+    assert need > 0 and _attention(cu=P, bytes=need - 1) == _lib.ERR_BUFFER and _attention(cu=P, scratch=None) == _lib.ERR_BUFFER
+    assert size(4, 2, 4, 2, 64, 16, 4, 1) == 0 and size(4, 2, 4, 2, 64, 16, 4000, 1) > 0  # short tables: a cluster to a unit, no scratch
+    assert _attention(blocks=4000, bytes=8) == _lib.ERR_BUFFER
+    w4 = _lib.load().ib200_w4_scratch_bytes
+    assert w4(_lib.BF16, 4, 64, 64, 32) == 0 and w4(_lib.BF16, 20, 64, 64, 32) == 32 * 256 * 2 and _w4(m=20, bytes=8) == _lib.ERR_BUFFER
     for entry in ("ib200_rmsnorm", "ib200_w4_matmul", "ib200_kv8_append", "ib200_attention_kv8"):
         assert getattr(_lib.load(), entry)(None, None) == _lib.ERR_INVALID
 
