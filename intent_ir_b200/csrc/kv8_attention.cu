@@ -702,16 +702,16 @@ int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int
   return units > most || units * tiles > most ? most : units * tiles;
 }
 
-// CTAs of a cluster that takes a unit, 0 where the general form is to be used.  Its CTAs must all run at once and have at most four tiles each, by the
-// room in the table: 1 sequence of 701 tokens, 8 key heads, 9.0 -> 7.1 us on the device and a launch less (see run_attention); longer or more
-// sequences gain from the even split of their tiles.
+// CTAs of a cluster that takes a unit, 0 where the general form is to be used.  Its CTAs must all run at once and have at most eight tiles each, by the
+// room in the table.  Device time against the general form's: 1 sequence of 701 tokens 6.9 / 9.0 us, 1 of 8000 13.6 / 15.1, 16 of up to 3000 18.4 / 20.5, 48 of
+// up to 900 17.5 / 21.2, and 4.5 us less to enqueue; with sixteen tiles 2 of 16 000 take 22.4 / 19.2: longer ones gain from the even split of all tiles.
 int cluster_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, int nt, bool uniform) {
   if (!uniform) return 0;
   const int64_t units = batch * heads * ((tokens / batch * group + 8 * nt - 1) / (8 * nt)), tiles = (table_blocks * block + kTile - 1) / kTile;
   const int64_t most = (int64_t)kSmCount * ((dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas) - (nt > 1));
   if (units <= 0 || units > most) return 0;
   const int64_t split = std::min<int64_t>(8, std::max<int64_t>(1, std::min(tiles, most / units)));
-  return tiles <= 4 * split ? (int)split : 0;
+  return tiles <= 8 * split ? (int)split : 0;
 }
 
 template <typename T, int HELD, int D, int NT, bool CLUSTER> int run_attention(const Kv8Attention& a, int grid, int split, void* scratch, cudaStream_t s) {
