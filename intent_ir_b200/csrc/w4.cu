@@ -471,17 +471,17 @@ template <int XK> int run_stream_rows(const W4Args& a, cudaStream_t s) {
 // ---- tensor memory ----------------------------------------------------------------------------------------
 template <int N> __device__ __forceinline__ void tmem_load(uint32_t at, uint32_t (&r)[N]);
 template <> __device__ __forceinline__ void tmem_load<8>(uint32_t at, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(at) : "memory");
 }
 template <> __device__ __forceinline__ void tmem_load<16>(uint32_t at, uint32_t (&r)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n tcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                : "r"(at) : "memory");
 }
 template <> __device__ __forceinline__ void tmem_load<32>(uint32_t at, uint32_t (&r)[32]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                : "r"(at) : "memory");
 }
@@ -686,9 +686,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       uint32_t r[COLS];
       tmem_load<COLS>(d_at + (j % ND) * NX, r);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-      for (int e = 0; e < COLS; ++e) asm volatile("" : "+r"(r[e]));  // (values are there from here on)
       if (xs_many) {
         const float4* f = reinterpret_cast<const float4*>(old_stage + S::XS_AT + (old_group * NX + half * COLS) * 4);
 #pragma unroll
@@ -713,6 +710,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
         block = s * GROUPS >> 3;
         next_block();
       }
+      // the row's bytes of the stage, chunks swizzled by row % 8: both the chunk and the half only flip address bits
+      const uint32_t row_at = (smem_addr(smem) + (uint32_t)((s - s0) % kStages * S::BYTES + row * kRowBytes)) ^ (uint32_t)((row & 7) << 4) ^ (uint32_t)(half * (KS / 2));
       const float* scales_of = reinterpret_cast<const float*>(scales + (block & 1) * 32) + (s * GROUPS & 7);
       const uint8_t* zeros_of = scales + 64 + (block & 1) * 8 + (s * GROUPS & 7);
 #pragma unroll
@@ -722,16 +721,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
         constexpr int WORDS = KS >= 32 ? 4 : 2;  // of q a time
 #pragma unroll
         for (int q = 0; q < KS / (8 * WORDS); ++q) {
-          const int byte = c * (G / 2) + half * (KS / 2) + q * 16;  // of the row
-          const uint8_t* p = st + row * kRowBytes + (((byte >> 4) ^ (row & 7)) << 4) + (byte & 15);
           uint32_t w[4], r[4 * WORDS];
-          if (WORDS == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            w[0] = v.x, w[1] = v.y;
-          }
+          const uint32_t p = row_at ^ (uint32_t)(c * (G / 2) + q * 16);
+          if (WORDS == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(p) : "memory");
+          else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(p) : "memory");
 #pragma unroll
           for (int k = 0; k < WORDS; ++k) {
             uint32_t pairs[4];
