@@ -630,7 +630,10 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const
   if (u >= a.tokens * a.q_heads) return;  // (warps of one row leave together, here and below)
   const int t = (int)(u / a.q_heads), qh = (int)(u - (int64_t)t * a.q_heads), group = (int)by.group.d;
   int b, first, count;
-  if (!find_sequence(a.cu, (int)a.batch, a.each, t, b, first, count)) return;
+  if (!find_sequence(a.cu, (int)a.batch, a.each, t, b, first, count)) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // (this launch ends after the one in front, whatever the offsets say)
+    return;
+  }
   const Seq s = seq_of(a, group, b, ROWS);
   const int64_t pos = (int64_t)a.lens[b] - count + (t - first);
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -255,7 +255,6 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
           }
         }
       }
-      if (!a.x_vec) __threadfence_block();
       if (XK >= X_E4M3 && a.xs_groups > 1) {
         for (int e = lane; e < GROUPS * NT * 8; e += 32) {
           const int m = m0 + e % (NT * 8), grp = s * GROUPS + e / (NT * 8);
@@ -263,8 +262,15 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
           copy4(dst + S::XS_AT + e * 4, a.xs + (take ? (int64_t)m * a.groups + grp : 0), take ? 4 : 0);
         }
       }
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
+      if (a.x_vec) {
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
+      } else {  // x was written by stores, which an arrival of this thread's own releases
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&full[i])) : "memory");
+      }
     }
+    if (dead)  // copies that are still on their way land before the CTA ends
+      for (int s = max(s0, s1 - kStages); s < s1; ++s) (void)mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
   } else {
   // this thread's rows: 32 * wr + pg, + 8, + 16, + 24.  A stage's groups lie in one block.
   const uint8_t* scales = smem + S::S_AT + (wr * 32 + pg) * kRowScales;

@@ -537,7 +537,7 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     args = _lib.ATTENTION_KV8_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_table.data_ptr(),
                                         seq_lens.data_ptr(), _address(cu_new), out.data_ptr(), _address(lse), _address(scratch), q_token, q_head,
                                         _code("q", q, _HALF_CODE), held, tokens, batch, q_heads, heads, dim, pages, block, table_blocks, window, need,
-                                        dim ** -0.5 if scale is None else scale)
+                                        max(dim, 1) ** -0.5 if scale is None else scale)
     rc = _lib.load().ib200_attention_kv8(args, _stream_of(index))
     if rc:
         _check(rc, "attention_kv8")

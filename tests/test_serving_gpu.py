@@ -572,6 +572,15 @@ def test_attention_strides_refusals_and_empty(ops):
         ops.kv8_append(dev["k"][:, :1], dev["v"][:, :1], *args)
 
 
+def test_heads_without_width_are_refused(ops):
+    d = _cuda(_paged(31, [1, 1], [5, 20], 2, 64, 16, BF16, E4M3))
+    caches = [d["k_cache"][..., :0].contiguous(), d["v_cache"][..., :0].contiguous(), d["k_scale"], d["v_scale"], d["block_table"], d["seq_lens"]]
+    with pytest.raises(B200LoweringError):
+        ops.attention_kv8(d["k"][..., :0], *caches)
+    with pytest.raises(B200LoweringError):
+        ops.kv8_append(d["k"][..., :0], d["v"][..., :0], *caches)
+
+
 # ---- a run of them together -------------------------------------------------------------------------
 
 def _layer(ops, s, held, out8):
