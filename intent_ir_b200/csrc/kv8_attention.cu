@@ -2,7 +2,7 @@
 //   o[t, h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * q . k_j - m),   k_j = k8 * ks(page, head),   v_j = v8 * vs(page, head)
 // in one pass over the keys with a running maximum m and sum, in f32.
 //
-// Work.  The queries that share a key head (new tokens x heads of a group) are rows, 8 * NT of them to a unit; a unit reads
+// Work.  The queries that share a key head (new tokens x heads of a group) are rows, 8 * NT of them to a unit (8, 16 or 24); a unit reads
 // its keys in tiles of 128.  All tiles of all units, in order, are cut into one equal range per CTA whatever the lengths are (each
 // CTA adds up the lengths itself), so a batch of mixed lengths fills the GPU evenly.  A unit that lies in one range is
 // finished there; the pieces of others go to scratch as (sum, maximum, unnormalised o), and a second launch joins them in order.
@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
   constexpr int ROWS = 8 * NT, HALVES = D / 64, MT = D / 16, CH = D / 16;  // CH: 16-byte chunks of a token
   // An f16 result is off by 2^-12 of itself, no more than p rounded to f16 once: there p is multiplied in two parts.  (bf16's 2^-9 hides it.)
   constexpr bool kTwice = std::is_same<T, __half>::value;
+  static_assert((kWarps + (CLUSTER ? 1 : 0)) * ROWS * C::kPitch * 4 <= C::kSmem, "the warps' results, and a cluster's piece, where the stages were");
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t sums[kWarps], found_before;
   __shared__ int found;
@@ -692,16 +693,24 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const
   if (a.lse && lane == 0) a.lse[u] = (m + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Rows of a unit, in eights: one where 8 rows suffice, two where a sequence has more (several new tokens, many heads to a group) so
-// that its keys are read half as often; with offsets the average number of new tokens decides.  (Four spill registers at D = 128.)
-int tiles_of_rows(int64_t tokens, int64_t batch, int64_t group) {
-  const int64_t rows = group * ((tokens + batch - 1) / batch);
-  return rows <= 8 ? 1 : 2;
+int64_t most_ctas(int64_t dim, int nt) { return (int64_t)kSmCount * ((dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas) - (nt > 1)); }
+
+// Rows of a unit, in eights: one where 8 rows suffice, two or three where a sequence has more (several new tokens, many heads to a group) so
+// that its keys are read and widened less often.  A unit of three takes 1.36 to 1.6 times a unit of two: 16 x 15 000 keys of 128 for 20 rows (one unit or
+// two) 82 / 102 us, 40 rows (two or three) 137 / 151, chunks of up to 512 tokens 357 / 388, but 33 x up to 8 tokens x 4 heads 36 / 34, and 11.3 / 10.4 us where
+// two sequences of 700 keys leave the GPU room for every tile of twice the units.  With offsets only the average number of new tokens is known here.
+// (Units of three spill up to 39 registers at D = 128 and f16, 7 in bf16.)
+int tiles_of_rows(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, bool uniform) {
+  const int64_t rows = group * ((tokens + batch - 1) / batch), two = (rows + 15) / 16, three = (rows + 23) / 24;
+  if (rows <= 8) return 1;
+  const int64_t units = batch * heads * two, most = most_ctas(dim, 2);
+  if (units <= most && units * ((table_blocks * block + kTile - 1) / kTile) <= most) return 2;
+  return (uniform ? 4 * three <= 3 * two : rows > 48) ? 3 : 2;
 }
 int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, int nt) {
   // no more CTAs than there can be tiles
   const int64_t units = heads * ((tokens * group + 8 * nt - 1) / (8 * nt) + batch), tiles = table_blocks * block / kTile + 2 + kStart;
-  const int64_t most = (int64_t)kSmCount * ((dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas) - (nt > 1));
+  const int64_t most = most_ctas(dim, nt);
   return units > most || units * tiles > most ? most : units * tiles;
 }
 
@@ -711,7 +720,7 @@ int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int
 int cluster_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, int nt, bool uniform) {
   if (!uniform) return 0;
   const int64_t units = batch * heads * ((tokens / batch * group + 8 * nt - 1) / (8 * nt)), tiles = (table_blocks * block + kTile - 1) / kTile;
-  const int64_t most = (int64_t)kSmCount * ((dim == 128 ? Cfg<128>::kCtas : Cfg<64>::kCtas) - (nt > 1));
+  const int64_t most = most_ctas(dim, nt);
   if (units <= 0 || units > most) return 0;
   const int64_t split = std::min<int64_t>(8, std::max<int64_t>(1, std::min(tiles, most / units)));
   return tiles <= 8 * split ? (int)split : 0;
@@ -758,8 +767,9 @@ template <typename T, int HELD, int D, int NT, bool CLUSTER> int run_attention(c
   return IB200_OK;
 }
 template <typename T, int HELD, int D> int run_nt(const Kv8Attention& a, int nt, int grid, int split, void* scratch, cudaStream_t s) {
-  if (split) return nt == 1 ? run_attention<T, HELD, D, 1, true>(a, grid, split, scratch, s) : run_attention<T, HELD, D, 2, true>(a, grid, split, scratch, s);
-  return nt == 1 ? run_attention<T, HELD, D, 1, false>(a, grid, split, scratch, s) : run_attention<T, HELD, D, 2, false>(a, grid, split, scratch, s);
+  if (nt == 1) return split ? run_attention<T, HELD, D, 1, true>(a, grid, split, scratch, s) : run_attention<T, HELD, D, 1, false>(a, grid, split, scratch, s);
+  if (nt == 2) return split ? run_attention<T, HELD, D, 2, true>(a, grid, split, scratch, s) : run_attention<T, HELD, D, 2, false>(a, grid, split, scratch, s);
+  return split ? run_attention<T, HELD, D, 3, true>(a, grid, split, scratch, s) : run_attention<T, HELD, D, 3, false>(a, grid, split, scratch, s);
 }
 template <typename T, int HELD> int run_dim(const Kv8Attention& a, int nt, int grid, int split, void* scratch, cudaStream_t s) {
   return a.dim == 128 ? run_nt<T, HELD, 128>(a, nt, grid, split, scratch, s) : run_nt<T, HELD, 64>(a, nt, grid, split, scratch, s);
@@ -771,7 +781,7 @@ size_t kv8_attention_scratch_bytes(int64_t tokens, int64_t batch, int64_t q_head
   if (tokens <= 0 || batch <= 0 || heads <= 0 || q_heads < heads || (dim != 64 && dim != 128) || block <= 0 || table_blocks < 0 || batch > INT32_MAX ||
       tokens > INT32_MAX || q_heads > 65535 || beyond_any_device(table_blocks, block))
     return 0;  // the launch refuses these, or does nothing
-  const int nt = tiles_of_rows(tokens, batch, q_heads / heads);
+  const int nt = tiles_of_rows(tokens, batch, heads, q_heads / heads, dim, block, table_blocks, uniform);
   if (cluster_of(tokens, batch, heads, q_heads / heads, dim, block, table_blocks, nt, uniform)) return 0;
   return prefix_bytes(batch) + (size_t)grid_of(tokens, batch, heads, q_heads / heads, dim, block, table_blocks, nt) * 2 * 8 * nt * (dim + 2) * 4;
 }
@@ -793,7 +803,7 @@ int launch_kv8_attention(Kv8Attention& a, int dtype, int held, void* scratch, si
   if (a.pages == 0) a.k_cache = a.v_cache = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(a.lens) & ~(uintptr_t)15);
   a.each = (int)(a.tokens / a.batch);
   const int64_t group = a.q_heads / a.heads;
-  const int nt = tiles_of_rows(a.tokens, a.batch, group), split = cluster_of(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, nt, !a.cu);
+  const int nt = tiles_of_rows(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, !a.cu), split = cluster_of(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, nt, !a.cu);
   const int grid = (int)grid_of(a.tokens, a.batch, a.heads, group, a.dim, a.block, a.table_blocks, nt);
   if (dtype == IB200_BF16)
     return held == IB200_E4M3 ? run_dim<__nv_bfloat16, HELD_E4M3>(a, nt, grid, split, scratch, s) : run_dim<__nv_bfloat16, HELD_I8>(a, nt, grid, split, scratch, s);

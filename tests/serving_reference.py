@@ -145,6 +145,6 @@ def attention(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, scale, win
             wrong = size * (dim / 16 + 4) * 2.0**-22 + 2.0**-21  # of a score, in units of 1
             spread = torch.einsum("hgj,jhd->hgd", p, vv.abs())
             bound[t] = (spread * (2.0**-11 + 2.0**-18 + 2 * wrong[..., None])).reshape(-1, dim) + o[t].abs() * half_step(q.dtype)
-            bound[t] += vv.abs().max() * 2.0**-24  # numerators below the 16-bit range, and results below f16's
+            bound[t] += vv.abs().nan_to_num(nan=0.0).max() * 2.0**-24  # numerators below the 16-bit range, and results below f16's; a NaN counts for its own column
             lse_bound[t] = (wrong + 2.0**-20).reshape(-1) + lse[t].abs() * 2.0**-22
     return o, lse, bound, lse_bound

@@ -572,6 +572,22 @@ def test_attention_strides_refusals_and_empty(ops):
         ops.kv8_append(dev["k"][:, :1], dev["v"][:, :1], *args)
 
 
+@pytest.mark.parametrize("held", [E4M3, I8])
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (64, BF16), (128, F16), (128, BF16)])
+def test_attention_units_of_twenty_four_rows(ops, held, dim, dtype):
+    """Taken where a table has room for more tiles than the GPU takes at once: a cluster to a unit, the even split, ragged sequences."""
+    for room, window in ((400, 0), (1200, 0), (1200, 100)):
+        d = _paged(60, [5, 5, 5], [700, 3, 131], 2, dim, 16, dtype, held, table_blocks=room)
+        if held == E4M3:  # the last new token's value is NaN: only its own rows see it
+            page, slot = int(d["block_table"][0, 699 // 16]), 699 % 16
+            d["v_cache"].view(torch.uint8)[page, 1, slot, 3] = 0x7F
+        _check_attention(ops, d, 8, uniform=True, window=window)  # 20 rows
+        _check_attention(ops, d, 16, uniform=True, window=window)  # 40 rows: the second unit has 16
+    d = _paged(61, [20, 9, 14, 1], [600, 9, 3, 77], 2, dim, 16, dtype, held, table_blocks=600)
+    _check_attention(ops, d, 10)  # 100 rows, 45, 70, 5
+    _check_attention(ops, d, 10, window=33)
+
+
 def test_heads_without_width_are_refused(ops):
     d = _cuda(_paged(31, [1, 1], [5, 20], 2, 64, 16, BF16, E4M3))
     caches = [d["k_cache"][..., :0].contiguous(), d["v_cache"][..., :0].contiguous(), d["k_scale"], d["v_scale"], d["block_table"], d["seq_lens"]]
