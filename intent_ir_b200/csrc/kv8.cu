@@ -179,7 +179,8 @@ template <typename T, int HELD, int D> int run_append(const Kv8Append& a, cudaSt
   const int64_t units = a.cu ? a.tokens / a.block + 2 * a.batch + 1 : a.batch * a.per;
   if (units > INT32_MAX) return fail(IB200_ERR_UNSUPPORTED, "kv8_append: too many blocks");
   const int vec = aligned16(a.k) && aligned16(a.v) && a.k_token % 8 == 0 && a.k_head % 8 == 0 && a.v_token % 8 == 0 && a.v_head % 8 == 0;
-  // a warp holds 16 tokens of 128 in its registers; where a block takes more, a CTA
+  // a warp holds 16 tokens of 128 in its registers; where a block takes more, a CTA.  128 sequences x 1 token 3.4 / 8.1 us by a warp / a CTA, x 8 6.0 / 9.3,
+  // x 16 9.2 / 10.9, x 32 16.6 / 13.1, blocks of 64 filled by long sequences 127 / 46
   const int64_t expect = (a.tokens + a.batch - 1) / a.batch;
   if ((expect < a.block ? expect : a.block) * D <= 16 * 128) append_kernel<T, HELD, D, 32><<<dim3((unsigned)units, (unsigned)a.heads, 2), 32, 0, s>>>(a, vec);
   else append_kernel<T, HELD, D, 256><<<dim3((unsigned)units, (unsigned)a.heads), 256, 0, s>>>(a, vec);

@@ -14,6 +14,11 @@
 // O' = V' P', so that 8 queries fill a fragment where queries as rows would need 16.  Bytes are widened to f16, which
 // is exact for both types; scales are applied to the scores and to p.  q is scaled by a power of two to below 2 (exact), p * vs
 // by another one to below 2^15, so that f16 holds them to 2^-12 over 2^39.
+//
+// With 8 rows to a unit HBM bounds it: 64 sequences of up to 8193 keys, 32 / 8 heads of 128, e4m3, 93 us (5.8 TB/s, 0.89 of a copy's rate); 2 of 131 073 keys,
+// 64 / 8 heads, 69 us (5.4 TB/s).  With more rows the instructions around the products do (39 to 45 % of the issue slots, the rest waits on their chains): 16 x 5
+// new tokens over 15 000 keys 82 us (3.3 TB/s, 133 TFLOP/s).  Short work is a chain of latencies: 702 keys 7.0 us, 33 x up to 5 new tokens in a window of 2048 20.6 us.
+// A third stage of copies changed nothing at a width of 64 (20.8 / 20.7 us; 64 sequences 58.0 / 55.9).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -756,7 +761,8 @@ template <typename T, int HELD, int D, int NT, bool CLUSTER> int run_attention(c
   }
   kern<<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, by, q_vec);
   if (cudaPeekAtLastError() != cudaSuccess) return cuda_fail(cudaGetLastError(), "attention_kv8 launch");
-  // few rows have many pieces each: a CTA for a row; many rows have few: a warp
+  // few rows have many pieces each: a CTA for a row (2 sequences of 131 073 keys: 69.2 us in all, 73.5 with a warp); many rows have few: a warp (64 of up to
+  // 8193: 93.2, 94.4 with a CTA)
   const int64_t rows = a.tokens * a.q_heads;
   const bool many = rows > 4 * kSmCount;
   cfg.gridDim = dim3((unsigned)(many ? (rows + 3) / 4 : rows));

@@ -69,6 +69,9 @@ __device__ __forceinline__ float inverse_fast(int type, float top) {
 // or 8 * THREADS apart (16-byte accesses).  Rows that do not begin on 16-byte boundaries are read element by
 // element; a warp then has 256 * NV adjacent columns, lane by lane (coalesced).  Either way the columns that share a scale
 // lie in one warp.
+// bf16 16384 x 8192 + residual -> e4m3 with scales of 128: 154 us (6.1 TB/s, 0.93 of a copy's rate); three passes over the row took 254, and divisions
+// instead of the approximate reciprocal for the scales of groups 180, bound by instruction issue.  f32 1021 x 5001, where no row is aligned:
+// 15.4 us (5.3 TB/s) lane by lane, 46.6 with eight adjacent columns to a thread.  16 x 4096: 3.0 us, one chain of load, two reductions and store.
 template <typename T> struct Raw { uint4 v[sizeof(T) / 2]; };  // 8 elements as they lie in memory
 template <typename T> __device__ __forceinline__ Raw<T> read8(const T* p) {
   Raw<T> r;
@@ -363,9 +366,18 @@ template <typename T, bool HELD, int THREADS, int NV> int run_resident(const Rms
   else rmsnorm_resident<T, HELD, THREADS, NV, false><<<grid, threads, 0, s>>>(a);
   return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "rmsnorm launch");
 }
+// Threads of a row: many rows want few, with the work of a thread in flight, few rows all that help.  bf16 + residual -> e4m3 with scales of 128, a warp or fewer threads
+// against 256: 65 536 x 256 24.7 / 142 us (52 with registers for 1024), 16 384 x 1024 23.0 / 42.4, 16 384 x 1536 32.8 / 46.9, 16 384 x 2560 60.6 / 70.5; 592 x 1024 3.9 / 2.9,
+// 16 x 2048 4.0 / 2.7, 600 x 4096 5.7 / 5.1 (and 1500 x 1024 4.8 / 5.4).  4096 x 16 384 in registers 89 us, streamed 140.
 template <typename T, bool HELD> int run_rms(const RmsArgs& a, bool vec, cudaStream_t s) {
+  const bool many = a.rows > 4 * kSmCount;
   if (a.rows <= INT32_MAX) {
-    if (a.cols <= 1024) return run_resident<T, HELD, 32, 4>(a, vec, s);
+    if (many && a.cols <= 4096) {
+      if (a.cols <= 256) return run_resident<T, HELD, 32, 1>(a, vec, s);
+      if (a.cols <= 512) return run_resident<T, HELD, 32, 2>(a, vec, s);
+      if (a.cols <= 1024) return run_resident<T, HELD, 32, 4>(a, vec, s);
+      return a.cols <= 2048 ? run_resident<T, HELD, 64, 4>(a, vec, s) : run_resident<T, HELD, 128, 4>(a, vec, s);
+    }
     if (a.cols <= 2048) return run_resident<T, HELD, 256, 1>(a, vec, s);
     if (a.cols <= 4096) return run_resident<T, HELD, 256, 2>(a, vec, s);
     if (a.cols <= 8192) return run_resident<T, HELD, 256, 4>(a, vec, s);

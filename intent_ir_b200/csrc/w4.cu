@@ -43,7 +43,10 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
 // the G / 4 adjacent k from t * G / 4, one 32-bit word of q (8 k) per two products, which keeps every product inside one
 // group; the group's sum is then scaled in f32.  A word gives pairs (0, 4), (1, 5), (2, 6), (3, 7), so x is laid down in that order, in
 // the order in which the warps read it.  128 + q in bf16 (1024 + q in f16) is q under the exponent of 128 (1024); minus 128 + z it is exact.
-// A ninth warp brings everything: the weights as said, x, scales and zero points by cp.async; it and the others meet at mbarriers only.
+// A ninth warp brings the weights and x as said; it and the others meet at mbarriers only.  The scales are read by the threads that use them.
+// 8192 x 8192 of groups of 128 and one row of bf16: 16.4 us (2.1 TB/s); 4096 x 4096: 6.6 us, of which two stages of loads and the cluster's sum are most; 7 x 5003 x 8192 in
+// groups of 32 with zero points, f16: 15.0 us.  Instruction issue and the waits between stages bound it, not HBM: eight weights cost nine instructions in front
+// of their products.  A ring filled by all warps took 24 us for the last, one warp to an output 161.
 constexpr int kRows = 128, kThreads = 288, kStageK = 256, kRowBytes = kStageK / 2;
 enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
 constexpr int kRowScales = 144;  // a row's two blocks of eight scales, then of eight zero points' patterns; 16 bytes keep rows in different banks
@@ -518,6 +521,8 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t at) {
 //   warp 16     brings the operands; x comes permuted and widened by a small launch in front, on which only x's copies wait
 //   warps 17-18 one thread each issues the MMAs of a block
 // Chunk i's widened weights arriving says that chunk i - 2 has been read back, so its buffers need no barrier of their own.
+// 64 x 16384 x 8192, e4m3, groups of 128: 34.8 us (494 TFLOP/s; the weights' bytes alone 11 us).  Issue of the widening's instructions bounds it (55 % of the slots; the tensor
+// cores are busy 15 % of the time).  On mma.sync the same product took 110 us; with eight widening warps 43, with scales fetched when they were needed 58.
 constexpr int kTcRowScales = 84;  // a row's two blocks of eight scales, then of eight zero points as bytes; 21 words, so that rows lie in different banks
 constexpr int kTcRows = 256, kTcThreads = 608;
 template <int NX, int G> struct TcStage {

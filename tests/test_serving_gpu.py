@@ -84,6 +84,17 @@ def test_rmsnorm_zero_rows_tiny_and_huge_values(ops):
     assert (y == 0).all() and (scale == 0).all()
 
 
+@pytest.mark.parametrize("cols", [200, 250, 256, 512, 501, 1024, 1000, 2048, 1537, 4096, 2050])
+@pytest.mark.parametrize("out_dtype,group", [(None, 0), (E4M3, 0), (E4M3, 64), (I8, 256)])
+def test_rmsnorm_more_rows_than_the_gpu_takes_at_once(ops, cols, out_dtype, group):
+    g = _gen(cols)
+    x, r = (torch.randn(601, cols, generator=g).to(BF16) for _ in range(2))
+    _check_norm(ops, x, torch.rand(cols, generator=g), r, 1e-5, out_dtype, group)
+    _check_norm(ops, x.float(), None, None, 1e-5, out_dtype, group)
+    x[7] *= 2.0**70  # squares beyond f32: the row is summed again
+    _check_norm(ops, x, None, r, 1e-5, out_dtype, group)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_rmsnorm_non_finite_rows_stand_for_nan_and_touch_no_other_row(ops, bad):
     x = torch.randn(4, 640, generator=_gen(5))
