@@ -65,9 +65,9 @@ __device__ __forceinline__ float inverse_fast(int type, float top) {
 }
 
 // ---- rows that fit the registers of a warp or a CTA -------------------------------------------------------
-// One read of x and the residual, one write of everything: HBM-bound.  With VEC a thread has vectors of 8 adjacent columns, 8 * 32
+// One read of x and the residual, one write of everything: HBM-bound.  With VECTORS a thread has 8 adjacent columns, 8 * 32
 // or 8 * THREADS apart (16-byte accesses).  Rows that do not begin on 16-byte boundaries are read element by
-// element; a warp then has 256 * NV adjacent columns, lane by lane (coalesced).  Either way the columns that share a scale
+// element, or two by two where 16-bit rows allow it; a warp then has 256 * NV adjacent columns, lane by lane (coalesced).  Either way the columns that share a scale
 // lie in one warp.
 // bf16 16384 x 8192 + residual -> e4m3 with scales of 128: 154 us (6.1 TB/s, 0.93 of a copy's rate); three passes over the row took 254, and divisions
 // instead of the approximate reciprocal for the scales of groups 180, bound by instruction issue.  f32 1021 x 5001, where no row is aligned:
@@ -93,8 +93,17 @@ template <typename T> __device__ __forceinline__ void write8(T* p, const float (
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, r.v[i]);
 }
 
-template <typename T, bool HELD, int THREADS, int NV, bool VEC>
+enum : int { LANES = 0, PAIRS = 1, VECTORS = 2 };
+template <typename T> struct alignas(2 * sizeof(T)) Two { T v[2]; };
+template <typename T> __device__ __forceinline__ void read2(const T* p, float& x, float& y) {
+  const Two<T> r = *reinterpret_cast<const Two<T>*>(p);
+  x = to_f32(r.v[0]), y = to_f32(r.v[1]);
+}
+template <typename T> __device__ __forceinline__ void write2(T* p, float x, float y) { *reinterpret_cast<Two<T>*>(p) = {from_f32<T>(x), from_f32<T>(y)}; }
+
+template <typename T, bool HELD, int THREADS, int NV, int HOW>
 __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_resident(const RmsArgs a) {
+  constexpr bool VEC = HOW == VECTORS, PAIR = HOW == PAIRS;
   __shared__ float slots[2][32];
   const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31, cols = (int)a.cols;
   const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
@@ -103,7 +112,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
   const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
   auto total = [&](float v, float* at) { return THREADS == 32 ? warp_reduce<SumOp>(v) : block_reduce<SumOp>(v, at); };
   // column of element i of vector k
-  auto col = [&](int k, int i) { return VEC ? (k * THREADS + tid) * VE + i : (tid >> 5) * (256 * NV) + (k * VE + i) * 32 + lane; };
+  auto col = [&](int k, int i) { return VEC ? (k * THREADS + tid) * VE + i : PAIR ? (tid >> 5) * (256 * NV) + (k * VE + (i & ~1)) * 32 + lane * 2 + (i & 1) : (tid >> 5) * (256 * NV) + (k * VE + i) * 32 + lane; };
 
   float e[NV][VE];
   if (VEC) {
@@ -131,6 +140,25 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
         }
       }
     }
+  } else if (PAIR) {
+    auto read = [&](const T* p, float (&v)[NV][VE]) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; i += 2) {
+          v[k][i] = v[k][i + 1] = 0.0f;
+          if (col(k, i) < cols) read2(p + col(k, i), v[k][i], v[k][i + 1]);
+        }
+    };
+    read(x, e);
+    if (res) {
+      float r[NV][VE];
+      read(res, r);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) e[k][i] += r[k][i];
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
@@ -154,6 +182,10 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
     for (int k = 0; k < NV; ++k) {
       if (VEC) {
         if (col(k, 0) < cols) write8(h + col(k, 0), e[k]);
+      } else if (PAIR) {
+#pragma unroll
+        for (int i = 0; i < VE; i += 2)
+          if (col(k, i) < cols) write2(h + col(k, i), e[k][i], e[k][i + 1]);
       } else {
 #pragma unroll
         for (int i = 0; i < VE; ++i)
@@ -183,6 +215,14 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
     if (a.w) {
       if (VEC) {
         if (col(k, 0) < cols) load_w8<T>(a, col(k, 0), w, true, VE);
+      } else if (PAIR) {
+#pragma unroll
+        for (int i = 0; i < VE; i += 2) {
+          w[i] = w[i + 1] = 0.0f;
+          if (col(k, i) >= cols) continue;
+          if (a.wide_w) read2(static_cast<const float*>(a.w) + col(k, i), w[i], w[i + 1]);
+          else read2(static_cast<const T*>(a.w) + col(k, i), w[i], w[i + 1]);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < VE; ++i) w[i] = col(k, i) < cols ? load_w<T>(a, col(k, i)) : 0.0f;
@@ -201,6 +241,10 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
     for (int k = 0; k < NV; ++k) {
       if (VEC) {
         if (col(k, 0) < cols) write8(y + col(k, 0), e[k]);
+      } else if (PAIR) {
+#pragma unroll
+        for (int i = 0; i < VE; i += 2)
+          if (col(k, i) < cols) write2(y + col(k, i), e[k][i], e[k][i + 1]);
       } else {
 #pragma unroll
         for (int i = 0; i < VE; ++i)
@@ -242,8 +286,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
           else hold8<HELD_I8>(y + col(k, 0), e[k], inv, true, VE);
         }
       } else {
-        float m[VE];  // the maximum of element i's group
-        if (a.group) {
+        float m[VE];  // the maximum of element i's group (PAIRS have none)
+        if (!PAIR && a.group) {
 #pragma unroll
           for (int i = 0; i < VE; ++i) m[i] = warp_reduce<MaxOp>(fabsf(e[k][i]));
 #pragma unroll
@@ -259,7 +303,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
           const int c = col(k, i);
-          if (a.group) {
+          if (!PAIR && a.group) {
             inv = inverse_fast(a.out_type, m[i]);
             if (c < cols && lane == 0 && i % steps == 0) a.scale[row * a.groups + (c >> shift)] = m[i] * top_inverse(a.out_type);
           }
@@ -360,31 +404,32 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
   }
 }
 
-template <typename T, bool HELD, int THREADS, int NV> int run_resident(const RmsArgs& a, bool vec, cudaStream_t s) {
+template <typename T, bool HELD, int THREADS, int NV> int run_resident(const RmsArgs& a, int how, cudaStream_t s) {
   const unsigned grid = (unsigned)(THREADS == 32 ? (a.rows + 7) / 8 : a.rows), threads = THREADS == 32 ? 256 : THREADS;
-  if (vec) rmsnorm_resident<T, HELD, THREADS, NV, true><<<grid, threads, 0, s>>>(a);
-  else rmsnorm_resident<T, HELD, THREADS, NV, false><<<grid, threads, 0, s>>>(a);
+  if (how == VECTORS) rmsnorm_resident<T, HELD, THREADS, NV, VECTORS><<<grid, threads, 0, s>>>(a);
+  else if (how == PAIRS && sizeof(T) == 2) rmsnorm_resident<T, HELD, THREADS, NV, sizeof(T) == 2 ? PAIRS : LANES><<<grid, threads, 0, s>>>(a);
+  else rmsnorm_resident<T, HELD, THREADS, NV, LANES><<<grid, threads, 0, s>>>(a);
   return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "rmsnorm launch");
 }
 // Threads of a row: many rows want few, with the work of a thread in flight, few rows all that help.  bf16 + residual -> e4m3 with scales of 128, a warp or fewer threads
 // against 256: 65 536 x 256 24.7 / 142 us (52 with registers for 1024), 16 384 x 1024 23.0 / 42.4, 16 384 x 1536 32.8 / 46.9, 16 384 x 2560 60.6 / 70.5; 592 x 1024 3.9 / 2.9,
 // 16 x 2048 4.0 / 2.7, 600 x 4096 5.7 / 5.1 (and 1500 x 1024 4.8 / 5.4).  4096 x 16 384 in registers 89 us, streamed 140.
-template <typename T, bool HELD> int run_rms(const RmsArgs& a, bool vec, cudaStream_t s) {
+template <typename T, bool HELD> int run_rms(const RmsArgs& a, int how, cudaStream_t s) {
   const bool many = a.rows > 4 * kSmCount;
   if (a.rows <= INT32_MAX) {
     if (many && a.cols <= 4096) {
-      if (a.cols <= 256) return run_resident<T, HELD, 32, 1>(a, vec, s);
-      if (a.cols <= 512) return run_resident<T, HELD, 32, 2>(a, vec, s);
-      if (a.cols <= 1024) return run_resident<T, HELD, 32, 4>(a, vec, s);
-      return a.cols <= 2048 ? run_resident<T, HELD, 64, 4>(a, vec, s) : run_resident<T, HELD, 128, 4>(a, vec, s);
+      if (a.cols <= 256) return run_resident<T, HELD, 32, 1>(a, how, s);
+      if (a.cols <= 512) return run_resident<T, HELD, 32, 2>(a, how, s);
+      if (a.cols <= 1024) return run_resident<T, HELD, 32, 4>(a, how, s);
+      return a.cols <= 2048 ? run_resident<T, HELD, 64, 4>(a, how, s) : run_resident<T, HELD, 128, 4>(a, how, s);
     }
-    if (a.cols <= 2048) return run_resident<T, HELD, 256, 1>(a, vec, s);
-    if (a.cols <= 4096) return run_resident<T, HELD, 256, 2>(a, vec, s);
-    if (a.cols <= 8192) return run_resident<T, HELD, 256, 4>(a, vec, s);
-    if (a.cols <= 16384) return run_resident<T, HELD, 512, 4>(a, vec, s);
+    if (a.cols <= 2048) return run_resident<T, HELD, 256, 1>(a, how, s);
+    if (a.cols <= 4096) return run_resident<T, HELD, 256, 2>(a, how, s);
+    if (a.cols <= 8192) return run_resident<T, HELD, 256, 4>(a, how, s);
+    if (a.cols <= 16384) return run_resident<T, HELD, 512, 4>(a, how, s);
   }
   const int64_t grid = a.rows < (1 << 20) ? a.rows : (1 << 20);
-  rmsnorm_stream<T, HELD, 512><<<(unsigned)grid, 512, 0, s>>>(a, vec);
+  rmsnorm_stream<T, HELD, 512><<<(unsigned)grid, 512, 0, s>>>(a, how == VECTORS);
   return cudaPeekAtLastError() == cudaSuccess ? IB200_OK : cuda_fail(cudaGetLastError(), "rmsnorm launch");
 }
 
@@ -411,13 +456,17 @@ int launch_rmsnorm(const void* x, int64_t x_stride, const void* res, int64_t res
   const int e = dtype_size(dtype);
   RmsArgs a{x, res, w, y, h, scale, x_stride, res_stride, h_stride, rows, cols, group ? (cols + group - 1) / group : 1, (int)group, out_dtype,
             w_dtype == IB200_F32, eps};
-  // 16-byte loads: every row of every operand has to begin on a 16-byte boundary (8 bytes for the held result)
-  auto even = [&](const void* p, int64_t stride, int bytes) { return !p || (aligned16(p) && (rows == 1 || stride * bytes % 16 == 0)); };
-  const bool vec = cols % VE == 0 && even(x, x_stride, e) && even(res, res_stride, e) && even(h, h_stride, e) && even(w, 0, 4) &&
-                   (held ? (reinterpret_cast<uintptr_t>(y) & 7) == 0 : even(y, cols, e));
-  if (dtype == IB200_F32) return held ? run_rms<float, true>(a, vec, s) : run_rms<float, false>(a, vec, s);
-  if (dtype == IB200_BF16) return held ? run_rms<__nv_bfloat16, true>(a, vec, s) : run_rms<__nv_bfloat16, false>(a, vec, s);
-  return held ? run_rms<__half, true>(a, vec, s) : run_rms<__half, false>(a, vec, s);
+  // Every row of every operand has to begin on a boundary of `bytes`: 16 for vectors of eight (8 for the held result), 4 for pairs (2).  Scales of
+  // groups are taken over the lanes of whole groups, which pairs do not have.  Pairs halve the accesses of 16-bit rows: f16 10 880 x 3084 63 us (95 element by element),
+  // to e4m3 76 (130), 20 000 x 1002 33 (53); f32 rows lose by them (4000 x 5002 63, 54).
+  auto at = [&](const void* p, int64_t row_bytes, int bytes) { return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && (rows == 1 || row_bytes % bytes == 0)); };
+  auto even = [&](int bytes, int w_bytes, int y_bytes) {
+    return at(x, x_stride * e, bytes) && at(res, res_stride * e, bytes) && at(h, h_stride * e, bytes) && at(w, 0, w_bytes) && at(y, held ? cols : cols * e, y_bytes);
+  };
+  const int how = cols % VE == 0 && even(16, 16, held ? 8 : 16) ? VECTORS : e == 2 && cols % 2 == 0 && group == 0 && even(4, w_dtype == IB200_F32 ? 8 : 4, held ? 2 : 4) ? PAIRS : LANES;
+  if (dtype == IB200_F32) return held ? run_rms<float, true>(a, how, s) : run_rms<float, false>(a, how, s);
+  if (dtype == IB200_BF16) return held ? run_rms<__nv_bfloat16, true>(a, how, s) : run_rms<__nv_bfloat16, false>(a, how, s);
+  return held ? run_rms<__half, true>(a, how, s) : run_rms<__half, false>(a, how, s);
 }
 
 }  // namespace ib200

@@ -25,10 +25,16 @@ def _gen(seed):
     return g
 
 
+def _placed(t):
+    """On the GPU with the strides and the storage offset that it has."""
+    last = t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
+    return torch.as_strided(torch.as_strided(t, (last,), (1,), 0).cuda(), t.shape, t.stride(), t.storage_offset())
+
+
 # ---- rms-norm ---------------------------------------------------------------------------------------
 
 def _check_norm(ops, x, w, residual, eps, out_dtype, group, **more):
-    y, scale, h = ops.rmsnorm(x.cuda(), None if w is None else w.cuda(), residual=None if residual is None else residual.cuda(), eps=eps,
+    y, scale, h = ops.rmsnorm(_placed(x), None if w is None else _placed(w), residual=None if residual is None else _placed(residual), eps=eps,
                               out_dtype=out_dtype, group=group, **more)
     want_h, want = ref.rmsnorm(x, w, residual, eps)
     cols = x.shape[-1]
@@ -93,6 +99,20 @@ def test_rmsnorm_more_rows_than_the_gpu_takes_at_once(ops, cols, out_dtype, grou
     _check_norm(ops, x.float(), None, None, 1e-5, out_dtype, group)
     x[7] *= 2.0**70  # squares beyond f32: the row is summed again
     _check_norm(ops, x, None, r, 1e-5, out_dtype, group)
+
+
+@pytest.mark.parametrize("cols", [2, 6, 250, 1002, 3084, 5002, 10002])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shift", [0, 1, 2])
+def test_rmsnorm_rows_that_begin_on_pairs(ops, cols, dtype, shift):
+    """Even widths; rows, residuals and weights that begin where pairs do, or `shift` elements later."""
+    g = _gen(cols + shift)
+    a, b = (torch.randn(5, cols + 2, generator=g).to(dtype) for _ in range(2))
+    w = torch.randn(cols + 2, generator=g)
+    for out_dtype in (None, E4M3, I8):
+        _check_norm(ops, a[:, shift:shift + cols], None, b[:, :cols], 1e-5, out_dtype, 0)
+        _check_norm(ops, a[:, :cols], w.to(dtype)[:cols], b[:, shift:shift + cols], 1e-5, out_dtype, 0)
+        _check_norm(ops, a[:, :cols], w[shift:shift + cols], None, 1e-5, out_dtype, 0)
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
@@ -337,10 +357,7 @@ def _paged(seed, news, lens, heads, dim, block, dtype, held, slack_pages=3, tabl
 
 def _on_gpu(t):
     """On the GPU with the strides it has."""
-    if t.is_contiguous():
-        return t.cuda()
-    last = t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1
-    return torch.as_strided(torch.as_strided(t, (last,), (1,), 0).cuda(), t.shape, t.stride(), t.storage_offset())
+    return t.cuda() if t.is_contiguous() else _placed(t)
 
 
 def _cuda(d):
