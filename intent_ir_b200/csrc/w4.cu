@@ -1,6 +1,6 @@
 // Products with 4-bit weights:
 //   y[m, n] = sum over groups g of  s[n, g] * xs[m, g] * sum over k in g of  x[m, k] * (q[n, k] - z[n, g])   + bias[n]
-// q is [N, K/2], the even k of a byte in its low half; z is 8 where there are no zero points; xs (the scales of 8-bit
+// q is [N, K/2], the even k of a byte in its low half; z is 0 .. 127, and 8 where there are no zero points; xs (the scales of 8-bit
 // activations) is 1, one value per row, or one per row and group.  x * (q - z) is exact in f32 (and in the 16-bit types),
 // sums are f32.
 #include <array>
@@ -76,13 +76,20 @@ template <uint32_t MASK> __device__ __forceinline__ uint32_t under(uint32_t x, u
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "n"(MASK), "r"(magic));
   return y;
 }
-// What brings a nibble under an exponent back to q - z, in both halves: 128 + z in bf16; 1024 + z, and -(64 + z) for nibbles four bits up, in f16
+// What brings a nibble under an exponent back to q - z, in both halves: 128 + z in bf16; 1024 + z, and -(64 + z) for nibbles four bits up, in f16.
+// 128 + z fits bf16's eight bits up to z = 127; a zero point above makes the group's products NaN, in every type alike.
 struct Zero {
   uint32_t lo, hi;
 };
-template <bool BF> __device__ __forceinline__ uint32_t pattern_of(uint32_t z) { return (BF ? 0x43004300u : 0x64006400u) | z * 0x10001u; }
-template <bool BF> __device__ __forceinline__ Zero zero_of(uint32_t pattern) { return {pattern, BF ? 0u : (pattern << 4 & 0x00f000f0u) | 0xD400D400u}; }
+__device__ __forceinline__ uint32_t both_halves(uint32_t x) { return x * 0x10001u; }
+template <bool BF> __device__ __forceinline__ uint32_t pattern16_of(uint32_t z) { return z > 127u ? 0x7fffu : (BF ? 0x4300u : 0x6400u) + z; }
+template <bool BF> __device__ __forceinline__ uint32_t pattern_of(uint32_t z) { return both_halves(pattern16_of<BF>(z)); }
 template <typename H> __device__ __forceinline__ H as_pair(uint32_t x) { return *reinterpret_cast<const H*>(&x); }
+template <bool BF> __device__ __forceinline__ Zero zero_of(uint32_t pattern) {
+  if (BF) return {pattern, 0u};
+  const __half2 hi = __hsub2(__half2half2(__ushort_as_half(0x6380)), as_pair<__half2>(pattern));  // 960 - (1024 + z), exact
+  return {pattern, *reinterpret_cast<const uint32_t*>(&hi)};
+}
 // the pairs (0, 4), (1, 5), (2, 6), (3, 7) of a word's eight q - z; `magic`: the exponent, in a register
 template <bool BF> __device__ __forceinline__ void weights_of(uint32_t w, const Zero& z, uint32_t magic, uint32_t (&v)[4]) {
   if (BF) {
@@ -169,6 +176,7 @@ __device__ __forceinline__ RowBlock read_block(const W4Args& a, bool zeros, int 
 __device__ __forceinline__ float scale_of(const W4Args& a, const RowBlock& r, int i) {
   return value_of(a.s_vec && a.s_type != IB200_F32 ? r.v[i / 2] >> (i & 1) * 16 & 0xffffu : r.v[i], a.s_type);
 }
+__device__ __forceinline__ uint32_t zero_byte(const W4Args& a, const RowBlock& r, int i) { return a.z_vec ? r.v[i / 4] >> (i & 3) * 8 & 0xffu : r.v[i]; }
 template <bool BF> __device__ __forceinline__ void leave_block(const W4Args& a, bool zeros, uint8_t* row, int block, const RowBlock& r) {
   uint4* to = reinterpret_cast<uint4*>(row + (zeros ? 64 : 0) + (block & 1) * 32);
 #pragma unroll
@@ -176,7 +184,7 @@ template <bool BF> __device__ __forceinline__ void leave_block(const W4Args& a, 
     uint32_t v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (zeros) v[e] = pattern_of<BF>((a.z_vec ? r.v[(i + e) / 4] >> (e * 8) : r.v[i + e]) & 15u);
+      if (zeros) v[e] = pattern_of<BF>(zero_byte(a, r, i + e));
       else v[e] = __float_as_uint(scale_of(a, r, i + e));
     }
     to[i / 4] = make_uint4(v[0], v[1], v[2], v[3]);
@@ -523,7 +531,7 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t at) {
 // Chunk i's widened weights arriving says that chunk i - 2 has been read back, so its buffers need no barrier of their own.
 // 64 x 16384 x 8192, e4m3, groups of 128: 34.8 us (494 TFLOP/s; the weights' bytes alone 11 us).  Issue of the widening's instructions bounds it (55 % of the slots; the tensor
 // cores are busy 15 % of the time).  On mma.sync the same product took 110 us; with eight widening warps 43, with scales fetched when they were needed 58.
-constexpr int kTcRowScales = 84;  // a row's two blocks of eight scales, then of eight zero points as bytes; 21 words, so that rows lie in different banks
+constexpr int kTcRowScales = 100;  // a row's two blocks of eight scales, then of eight zero points' patterns; 25 words, so that rows lie in different banks
 constexpr int kTcRows = 256, kTcThreads = 608;
 template <int NX, int G> struct TcStage {
   static constexpr int GROUPS = kStageK / G;
@@ -672,10 +680,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
     int block = s0 * GROUPS >> 3;
     RowBlock ahead = read_block(a, half, n0 + row, block);
     auto next_block = [&] {
-      uint32_t* to = reinterpret_cast<uint32_t*>(scales + (half ? 64 + (block & 1) * 8 : (block & 1) * 32));
+      uint32_t* to = reinterpret_cast<uint32_t*>(scales + (half ? 64 + (block & 1) * 16 : (block & 1) * 32));
       if (half) {
-        to[0] = a.z_vec ? ahead.v[0] : ahead.v[0] | ahead.v[1] << 8 | ahead.v[2] << 16 | ahead.v[3] << 24;
-        to[1] = a.z_vec ? ahead.v[1] : ahead.v[4] | ahead.v[5] << 8 | ahead.v[6] << 16 | ahead.v[7] << 24;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = pattern16_of<BF>(zero_byte(a, ahead, 2 * e)) | pattern16_of<BF>(zero_byte(a, ahead, 2 * e + 1)) << 16;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) to[e] = __float_as_uint(scale_of(a, ahead, e));
@@ -724,10 +732,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
       // the row's bytes of the stage, chunks swizzled by row % 8: both the chunk and the half only flip address bits
       const uint32_t row_at = (smem_addr(smem) + (uint32_t)((s - s0) % kStages * S::BYTES + row * kRowBytes)) ^ (uint32_t)((row & 7) << 4) ^ (uint32_t)(half * (KS / 2));
       const float* scales_of = reinterpret_cast<const float*>(scales + (block & 1) * 32) + (s * GROUPS & 7);
-      const uint8_t* zeros_of = scales + 64 + (block & 1) * 8 + (s * GROUPS & 7);
+      const uint16_t* zeros_of = reinterpret_cast<const uint16_t*>(scales + 64 + (block & 1) * 16) + (s * GROUPS & 7);
 #pragma unroll
       for (int c = 0; c < GROUPS; ++c, ++i) {
-        const Zero zero = a.z ? zero_of<BF>(pattern_of<BF>(zeros_of[c] & 15u)) : eight;
+        const Zero zero = a.z ? zero_of<BF>(both_halves(zeros_of[c])) : eight;
         const float scale = scales_of[c];
         constexpr int WORDS = KS >= 32 ? 4 : 2;  // of q a time
 #pragma unroll
