@@ -12,12 +12,15 @@
 // Inside a CTA the four warps take 32 keys each of a tile, with copies of their own two stages deep (cp.async) and no
 // barrier between them until the unit ends.  Both products run on mma.sync with the keys as the 16 rows: S' = K Q' and
 // O' = V' P', so that 8 queries fill a fragment where queries as rows would need 16.  Bytes are widened to f16, which
-// is exact for both types; scales are applied to the scores and to p.  q is scaled by a power of two to below 2 (exact), p * vs
-// by another one to below 2^15, so that f16 holds them to 2^-12 over 2^39.
+// is exact for both types; scales are applied to the scores and to p.  q is scaled by a power of two to below 2 (f16 then holds it to 2^-12 of itself
+// down to 2^-14 of the row's largest), and p * vs by what takes the row's own largest to between 2^10 and 2^14: f16 holds each of them to 2^-12 of itself
+// or 2^-35 of the largest.  A key that a row does not see or give weight to does not enter that, whatever scale its page has; one whose weight is below
+// 2^-112 of the row's largest may count for less than its scale would make of it.
 //
 // With 8 rows to a unit HBM bounds it: 64 sequences of up to 8193 keys, 32 / 8 heads of 128, e4m3, 93 us (5.8 TB/s, 0.89 of a copy's rate); 2 of 131 073 keys,
 // 64 / 8 heads, 69 us (5.4 TB/s).  With more rows the instructions around the products do (39 to 45 % of the issue slots, the rest waits on their chains): 16 x 5
 // new tokens over 15 000 keys 82 us (3.3 TB/s, 133 TFLOP/s).  Short work is a chain of latencies: 702 keys 7.0 us, 33 x up to 5 new tokens in a window of 2048 20.6 us.
+// One power for all rows instead, led by every page's scale, would take 64 sequences in 92 us, 16 x 5 new tokens in 81; it lost a window's keys to a page in front of it.
 // A third stage of copies changed nothing at a width of 64 (20.8 / 20.7 us; 64 sequences 58.0 / 55.9).
 #include <algorithm>
 #include <atomic>
@@ -33,6 +36,8 @@ constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 32, kTile = kWarps * k
 // What beginning a unit costs, in tiles: tables, pages and queries are fetched one after the other and the warps' results joined.
 // 64 sequences of up to 8193 tokens: 115 us with 0, 106 with 1, 98 with 2, 95 with 4, 96 with 6.
 constexpr int kStart = 4;
+constexpr float kNone = -3.402823466e38f;  // a row's maxima before its first key: finite, so that differences of two are numbers
+constexpr float kUp = 14.0f;               // a row's numerators p * vs are raised to at most 2^kUp
 template <int D> struct Cfg {
   static constexpr int kStageBytes = 2 * kStep * D;  // keys, values
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
@@ -53,6 +58,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -62,6 +72,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+// the largest of the eight lanes that hold a row's other keys
+__device__ __forceinline__ float over_rows(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
 }
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -131,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ int64_t sums[kWarps], found_before;
   __shared__ int found;
-  __shared__ float stat[kWarps][ROWS][2], top_v[kWarps], joined[ROWS][2];
+  __shared__ float stat[kWarps][ROWS][2], joined[ROWS][2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int batch = (int)a.batch, group = (int)by.group.d;
 
@@ -335,11 +351,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
       }
     }
 
-    float o[NT][MT][4], m[NT][2], l[NT][2], vtop = 0x1p-100f;
+    // l is the sum of p = 2^(score - m), o that of p * vs * v8 * 2^(m - high): m is the row's largest score so far, high that of score + log2(vs) - kUp (a bound)
+    float o[NT][MT][4], m[NT][2], high[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) m[nt][c] = -INFINITY, l[nt][c] = 0.0f;
+      for (int c = 0; c < 2; ++c) m[nt][c] = high[nt][c] = kNone, l[nt][c] = 0.0f;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -378,20 +395,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
       // ---- running maximum and sum ------------------------------------------------------------------
       const float ks[2] = {__shfl_sync(0xffffffffu, cur.ks, 2 * (step & 15)), __shfl_sync(0xffffffffu, cur.ks, 2 * (step & 15) + 1)};
       const float vs[2] = {__shfl_sync(0xffffffffu, cur.vs, 2 * (step & 15)), __shfl_sync(0xffffffffu, cur.vs, 2 * (step & 15) + 1)};
-      // the power of two above the values' scales so far; NaN scales do not enter it (they reach p below)
-      const float vmax = fmaxf(vtop, fmaxf(fabsf(vs[0]), fabsf(vs[1])));
-      float grow = 1.0f;
-      if (vmax > vtop) {
-        const float up = __uint_as_float(min((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u, 0x7f000000u));
-        grow = vtop / up;
-        vtop = up;
-      }
-      const float vf[2] = {vs[0] * (0x1p14f / vtop), vs[1] * (0x1p14f / vtop)};
-      uint32_t pf[NT][2][2];
-      [[maybe_unused]] uint32_t pl[NT][2][2];  // what p's rounding left
+      // log2 of the values' larger scale, 2^-100 at least; a NaN counts for nothing (it reaches p below)
+      const float vs_top = fmaxf(fmaxf(fabsf(vs[0]), fabsf(vs[1])), 0x1p-100f);
+      float vs_most = log2_fast(vs_top) - kUp;
+      // every row's largest score of the step (over both halves' keys), and a bound on score + log2(vs)
+      float top[NT][2], most[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float top[2] = {-INFINITY, -INFINITY};
+        top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -402,28 +413,48 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
               if (key > hi[nt][c & 1] || key < low[nt][c & 1]) x = -INFINITY;
             }
             sv[mt][nt][c] = x;
-            top[c & 1] = fmaxf(top[c & 1], x);
+            top[nt][c & 1] = fmaxf(top[nt][c & 1], x);
           }
-        float base[2], keep[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 4));
-          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 8));
-          top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], 16));
-          const float now = fmaxf(m[nt][c], top[c]);
-          base[c] = now == -INFINITY ? 0.0f : now;
-          keep[c] = exp2_fast(m[nt][c] - base[c]);
+          top[nt][c] = over_rows(top[nt][c]);
+          most[nt][c] = top[nt][c] + vs_most;
+        }
+      }
+      if (!(vs_top <= fminf(16.0f * fminf(fabsf(vs[0]), fabsf(vs[1])), 3.402823466e38f))) {  // far apart: a half's scale counts with the half's own scores only,
+        float by_half[2];                                                                  // an infinite one (whose rows are not finite) not at all
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) by_half[mt] = isinf(vs[mt]) ? -100.0f - kUp : log2_fast(fmaxf(fabsf(vs[mt]), 0x1p-100f)) - kUp;
+        vs_most = fmaxf(by_half[0], by_half[1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            most[nt][c] = fmaxf(over_rows(fmaxf(sv[0][nt][c], sv[0][nt][c + 2])) + by_half[0], over_rows(fmaxf(sv[1][nt][c], sv[1][nt][c + 2])) + by_half[1]);
+      }
+      uint32_t pf[NT][2][2];
+      [[maybe_unused]] uint32_t pl[NT][2][2];  // what p's rounding left
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float keep[2], raise[2];  // what o is to be multiplied by, and p for its numerators
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float now = fmaxf(m[nt][c], top[nt][c]), now_most = fmaxf(high[nt][c], most[nt][c]);
+          l[nt][c] *= exp2_fast(m[nt][c] - now);
+          keep[c] = exp2_fast(high[nt][c] - now_most);
+          raise[c] = exp2_fast(fminf(now - now_most, (126.0f - kUp) - vs_most));  // (finite times either scale)
           m[nt][c] = now;
-          l[nt][c] *= keep[c];
+          high[nt][c] = now_most;
         }
         float p[2][4];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
+          const float raised[2] = {vs[mt] * raise[0], vs[mt] * raise[1]};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float x = exp2_fast(sv[mt][nt][c] - base[c & 1]);
+            const float x = exp2_fast(sv[mt][nt][c] - m[nt][c & 1]);
             l[nt][c & 1] += x;
-            p[mt][c] = x * vf[mt];
+            p[mt][c] = x * raised[c & 1];
             if constexpr (masked) {  // a NaN scale counts only for the rows that see the key
               const int key = key0 + mt * 16 + (c >> 1) * 8 + g;
               if (key > hi[nt][c & 1] || key < low[nt][c & 1]) p[mt][c] = 0.0f;
@@ -438,13 +469,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
             pl[nt][mt][1] = transpose8x8(pack16(p[mt][2] - h1.x, p[mt][3] - h1.y));
           }
         }
-        const float k0 = keep[0] * grow, k1 = keep[1] * grow;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          o[nt][i][0] *= k0;
-          o[nt][i][1] *= k1;
-          o[nt][i][2] *= k0;
-          o[nt][i][3] *= k1;
+          o[nt][i][0] *= keep[0];
+          o[nt][i][1] *= keep[1];
+          o[nt][i][2] *= keep[0];
+          o[nt][i][3] *= keep[1];
         }
       }
 
@@ -464,14 +494,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
             vb[e][0] = x.x, vb[e][1] = x.y;
           }
         }
-        bool apart = false;  // a NaN among values that some rows do not see: the rows' products are taken one by one
+        bool by_row = false;  // a NaN among values that some rows do not see: the rows' products are taken one by one
         if constexpr (HELD == HELD_E4M3 && masked) {
           uint32_t any = 0;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int k = 0; k < D / 32; ++k) any |= __vcmpeq4(vb[e][k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-          apart = __any_sync(0xffffffffu, any != 0);
+          by_row = __any_sync(0xffffffffu, any != 0);
         }
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
@@ -480,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
           widen<HELD>(__byte_perm(vb[2][k], vb[3][k], 0x5140), f[0][2], f[0][3]);
           widen<HELD>(__byte_perm(vb[0][k], vb[1][k], 0x7362), f[1][0], f[1][1]);
           widen<HELD>(__byte_perm(vb[2][k], vb[3][k], 0x7362), f[1][2], f[1][3]);
-          if (!apart) {
+          if (!by_row) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -552,11 +582,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
           stat[warp][row][1] = x;
         }
         float* to_row = box + (warp * ROWS + row) * C::kPitch + g * (D / 8);
+        const float down = exp2_fast(high[nt][c] - m[nt][c]);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(to_row + 2 * i) = make_float2(o[nt][i][c], o[nt][i][2 + c]);
+        for (int i = 0; i < MT; ++i) *reinterpret_cast<float2*>(to_row + 2 * i) = make_float2(o[nt][i][c] * down, o[nt][i][2 + c] * down);
       }
     }
-    if (lane == 0) top_v[warp] = vtop;
     __syncthreads();
     const bool whole = from == 0 && to == s.tiles;
     float* part = CLUSTER ? nullptr : sc.part + ((int64_t)blockIdx.x * 2 + (piece_start == w_start ? 0 : 1)) * (ROWS * (D + 2));
@@ -574,16 +604,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
     for (int idx = threadIdx.x; idx < ROWS * (D / 4); idx += kThreads) {
       const int row = idx / (D / 4), d = idx % (D / 4) * 4;
       if (row >= rows) break;
-      float mm = fmaxf(fmaxf(stat[0][row][0], stat[1][row][0]), fmaxf(stat[2][row][0], stat[3][row][0]));
-      const float base = mm == -INFINITY ? 0.0f : mm;
+      const float mm = fmaxf(fmaxf(stat[0][row][0], stat[1][row][0]), fmaxf(stat[2][row][0], stat[3][row][0]));
       float sum = 0.0f, v[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
-        const float f = exp2_fast(stat[i][row][0] - base);
+        const float f = exp2_fast(stat[i][row][0] - mm);
         sum += stat[i][row][1] * f;
         const float4 x = *reinterpret_cast<const float4*>(box + (i * ROWS + row) * C::kPitch + d);
-        const float fv = f * (top_v[i] * 0x1p-14f);
-        v[0] += x.x * fv, v[1] += x.y * fv, v[2] += x.z * fv, v[3] += x.w * fv;
+        v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
       }
       if constexpr (CLUSTER) {
         *reinterpret_cast<float4*>(joint + row * C::kPitch + d) = make_float4(v[0], v[1], v[2], v[3]);
@@ -604,9 +632,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kC
         const int row = idx / (D / 4), d = idx % (D / 4) * 4;
         float mm = -INFINITY, sum = 0.0f, v[4] = {0, 0, 0, 0};
         for (int r = 0; r < by.split; ++r) mm = fmaxf(mm, cluster_read(&joined[row][0], r));
-        const float base = mm == -INFINITY ? 0.0f : mm;
         for (int r = 0; r < by.split; ++r) {
-          const float f = exp2_fast(cluster_read(&joined[row][0], r) - base);
+          const float f = exp2_fast(cluster_read(&joined[row][0], r) - mm);
           sum += cluster_read(&joined[row][1], r) * f;
           const float4 x = cluster_read4(joint + row * C::kPitch + d, r);
           v[0] += x.x * f, v[1] += x.y * f, v[2] += x.z * f, v[3] += x.w * f;
@@ -664,8 +691,7 @@ __global__ void __launch_bounds__(kJoin) join_kernel(const Kv8Attention a, const
   for (int base = c0; base <= c1; base += 32) {  // every warp has the weights of 32 pieces, a lane each
     const int c = base + lane, n = min(32, c1 - base + 1);
     const float pm = c <= c1 ? piece(c)[ROWS * D + row] : -INFINITY, pl = c <= c1 ? piece(c)[ROWS * D + ROWS + row] : 0.0f;
-    const float now = fmaxf(m, warp_reduce<MaxOp>(pm)), from = now == -INFINITY ? 0.0f : now;
-    const float keep = exp2_fast(m - from), f = exp2_fast(pm - from);
+    const float now = fmaxf(m, warp_reduce<MaxOp>(pm)), keep = exp2_fast(m - now), f = exp2_fast(pm - now);
     sum = sum * keep + warp_reduce<SumOp>(c <= c1 ? pl * f : 0.0f);
 #pragma unroll
     for (int e = 0; e < PER; ++e) v[e] *= keep;

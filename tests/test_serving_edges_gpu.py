@@ -41,3 +41,135 @@ def test_w4_every_zero_point_and_nibble(ops, m, dtype, group):
         got = ops.w4_matmul(x.cuda(), q.cuda(), scales.cuda(), zeros=zeros.cuda(), group=group, out_dtype=F32).cpu()
         assert torch.equal(got[:, :128].double(), w[:128, at:at + m].t())
         assert torch.isnan(got[:, 128:]).all()
+
+
+# ---- attention: value scales that lie far apart -----------------------------------------------------
+
+def _tight_bound(q, d, scale, window):
+    """o in 64 bits and a bound for numerators that are held in 16 bits relative to the largest of the ROW's own: as the reference's
+    (2^-11, 2^-18 and twice a score's error of the summed magnitudes, half a step of the result), but with a floor that no value outside the
+    row's weights raises.  A numerator p * scale is scaled so that the row's largest lies between 2^10 and 2^14; one that is subnormal in f16
+    is off by 2^-25, 2^-35 of the largest, times the 8-bit value (448, 127 at most): for each of the n keys."""
+    want, _, bound, _ = ref.attention(q, *(d[c] for c in CACHE), d["block_table"], d["seq_lens"], d["cu_new"], scale, window)
+    pages, heads, block, dim = d["k_cache"].shape
+    group = q.shape[1] // heads
+    for b in range(len(d["seq_lens"])):
+        n = int(d["cu_new"][b + 1] - d["cu_new"][b])
+        for i in range(n):
+            pos, t = int(d["seq_lens"][b]) - n + i, int(d["cu_new"][b]) + i
+            at = torch.arange(max(0, pos - window + 1) if window else 0, pos + 1)
+            page = d["block_table"][b, at // block].long()
+            kk = d["k_cache"][page, :, at % block].double() * d["k_scale"][page].double()[:, :, None]
+            v8, vs = d["v_cache"][page, :, at % block].double(), d["v_scale"][page].double()
+            p = torch.softmax(torch.einsum("hgd,jhd->hgj", q[t].double().reshape(heads, group, dim), kk) * scale, -1)
+            size = (torch.einsum("hgd,jhd->hgj", q[t].double().reshape(heads, group, dim).abs(), kk.abs()) * abs(scale)).amax(-1)
+            wrong = size * (dim / 16 + 4) * 2.0**-22 + 2.0**-21
+            weight = p * vs.t()[:, None, :]
+            spread = torch.einsum("hgj,jhd->hgd", weight, v8.abs())
+            floor = weight.amax(-1) * len(at) * ref.TOP[d["v_cache"].dtype] * 2.0**-35
+            bound[t] = (spread * (2.0**-11 + 2.0**-18 + 2 * wrong[..., None]) + floor[..., None]).reshape(-1, dim) + want[t].abs() * ref.half_step(q.dtype)
+            bound[t] += 2.0**-25 if q.dtype == F16 else 0.0
+    return want, bound
+
+
+def _check_tight(ops, d, q_heads, uniform, scale=None, window=0, q=None, rows=slice(None)):
+    dim = d["k_cache"].shape[3]
+    scale = dim ** -0.5 if scale is None else scale
+    if q is None:
+        q = torch.randn(d["k"].shape[0], q_heads, dim, generator=_gen(5)).to(d["k"].dtype)
+    dev = _cuda(d)
+    got = ops.attention_kv8(q.cuda(), *(dev[c] for c in CACHE), dev["block_table"], dev["seq_lens"], cu_new=None if uniform else dev["cu_new"], scale=scale,
+                            window=window).cpu().double()[rows]
+    want, bound = (x[rows] for x in _tight_bound(q, d, scale, window))
+    off = (got - want).abs()
+    assert (off <= bound).all(), (off / bound).nan_to_num(nan=float("inf")).max()
+
+
+SHAPES = [(1, 1, 64, F16), (2, 4, 128, BF16), (2, 6, 128, F16), (1, 10, 64, BF16)]
+
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+@pytest.mark.parametrize("heads,group,dim,dtype", SHAPES)
+@pytest.mark.parametrize("huge", [2.0**28, 1e30, float("inf")])
+@pytest.mark.parametrize("room", [20, 1200])
+def test_attention_a_page_in_front_of_the_window_costs_nothing(ops, held, heads, group, dim, dtype, huge, room):
+    """Blocks of 16 are half a step of keys: the page in front of the window is fetched with the window's first one."""
+    for lens, window in (([200, 90], 40), ([211, 215], 36), ([300, 300], 117)):  # the first key is 160, 50; 175, 179; 183
+        d = _paged(70, [1, 1], lens, heads, dim, 16, dtype, held, table_blocks=room)
+        for b, n in enumerate(lens):
+            for blk in range((n - window) // 16):
+                d["v_scale"][int(d["block_table"][b, blk])] = huge
+        _check_tight(ops, d, heads * group, True, window=window)
+        _check_tight(ops, d, heads * group, False, window=window)
+
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+@pytest.mark.parametrize("heads,group,dim,dtype", SHAPES)
+@pytest.mark.parametrize("huge", [2.0**28, 1e30, float("inf")])
+@pytest.mark.parametrize("room", [20, 1200])
+def test_attention_a_later_tokens_page_costs_earlier_rows_nothing(ops, held, heads, group, dim, dtype, huge, room):
+    for lens in ([97, 97], [209, 17], [113, 241]):  # the last new token begins a block, in the first or second half of a step
+        d = _paged(71, [5, 5], lens, heads, dim, 16, dtype, held, table_blocks=room)
+        for b, n in enumerate(lens):
+            d["v_scale"][int(d["block_table"][b, (n - 1) // 16])] = huge
+        d["v_scale"] = d["v_scale"].float()
+        earlier = torch.tensor([0, 1, 2, 3, 5, 6, 7, 8])
+        _check_tight(ops, d, heads * group, True, rows=earlier)
+        _check_tight(ops, d, heads * group, False, rows=earlier)
+
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+@pytest.mark.parametrize("heads,group,dim,dtype", SHAPES)
+@pytest.mark.parametrize("block", [16, 48])
+@pytest.mark.parametrize("uniform", [True, False])
+def test_attention_a_page_without_weight_costs_nothing(ops, held, heads, group, dim, dtype, block, uniform):
+    """A page of huge values whose keys point away from every query: its weight in the softmax is below 2^-126."""
+    for huge in (2.0**28, 2.0**60):
+        d = _paged(72, [3, 3], [500, 260], heads, dim, block, dtype, held, table_blocks=1200)
+        q = (torch.rand(6, heads * group, dim, generator=_gen(8)) + 0.5).to(dtype)
+        for b, n in enumerate((500, 260)):
+            for blk in (0, 2, 3, (n - 4) // block - 1):
+                page = int(d["block_table"][b, blk])
+                d["k_cache"][page] = torch.full(d["k_cache"][page].shape, -100.0).to(held)
+                d["k_scale"][page] = 0.5
+                d["v_scale"][page] = huge
+        _check_tight(ops, d, heads * group, uniform, q=q)
+
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+@pytest.mark.parametrize("heads,group,dim,dtype", [(2, 4, 128, BF16), (1, 10, 64, BF16), (2, 5, 128, BF16)])
+@pytest.mark.parametrize("new", [1, 2, 4])
+def test_attention_value_scales_over_the_whole_range(ops, held, heads, group, dim, dtype, new):
+    """Scales from 2^-100 to 2^100, zeros among them, in every order."""
+    for seed, room in ((73, 40), (74, 1500), (75, 1500)):
+        d = _paged(seed, [new] * 3, [600, 77, 1300], heads, dim, 16, dtype, held, table_blocks=max(room, 90))
+        order = torch.rand(d["v_scale"].shape, generator=_gen(seed)) * 200 - 100
+        if seed == 74:
+            order = order.sort(0).values
+        if seed == 75:
+            order = order / 4 - 70
+        d["v_scale"] = torch.where(torch.rand(order.shape, generator=_gen(seed + 1)) < 0.1, torch.zeros(()), torch.exp2(order))
+        _check_tight(ops, d, heads * group, True)
+        _check_tight(ops, d, heads * group, False)
+
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+@pytest.mark.parametrize("heads,group,dim", [(2, 1, 64), (1, 4, 128), (2, 9, 128)])
+def test_attention_of_f16_results_takes_its_numerators_in_two_parts(ops, held, heads, group, dim):
+    """Few keys, values that cancel: numerators rounded once to f16 (2^-12 of each) would exceed this bound.  Two parts leave 2^-22 of the summed magnitudes,
+    the exponential and a score's rounding 2^-18, each of the n / 16 + 8 sums 2^-22, and the result's own rounding 2^-11 of what is left."""
+    lens = [2, 3, 4, 6, 8, 16]
+    d = _paged(76, [1] * len(lens), lens, heads, dim, 16, F16, held)
+    d["k_scale"] = torch.full_like(d["k_scale"], 1e-3)  # scores of some tenths
+    d["v_scale"] = torch.full_like(d["v_scale"], 0.0173)
+    q = torch.randn(len(lens), heads * group, dim, generator=_gen(9)).to(F16)
+    dev = _cuda(d)
+    got = ops.attention_kv8(q.cuda(), *(dev[c] for c in CACHE), dev["block_table"], dev["seq_lens"]).cpu().double()
+    for t, n in enumerate(lens):
+        page = int(d["block_table"][t, 0])
+        k, v = (d[c + "_cache"][page, :, :n].double() * float(d[c + "_scale"][0, 0]) for c in ("k", "v"))
+        p = torch.softmax(torch.einsum("hgd,hjd->hgj", q[t].double().view(heads, group, dim), k) * dim ** -0.5, -1)
+        want, spread = (torch.einsum("hgj,hjd->hgd", p, x).reshape(-1, dim) for x in (v, v.abs()))
+        off = (got[t] - want).abs()
+        bound = spread * (2.0**-22 + 2.0**-18 + (n / 16 + 8) * 2.0**-22) + want.abs() * ref.half_step(F16) + 2.0**-25
+        assert (off <= bound).all(), (n, (off / bound).max())
