@@ -16,10 +16,20 @@ struct RmsArgs {
   int64_t rows, cols, groups;  // groups: scales per row
   int group;                   // columns per scale, 0: the whole row
   int out_type, wide_w;        // IB200_E4M3, IB200_I8 or the rows' type; whether w is f32
-  float eps;
+  float eps, least;            // least: sums of squares below it are taken again
 };
 
+// Rows whose squares overflow f32 (values beyond 2^60), and those whose squares vanish beside an eps that small, are summed again scaled by a power of two.
+// The sum's threshold leaves what subnormal squares lose (2^-150 each) below 2^-24 of it, and scaled up it stays finite.
 constexpr float kScaleDown = 0x1p-80f;  // takes every f32 to where its square, and 2^30 of them, stay finite
+constexpr float kScaleUp = 0x1p96f, kVanishing = 0x1p-80f, kVanishingEps = 0x1p-90f, kMost = 3.402823466e38f;
+// Such a row's 1 / sqrt(mean + eps) as two factors for its elements, one after the other, so that neither product leaves f32's range
+// where the result does not; sum: of the squares of the elements times scale_of(ss).
+__device__ __forceinline__ float scale_of(float ss) { return ss > 1.0f ? kScaleDown : kScaleUp; }
+__device__ __forceinline__ float2 two_factors(float ss, float sum, float cols, float eps) {
+  const float pre = scale_of(ss), r = 1.0f / sqrtf(sum / cols + eps * pre * pre);
+  return ss > 1.0f ? make_float2(r * 0x1p-40f, kScaleDown * 0x1p40f) : make_float2(kScaleUp, r);
+}
 constexpr int VE = 8;  // elements per thread and vector
 
 template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[VE], bool vec, int left) {
@@ -201,12 +211,16 @@ __global__ void __launch_bounds__(THREADS == 32 ? 256 : THREADS) rmsnorm_residen
       for (int i = 0; i < VE; ++i) s = fmaf(e[k][i] * pre, e[k][i] * pre, s);
     return s;
   };
-  float ss = total(squares(1.0f), slots[0]), rstd;
-  if (isinf(ss)) {  // values beyond 2^60: their squares overflow f32, so the row is summed again scaled down (uniform over the row's threads)
-    rstd = kScaleDown / sqrtf(total(squares(kScaleDown), slots[1]) / (float)cols);
+  const float ss = total(squares(1.0f), slots[0]);
+  float rstd = 1.0f / sqrtf(ss / (float)cols + a.eps);
+  if (!(ss >= a.least && ss <= kMost)) {  // (uniform over the row's threads; NaN comes here and stays)
+    const float2 f = two_factors(ss, total(squares(scale_of(ss)), slots[1]), (float)cols, a.eps);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) e[k][i] *= f.x;
+    rstd = f.y;
     if (THREADS != 32) __syncthreads();  // the slots are used again
-  } else {
-    rstd = 1.0f / sqrtf(ss / (float)cols + a.eps);
   }
   float top = 0.0f;
 #pragma unroll
@@ -334,11 +348,11 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
       }
       return left;
     };
-    auto norm8 = [&](int64_t v, float rstd, float(&out)[VE], int left) {
+    auto norm8 = [&](int64_t v, float first, float rstd, float(&out)[VE], int left) {
       float ww[VE];
       if (a.w) load_w8<T>(a, v * VE, ww, vec, left);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) out[i] = out[i] * rstd * (a.w ? ww[i] : 1.0f);
+      for (int i = 0; i < VE; ++i) out[i] = out[i] * first * rstd * (a.w ? ww[i] : 1.0f);
     };
     auto squares = [&](float pre, float* at) {
       float ss = 0.0f;
@@ -350,20 +364,20 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
       }
       return block_reduce<SumOp>(ss, at);
     };
-    float ss = squares(1.0f, slots[0]), rstd;
-    if (isinf(ss)) {  // values beyond 2^60: their squares overflow f32, so the row is summed again scaled down (uniform over the CTA)
-      ss = squares(kScaleDown, slots[1]);
-      rstd = kScaleDown / sqrtf(ss / (float)a.cols);
+    const float ss = squares(1.0f, slots[0]);
+    float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps), first = 1.0f;
+    if (!(ss >= a.least && ss <= kMost)) {  // (uniform over the CTA; NaN comes here and stays)
+      const float2 f = two_factors(ss, squares(scale_of(ss), slots[1]), (float)a.cols, a.eps);
+      first = f.x;
+      rstd = f.y;
       __syncthreads();
-    } else {
-      rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
     }
     float row_max = 0.0f;
     if (HELD && a.group == 0) {
       for (int64_t v = threadIdx.x; v < nv; v += THREADS) {
         float e[VE];
         const int left = sum8(v, e);
-        norm8(v, rstd, e, left);
+        norm8(v, first, rstd, e, left);
 #pragma unroll
         for (int i = 0; i < VE; ++i) row_max = max_nan(row_max, fabsf(e[i]));
       }
@@ -376,7 +390,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_stream(const RmsArgs a, const
       if (v < nv) {
         left = sum8(v, e);
         if (h) store8(h + v * VE, e, vec, left);
-        norm8(v, rstd, e, left);
+        norm8(v, first, rstd, e, left);
       } else {
 #pragma unroll
         for (int i = 0; i < VE; ++i) e[i] = 0.0f;
@@ -455,7 +469,7 @@ int launch_rmsnorm(const void* x, int64_t x_stride, const void* res, int64_t res
     return fail(IB200_ERR_INVALID, "rmsnorm: a row stride beyond any device");
   const int e = dtype_size(dtype);
   RmsArgs a{x, res, w, y, h, scale, x_stride, res_stride, h_stride, rows, cols, group ? (cols + group - 1) / group : 1, (int)group, out_dtype,
-            w_dtype == IB200_F32, eps};
+            w_dtype == IB200_F32, eps, eps < kVanishingEps ? kVanishing : -1.0f};
   // Every row of every operand has to begin on a boundary of `bytes`: 16 for vectors of eight (8 for the held result), 4 for pairs (2).  Scales of
   // groups are taken over the lanes of whole groups, which pairs do not have.  Pairs halve the accesses of 16-bit rows: f16 10 880 x 3084 63 us (95 element by element),
   // to e4m3 76 (130), 20 000 x 1002 33 (53); f32 rows lose by them (4000 x 5002 63, 54).

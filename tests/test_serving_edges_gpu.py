@@ -43,6 +43,54 @@ def test_w4_every_zero_point_and_nibble(ops, m, dtype, group):
         assert torch.isnan(got[:, 128:]).all()
 
 
+# ---- rms-norm ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,cols", [(3, 64), (5, 1000), (2, 2501), (700, 256), (601, 1537), (3, 8192), (2, 16384), (2, 40000), (3, 3002)])
+@pytest.mark.parametrize("eps", [0.0, 2.0**-130, 2.0**-100])
+@pytest.mark.parametrize("out,group", [(None, 0), (E4M3, 0), (I8, 64)])
+def test_rmsnorm_rows_whose_squares_vanish(ops, rows, cols, eps, out, group):
+    """Squares of rows below 2^-75 are nothing in f32, yet with an eps as small the result is near 1."""
+    g = _gen(cols)
+    x, r = (torch.randn(rows, cols, generator=g) for _ in range(2))
+    size = torch.tensor([1e-25, 1e-18, 1e-36, 1e-30, 1.0, 1e-22, 1e18])[torch.arange(rows) % 7][:, None]
+    w = torch.rand(cols, generator=g) + 0.5
+    _check_norm(ops, x * size, w, None, eps, out, group)
+    _check_norm(ops, x * size, None, r * size, eps, out, group)
+    _check_norm(ops, (x * size).to(BF16), w.to(BF16), (r * size).to(BF16), eps, out, group)
+    one = torch.zeros(rows, cols)
+    one[:, cols // 2] = 2.0**-140  # a subnormal alone in its row: sqrt(cols) without eps
+    _check_norm(ops, one, None, None, eps, out, group)
+
+
+def test_rmsnorm_the_largest_values(ops):
+    x = torch.full((4, 640), 3e38)
+    x[1] = torch.randn(640, generator=_gen(1)) * 1e37
+    x[2, 1:] = 1.0
+    for shape in ((4, 640), (2, 1280), (1, 2560)):
+        at = x.view(shape)
+        _check_norm(ops, at, None, None, 1e-6, None, 0)
+        _, want = ref.rmsnorm(at, None, None, 1e-6)
+        for out, group in ((E4M3, 0), (I8, 64)):
+            y, scale, _ = ops.rmsnorm(at.cuda(), out_dtype=out, group=group)
+            # the ones beside 3e38 come to less than 2^-119, and groups below that hold zeros: they are off by themselves
+            tiny = ref.spread_scale(ref.group_max(want, group), shape[1], group) < 2.0**-119
+            y, scale, slack = y.cpu(), scale.cpu().double(), (shape[1] / 16 + 16) * 2.0**-24
+            assert (y.float()[tiny] == 0).all()
+            s = ref.spread_scale(scale, shape[1], group)
+            step = 0.5 * s if out == I8 else torch.maximum(want.abs() * 2.0**-4, s * 2.0**-10)
+            assert (((y.double() * s - want).abs() <= step + want.abs() * slack * 2) | tiny).all()
+            top = ref.group_max(want, group) / ref.TOP[out]
+            assert ((scale - top).abs() <= top * slack + 1e-45).all()
+
+
+def test_rmsnorm_a_zero_row_without_eps_is_not_a_number(ops):
+    x = torch.randn(5, 320, generator=_gen(2))
+    x[3] = 0
+    for wide in (x, x.repeat(1, 60)):
+        y, _, _ = ops.rmsnorm(wide.cuda(), eps=0.0)
+        assert torch.isnan(y[3]).all() and torch.isfinite(y[[0, 1, 2, 4]]).all()
+
+
 # ---- attention: value scales that lie far apart -----------------------------------------------------
 
 def _tight_bound(q, d, scale, window):
