@@ -460,6 +460,12 @@ int launch_rmsnorm(const void* x, int64_t x_stride, const void* res, int64_t res
   if (group != 0 && (!held || (group != 32 && group != 64 && group != 128 && group != 256)))
     return fail(IB200_ERR_UNSUPPORTED, "rmsnorm: a scale covers 32, 64, 128 or 256 columns of an 8-bit result, or (0) the whole row");
   if (h && !res) return fail(IB200_ERR_INVALID, "rmsnorm: the sum is written only where there is a residual");
+  if (rows > 0 && cols == 0 && held && group == 0) {  // the largest of no values is 0, and so is its scale
+    if (!scale) return fail(IB200_ERR_INVALID, "rmsnorm: null operand");
+    if (beyond_any_device(rows, 1)) return fail(IB200_ERR_INVALID, "rmsnorm: more than 2^40 rows");
+    IB200_CUDA_OK(cudaMemsetAsync(scale, 0, (size_t)rows * sizeof(float), s));
+    return IB200_OK;
+  }
   if (rows == 0 || cols == 0) return IB200_OK;
   if (!x || !y || (held && !scale)) return fail(IB200_ERR_INVALID, "rmsnorm: null operand");
   if (rows > 1 && (x_stride < cols || (res && res_stride < cols) || (h && h_stride < cols)))

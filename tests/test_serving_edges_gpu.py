@@ -91,6 +91,17 @@ def test_rmsnorm_a_zero_row_without_eps_is_not_a_number(ops):
         assert torch.isnan(y[3]).all() and torch.isfinite(y[[0, 1, 2, 4]]).all()
 
 
+@pytest.mark.parametrize("out", [E4M3, I8])
+def test_rmsnorm_rows_without_columns_have_the_scale_zero(ops, out):
+    for rows in (1, 5, 3000):
+        garbage = torch.full((rows, 1), float("nan"), device="cuda")
+        del garbage  # the scale takes its memory
+        y, scale, _ = ops.rmsnorm(torch.empty(rows, 0, device="cuda", dtype=BF16), out_dtype=out)
+        assert y.shape == (rows, 0) and scale.shape == (rows, 1) and (scale == 0).all()
+        _, scale, _ = ops.rmsnorm(torch.empty(rows, 0, device="cuda", dtype=BF16), out_dtype=out, group=64)
+        assert scale.shape == (rows, 0)
+
+
 # ---- attention: value scales that lie far apart -----------------------------------------------------
 
 def _tight_bound(q, d, scale, window):
