@@ -305,8 +305,8 @@ IB200_API int ib200_rmsnorm(const ib200_rmsnorm_args* args, void* stream);
  * q: [N, K/2] bytes, 16-byte aligned, the even k of a pair in the low four bits; scales: [N, ceil(K / group)] of s_dtype (f32,
  * bf16, f16); zeros: bytes 0..127 of the same shape (a larger one makes its row's results NaN), or NULL (8); bias (NULL: none) and y have out_dtype (f32, bf16, f16).
  * x: [M, K] bf16 or f16 with x_scale NULL and x_scale_groups 0, or e4m3 / int8 with x_scale f32 [M, x_scale_groups], 1 or
- * ceil(K / group) of them.  group: 32, 64 or 128; K a multiple of 32; M and N any.  f32 sums.  scratch: 256-byte aligned,
- * ib200_w4_scratch_bytes(...) bytes, contents irrelevant, not shared with a launch that may run at the same time.  status: a device
+ * ceil(K / group) of them.  group: 32, 64 or 128; K a multiple of 32, up to 2^30 where M is above 16 (above 8 in groups of 128), 2^31 - 1056 otherwise; M and N
+ * any.  f32 sums.  scratch: 256-byte aligned, ib200_w4_scratch_bytes(...) bytes, contents irrelevant, not shared with a launch that may run at the same time.  status: a device
  * int32, zero, as for ib200_gemm_bias_act. */
 typedef struct ib200_w4_args {
   const void* x;

@@ -846,10 +846,11 @@ template <int XK> int run_tc_rows(const W4Args& a, void* scratch, cudaStream_t s
 static bool through_tensor_memory(int64_t m, int64_t n, int64_t k, int64_t group) {
   return k > 0 && (m > 16 || (m > 8 && group == 128 && n * k >= (int64_t)1 << 26));
 }
+constexpr int64_t kTcMostK = (int64_t)1 << 30;  // the copies of x count bytes in 32 bits, two to a value
 
 // room for x as the MMA reads it
 size_t w4_scratch_bytes(int, int64_t m, int64_t n, int64_t k, int64_t group) {
-  if (m <= 0 || n <= 0 || k <= 0 || beyond_any_device(m, k) || beyond_any_device(n, k) || k > INT32_MAX - 1024 || !through_tensor_memory(m, n, k, group)) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || beyond_any_device(m, k) || beyond_any_device(n, k) || k > kTcMostK || !through_tensor_memory(m, n, k, group)) return 0;
   return (size_t)(padded(m, tc_columns(m)) * padded(k, kStageK) * 2);
 }
 
@@ -880,6 +881,7 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
   a.s_vec = groups % 8 == 0 && aligned16(scales);
   a.z_vec = zeros && groups % 8 == 0 && (reinterpret_cast<uintptr_t>(zeros) & 7) == 0;
   if (through_tensor_memory(m, n, k, group)) {
+    if (k > kTcMostK) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: more than 16 rows of x (8 in groups of 128) take K up to 2^30");
     if (!scratch || scratch_bytes < w4_scratch_bytes(x_dtype, m, n, k, group)) return fail(IB200_ERR_BUFFER, "w4_matmul: scratch is smaller than ib200_w4_scratch_bytes");
     if (x_dtype == IB200_BF16) return run_tc_rows<X_BF16>(a, scratch, s);
     if (x_dtype == IB200_F16) return run_tc_rows<X_F16>(a, scratch, s);

@@ -373,7 +373,7 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
     ``q`` is uint8 [N, K/2] with the even k of a byte in its low half, ``scales`` [N, ceil(K / group)] f32 / bf16 / f16, ``zeros``
     uint8 of that shape (default 8), 0 to 127: one above makes its row of weights, a column of the result, NaN.  ``x`` [.., K] is bf16 or f16, or float8_e4m3fn / int8 with ``x_scale`` f32 [.., 1] or
     [.., ceil(K / group)], as ``rmsnorm`` returns them.  ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.
-    K is a multiple of 32, the group 32, 64 or 128."""
+    K is a multiple of 32 (up to 2^30 for more than 16 rows, or 8 in groups of 128), the group 32, 64 or 128."""
     index = _first("x", x)
     if index != _current_device():
         with torch.cuda.device(index):

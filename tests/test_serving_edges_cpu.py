@@ -6,10 +6,22 @@ pytest.importorskip("torch")
 
 from intent_ir_b200 import _lib  # noqa: E402
 
-from .test_serving_cpu import _norm  # noqa: E402
+from .test_serving_cpu import _norm, _w4  # noqa: E402
 
 
 def test_rows_without_columns_need_room_for_their_scales():
     assert _norm(cols=0, group=0, scale=None) == _lib.ERR_INVALID
     assert _norm(cols=0, group=0, rows=1 << 41) == _lib.ERR_INVALID
     assert _norm(cols=0, group=32, scale=None) == _lib.OK and _norm(cols=0, group=0, out=_lib.BF16, scale=None) == _lib.OK  # no scales
+
+
+@pytest.mark.parametrize("m,group,xt", [(17, 32, _lib.BF16), (64, 64, _lib.F16), (9, 128, _lib.BF16), (200, 128, _lib.E4M3)])
+def test_a_k_whose_bytes_pass_32_bits_is_refused_where_x_is_copied_by_bytes(m, group, xt):
+    """2^30 + 32 values of 16 bits: a copy's coordinate would wrap, and the rest of the sum be lost."""
+    k = (1 << 30) + 32
+    held = dict(xg=1) if xt == _lib.E4M3 else {}
+    assert _w4(m=m, n=1, k=k, xs=k, group=group, xt=xt, **held) == _lib.ERR_UNSUPPORTED
+    assert "2^30" in _lib.last_error()
+    scratch = _lib.load().ib200_w4_scratch_bytes
+    assert scratch(xt, m, 1, k, group) == 0
+    assert scratch(xt, 16, 1, 1 << 30, 128) == 16 * (1 << 30) * 2  # the last that is taken
