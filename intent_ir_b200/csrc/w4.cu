@@ -871,7 +871,7 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
   if (held != (xs_groups != 0) || (xs_groups != 0 && xs_groups != 1 && xs_groups != groups))
     return fail(IB200_ERR_INVALID, "w4_matmul: 8-bit x comes with one scale per row or one per row and group, other x with none");
   if (m == 0 || n == 0) return IB200_OK;
-  if (!y || (k > 0 && (!x || !q || !scales || (held && !xs)))) return fail(IB200_ERR_INVALID, "w4_matmul: null operand");
+  if (!y || (xs_groups && !xs) || (k > 0 && (!x || !q || !scales))) return fail(IB200_ERR_INVALID, "w4_matmul: null operand");
   if (!aligned16(q)) return fail(IB200_ERR_INVALID, "w4_matmul: q must be 16-byte aligned");
   if (m > 1 && (x_stride < k || beyond_any_device(m, x_stride > 0 ? x_stride : 1))) return fail(IB200_ERR_INVALID, "w4_matmul: bad row stride of x");
   const int e = held ? 1 : 2;

@@ -25,3 +25,10 @@ def test_a_k_whose_bytes_pass_32_bits_is_refused_where_x_is_copied_by_bytes(m, g
     scratch = _lib.load().ib200_w4_scratch_bytes
     assert scratch(xt, m, 1, k, group) == 0
     assert scratch(xt, 16, 1, 1 << 30, 128) == 16 * (1 << 30) * 2  # the last that is taken
+
+
+@pytest.mark.parametrize("m", [1, 12, 40])
+@pytest.mark.parametrize("xt", [_lib.E4M3, _lib.I8])
+def test_scales_of_x_are_needed_without_columns_too(m, xt):
+    """K = 0: the result is still multiplied by the row's scale on its way out."""
+    assert _w4(m=m, k=0, xt=xt, xg=1, xsc=None) == _lib.ERR_INVALID
