@@ -868,7 +868,7 @@ int launch_w4(const void* x, int64_t x_stride, const float* xs, int64_t xs_group
   if (group != 32 && group != 64 && group != 128) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: groups of 32, 64 or 128");
   if (k % 32) return fail(IB200_ERR_UNSUPPORTED, "w4_matmul: K must be a multiple of 32");
   const int64_t groups = (k + group - 1) / group;
-  if (held != (xs_groups != 0) || (xs_groups != 0 && xs_groups != 1 && xs_groups != groups))
+  if ((held ? xs_groups == 0 && groups != 0 : xs_groups != 0) || (xs_groups != 0 && xs_groups != 1 && xs_groups != groups))
     return fail(IB200_ERR_INVALID, "w4_matmul: 8-bit x comes with one scale per row or one per row and group, other x with none");
   if (m == 0 || n == 0) return IB200_OK;
   if (!y || (xs_groups && !xs) || (k > 0 && (!x || !q || !scales))) return fail(IB200_ERR_INVALID, "w4_matmul: null operand");

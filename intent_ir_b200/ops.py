@@ -406,7 +406,7 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
         if x_scale is not None:
             raise B200RuntimeError("w4_matmul: x_scale belongs to 8-bit x")
     if out_dtype is None:
-        out_dtype = torch.bfloat16 if x_groups else x.dtype
+        out_dtype = torch.bfloat16 if x.dtype in _HELD_CODE else x.dtype
     elif out_dtype not in _FLOAT_CODE:
         raise B200LoweringError(f"w4_matmul: the result is float32, bfloat16 or float16, not {out_dtype}")
     y = _dense_empty(front + (n,), out_dtype, x.device)

@@ -43,6 +43,15 @@ def test_w4_every_zero_point_and_nibble(ops, m, dtype, group):
         assert torch.isnan(got[:, 128:]).all()
 
 
+@pytest.mark.parametrize("x_groups", [0, 1])
+def test_w4_no_columns_of_eight_bits(ops, x_groups):
+    """K = 0: the bias alone, whether x_scale has a column for each row or one for each of no groups."""
+    bias = torch.randn(7, device="cuda", dtype=BF16)
+    got = ops.w4_matmul(torch.empty(3, 0, dtype=I8, device="cuda"), torch.empty(7, 0, dtype=torch.uint8, device="cuda"),
+                        torch.empty(7, 0, dtype=BF16, device="cuda"), bias=bias, x_scale=torch.ones(3, x_groups, device="cuda"))
+    assert got.dtype == BF16 and torch.equal(got, bias.expand(3, 7))
+
+
 # ---- rms-norm ---------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,cols", [(3, 64), (5, 1000), (2, 2501), (700, 256), (601, 1537), (3, 8192), (2, 16384), (2, 40000), (3, 3002)])
