@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
   constexpr int kStages = S::kStages;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[kStages], empty[kStages];
-  __shared__ volatile int dead;  // a wait ran out: nothing waits any more
+  __shared__ volatile int dead, brought;  // dead: a wait ran out, nothing waits any more; brought: stages in all
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, wr = warp & 3, wk = (warp >> 2) & 1, pg = row_of<G>(g);
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kRows, m0 = blockIdx.y * NT * 8;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
   };
   if (threadIdx.x == 0) {
     dead = 0;
+    brought = s1 - s0;
     for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 8);
     mbarrier_init_fence();
   }
@@ -280,8 +281,6 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
         asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(&full[i])) : "memory");
       }
     }
-    if (dead)  // copies that are still on their way land before the CTA ends
-      for (int s = max(s0, s1 - kStages); s < s1; ++s) (void)mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
   } else {
   // this thread's rows: 32 * wr + pg, + 8, + 16, + 24.  A stage's groups lie in one block.
   const uint8_t* scales = smem + S::S_AT + (wr * 32 + pg) * kRowScales;
@@ -393,6 +392,10 @@ __global__ void __launch_bounds__(kThreads, 2) w4_stream_kernel(const W4Args a, 
 
   // ---- add up the cluster's slices and write --------------------------------------------------------------
   __syncthreads();
+  if (dead) {  // whichever warp gave up: copies that are still on their way land before their memory is used again or the CTA ends
+    bool landed = true;
+    for (int n = brought, s = max(0, n - kStages); s < n; ++s) landed = landed && mbarrier_wait_bounded(&full[s % kStages], (s / kStages) & 1);
+  }
   float* box = reinterpret_cast<float*>(smem);  // [half of K][NT * 8][128] sums of this CTA
   constexpr int BOX = NT * 8 * kRows;
   if (warp < 8)
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ uint64_t full[kStages], empty[kStages], a_full[2][NA], d_full[2][ND];
   __shared__ uint32_t tmem_slot;
-  __shared__ volatile int dead;  // a wait ran out: nothing waits any more
+  __shared__ volatile int dead, brought;  // dead: a wait ran out, nothing waits any more; brought: stages in all
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (known to be the same for a warp)
   const int split = a.split, rank = blockIdx.x % split, n0 = (blockIdx.x / split) * kTcRows, m0 = blockIdx.y * NX;
   const int stages = (a.k + kStageK - 1) / kStageK, s0 = (int)((int64_t)stages * rank / split), s1 = (int)((int64_t)stages * (rank + 1) / split);
@@ -589,6 +592,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   auto arrive = [](uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory"); };
   if (threadIdx.x == 0) {
     dead = 0;
+    brought = s1 - s0;
     for (int i = 0; i < kStages; ++i) mbarrier_init(&full[i], 1 + 32), mbarrier_init(&empty[i], 16 + 2);
     for (int b = 0; b < 2; ++b) {
       for (int i = 0; i < NA; ++i) mbarrier_init(&a_full[b][i], 8);
@@ -634,8 +638,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
       }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&full[i])) : "memory");
     }
-    if (dead)  // copies that are still on their way land before the CTA ends
-      for (int s = max(s0, s1 - kStages); s < s1; ++s) (void)mbarrier_wait_bounded(&full[(s - s0) % kStages], ((s - s0) / kStages) & 1);
   } else if (warp >= 17) {
     // ---- the MMA warps, one for each block of rows.  All lanes walk the loop, so that its values stay in uniform registers, and one issues: moved there
     // from one thread's registers they took 100 cycles an MMA, three times its own time.
@@ -773,6 +775,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) w4_tc_kernel(const W4Args a, co
   // ---- add up the cluster's slices and write ----------------------------------------------------------------
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (dead) {  // whichever warp gave up: copies and products that are still on their way end before their memory is used again or freed
+    bool ended = true;
+    const int n = brought, chunks = n * GROUPS;
+    for (int s = max(0, n - kStages); s < n; ++s) ended = ended && mbarrier_wait_bounded(&full[s % kStages], (s / kStages) & 1);
+    for (int b = 0; b < 2; ++b)
+      for (int i = max(0, chunks - ND); i < chunks; ++i) ended = ended && mbarrier_wait_bounded(&d_full[b][i % ND], (i / ND) & 1);
+  }
   if (warp == 17) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
