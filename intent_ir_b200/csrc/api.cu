@@ -3,6 +3,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "guard.h"
 #include "kv8.h"
 
 namespace ib200 {
@@ -24,14 +25,7 @@ int cuda_fail(cudaError_t err, const char* what) {
 using namespace ib200;
 
 static int code(int64_t v) { return v >= 0 && v < 256 ? (int)v : -1; }
-// no exception (an allocation that failed, for a message or a map) leaves a C entry
-template <typename F> static int guarded(F f) noexcept {
-  try {
-    return f();
-  } catch (...) {
-    return IB200_ERR_CUDA;
-  }
-}
+template <typename F> static int guarded(F f) noexcept { return guarded(g_last_error, IB200_ERR_CUDA, f); }
 
 extern "C" {
 

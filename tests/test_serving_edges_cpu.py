@@ -1,5 +1,9 @@
 """What the serving entries refuse at the ends of their ranges, on a machine without a device."""
 
+import os
+import shutil
+import subprocess
+
 import pytest
 
 pytest.importorskip("torch")
@@ -32,3 +36,27 @@ def test_a_k_whose_bytes_pass_32_bits_is_refused_where_x_is_copied_by_bytes(m, g
 def test_scales_of_x_are_needed_without_columns_too(m, xt):
     """K = 0: the result is still multiplied by the row's scale on its way out."""
     assert _w4(m=m, k=0, xt=xt, xg=1, xsc=None) == _lib.ERR_INVALID
+
+
+GUARD = """
+#include <cstdio>
+#include <new>
+#include <stdexcept>
+#include "guard.h"
+int main() {
+  std::string message = "an older failure";
+  if (ib200::guarded(message, -3, [] { return 7; }) != 7 || message != "an older failure") return 1;
+  if (ib200::guarded(message, -3, []() -> int { throw std::runtime_error("no room"); }) != -3 || message != "exception: no room") return 2;
+  if (ib200::guarded(message, -3, []() -> int { throw std::bad_alloc(); }) != -3 || message != "exception: std::bad_alloc") return 3;
+  if (ib200::guarded(message, -3, []() -> int { throw 5; }) != -3 || message != "unknown exception") return 4;
+  puts("guarded");
+}
+"""
+
+
+@pytest.mark.skipif(not shutil.which("g++"), reason="needs a C++ compiler")
+def test_an_exception_at_a_c_entry_is_an_error_with_a_message_of_its_own(tmp_path):
+    (tmp_path / "guard.cpp").write_text(GUARD)
+    csrc = os.path.join(os.path.dirname(_lib.HERE), "intent_ir_b200", "csrc")
+    subprocess.run(["g++", "-std=c++17", "-I", csrc, str(tmp_path / "guard.cpp"), "-o", str(tmp_path / "guard")], check=True)
+    assert subprocess.run([str(tmp_path / "guard")], capture_output=True, text=True, check=True).stdout == "guarded\n"
