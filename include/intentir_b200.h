@@ -270,6 +270,9 @@ IB200_API size_t ib200_gemm_scratch_bytes(int in_dtype, int out_dtype, int64_t m
  * non-zero word to IB200_ERR_DEVICE_WAIT.  With status == NULL it checks the library's own word,
  * which the direct normalisation entry points use for their bounded waits on staged rows. */
 IB200_API int ib200_check_status(const int32_t* status, void* stream);
+/* The library's own status word on the current device (what ib200_check_status(NULL, ..) reads), zero when the library is loaded; NULL
+ * where there is no device.  May be called during stream capture. */
+IB200_API int32_t* ib200_status_word(void);
 
 /* out[i, j] = x[j, i] for a dense [rows, cols] matrix of 2- or 4-byte elements.
  * Replaces the generated transpose2d kernel (intentir_to_cuda.py:1487-1550). */

@@ -70,6 +70,7 @@ SIGNATURES = {
     "ib200_gemm_bias_act_ws": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i64, _i64, _i64, _i, _i, _i, _vp, _sz, _vp, _vp]),
     "ib200_gemm_scratch_bytes": (_sz, [_i, _i, _i64, _i64, _i64, _i, _i]),
     "ib200_check_status": (_i, [_vp, _vp]),
+    "ib200_status_word": (_vp, []),
     "ib200_transpose2d": (_i, [_vp, _vp, _i, _i64, _i64, _vp]),
     "ib200_rmsnorm": (_i, [_cp, _vp]),
     "ib200_w4_matmul": (_i, [_cp, _vp]),

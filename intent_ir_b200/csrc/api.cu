@@ -139,6 +139,8 @@ int ib200_check_status(const int32_t* status, void* stream) {
   return IB200_OK;
 }
 
+int32_t* ib200_status_word(void) { return norm_default_status(); }
+
 int ib200_transpose2d(const void* x, void* out, int elem_bytes, int64_t rows, int64_t cols, void* stream) {
   return launch_transpose2d(x, out, elem_bytes, rows, cols, static_cast<cudaStream_t>(stream));
 }

@@ -67,8 +67,23 @@ _status: Dict[int, torch.Tensor] = {}
 def status_word() -> torch.Tensor:
     dev = torch.cuda.current_device()
     if dev not in _status:
-        _status[dev] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
+        if torch.cuda.is_current_stream_capturing():
+            # memory of the graph's own pool may be written by its other nodes, and a node that zeroes the word would wipe out what
+            # earlier replays reported: the library's built-in word is neither
+            _status[dev] = torch.as_tensor(_BuiltInWord(), device=f"cuda:{dev}")
+        else:
+            _status[dev] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{dev}")
     return _status[dev]
+
+
+class _BuiltInWord:
+    """The library's status word on the current device, as torch takes foreign device memory."""
+
+    def __init__(self) -> None:
+        at = _lib.load().ib200_status_word()
+        if not at:
+            raise B200RuntimeError("the library has no status word on this device")
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (at, False), "version": 2}
 
 
 def check_device_status() -> None:
@@ -372,7 +387,7 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
     """``x @ w.T + bias`` for weights of 4 bits, ``w[n, k] = scales[n, k // group] * (q[n, k] - zeros[n, k // group])``, with f32 sums.
     ``q`` is uint8 [N, K/2] with the even k of a byte in its low half, ``scales`` [N, ceil(K / group)] f32 / bf16 / f16, ``zeros``
     uint8 of that shape (default 8), 0 to 127: one above makes its row of weights, a column of the result, NaN.  ``x`` [.., K] is bf16 or f16, or float8_e4m3fn / int8 with ``x_scale`` f32 [.., 1] or
-    [.., ceil(K / group)], as ``rmsnorm`` returns them.  ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.
+    [.., ceil(K / group)], as ``rmsnorm`` returns them.  A wait inside the kernel that runs out is reported by ``check_device_status``.  ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.
     K is a multiple of 32 (up to 2^30 for more than 16 rows, or 8 in groups of 128), the group 32, 64 or 128."""
     index = _first("x", x)
     if index != _current_device():
@@ -424,13 +439,9 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
 
 
 def _status_address(index: int) -> int:
-    """The device's status word; none inside a capture that comes before any other call (its zeroing would become part of the graph)."""
+    """The status word of the current device, `index`."""
     word = _status.get(index)
-    if word is None:
-        if torch.cuda.is_current_stream_capturing():
-            return 0
-        word = status_word()
-    return word.data_ptr()
+    return (status_word() if word is None else word).data_ptr()
 
 
 @functools.lru_cache(maxsize=4096)

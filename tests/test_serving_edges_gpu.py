@@ -1,6 +1,10 @@
 """The serving operators where their inputs reach the ends of what the entries accept: zero points beyond four bits, scales that
 lie far apart, rows whose squares vanish in 32 bits, empty extents, non-finite rows, the status word under capture."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -241,3 +245,43 @@ def test_attention_of_f16_results_takes_its_numerators_in_two_parts(ops, held, h
         off = (got[t] - want).abs()
         bound = spread * (2.0**-22 + 2.0**-18 + (n / 16 + 8) * 2.0**-22) + want.abs() * ref.half_step(F16) + 2.0**-25
         assert (off <= bound).all(), (n, (off / bound).max())
+
+
+# ---- the status word --------------------------------------------------------------------------------
+
+FIRST_CALL = """
+import torch
+from intent_ir_b200 import ops
+torch.manual_seed(0)
+x, q, s = torch.randn(2, 256).to(torch.bfloat16).cuda(), torch.randint(0, 256, (64, 128), dtype=torch.uint8).cuda(), torch.ones(64, 2).cuda()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    gone = torch.full((1,), 7, dtype=torch.int32, device="cuda")
+    del gone  # its memory is the pool's again, and every replay writes it
+    y = ops.w4_matmul(x, q, s)
+    assert ops._status_address(0), "the captured product has no word to report to"
+word = ops._status[0]
+assert word.data_ptr() == ops._status_address(0)
+for _ in range(3):
+    graph.replay()
+ops.check_device_status()
+assert int(word) == 0
+want = ops.w4_matmul(x, q, s)
+assert torch.equal(y, want) and ops._status[0] is word
+word.fill_(8)  # as a wait that ran out would leave it
+graph.replay()  # which a replay does not wipe out
+try:
+    ops.check_device_status()
+except ops.B200RuntimeError as e:
+    assert "4-bit product" in str(e)
+else:
+    raise AssertionError("not reported")
+ops.check_device_status()
+print("reported")
+"""
+
+
+def test_a_capture_that_comes_first_has_a_status_word():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "reported" in done.stdout, done.stderr[-2000:]
