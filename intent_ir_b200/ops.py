@@ -275,8 +275,10 @@ _HALF_CODE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _HELD_CODE = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.I8}
 
 
-_current_device = torch._C._cuda_getDevice  # what torch.cuda.current_device asks, once CUDA is up; there is a CUDA tensor by then
-_stream_of = torch._C._cuda_getCurrentRawStream  # the handle of torch.cuda.current_stream(device)
+# what torch.cuda.current_device asks, once CUDA is up (there is a CUDA tensor by then), and the handle of torch.cuda.current_stream(device); a torch built
+# without CUDA has neither, nor a tensor that would get as far
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _on_device(index: int, **tensors: Optional[torch.Tensor]) -> None:

@@ -3,6 +3,7 @@
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 
@@ -60,3 +61,21 @@ def test_an_exception_at_a_c_entry_is_an_error_with_a_message_of_its_own(tmp_pat
     csrc = os.path.join(os.path.dirname(_lib.HERE), "intent_ir_b200", "csrc")
     subprocess.run(["g++", "-std=c++17", "-I", csrc, str(tmp_path / "guard.cpp"), "-o", str(tmp_path / "guard")], check=True)
     assert subprocess.run([str(tmp_path / "guard")], capture_output=True, text=True, check=True).stdout == "guarded\n"
+
+
+WITHOUT_CUDA = """
+import torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda")]:
+    delattr(torch._C, name)
+from intent_ir_b200 import ops
+from intent_ir_b200.errors import B200RuntimeError
+try:
+    ops.rmsnorm(torch.zeros(2, 64))
+except B200RuntimeError:
+    print("imported")
+"""
+
+
+def test_the_entries_import_where_torch_was_built_without_cuda():
+    done = subprocess.run([sys.executable, "-c", WITHOUT_CUDA], cwd=os.path.dirname(_lib.HERE), capture_output=True, text=True, timeout=300)
+    assert done.stdout == "imported\n", done.stderr[-2000:]
