@@ -47,6 +47,19 @@ def test_w4_every_zero_point_and_nibble(ops, m, dtype, group):
         assert torch.isnan(got[:, 128:]).all()
 
 
+@pytest.mark.parametrize("m", [3, 12, 20, 64])
+@pytest.mark.parametrize("n,k,group", [(100, 256, 64), (100, 256, 128), (70, 512, 32)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_w4_a_non_finite_value_reaches_its_whole_row_and_no_other(ops, m, n, k, group, dtype, bad):
+    """inf * (q - z) is infinite, or NaN where q = z, and so is every sum that it enters."""
+    d, out = _w4_case(m, n, k, dtype, group, True, True, 0, dtype)
+    d["x"][m // 2, k // 3] = bad
+    got = ops.w4_matmul(**{a: v.cuda() if isinstance(v, torch.Tensor) else v for a, v in d.items()}).cpu()
+    rest = torch.arange(m) != m // 2
+    assert not torch.isfinite(got[~rest]).any() and torch.isfinite(got[rest]).all()
+
+
 @pytest.mark.parametrize("x_groups", [0, 1])
 def test_w4_no_columns_of_eight_bits(ops, x_groups):
     """K = 0: the bias alone, whether x_scale has a column for each row or one for each of no groups."""
