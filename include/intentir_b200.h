@@ -290,9 +290,10 @@ IB200_API int ib200_transpose2d(const void* x, void* out, int elem_bytes, int64_
  * h = x + residual;  y = h / sqrt(mean(h^2) + eps) * w  over rows of `cols` elements, computed from the unrounded sum.
  * residual may be NULL (h = x); h (its rounded value, row stride h_stride) may be NULL, and may be the memory of x or
  * residual.  dtype (x, residual, h): IB200_F32, IB200_BF16 or IB200_F16; w (NULL: ones) has dtype or IB200_F32.  out_dtype:
- * dtype, or IB200_E4M3 / IB200_I8 with scale[rows, groups] (f32):  s = max|y| * (1/Q) over a group, y / s rounded to nearest even,
- * Q = 448 / 127.  group: 32, 64, 128 or 256 columns (the last one may be shorter), 0: the row.  A group of zeros (or below
- * 2^-119) holds zeros; one with a NaN or an infinity has a NaN or infinite scale and stands for NaN.  y is dense. */
+ * dtype, or IB200_E4M3 / IB200_I8 with scale[rows, groups] (f32):  s = max|y| * (1/Q) over a group, y * (Q / max|y|) rounded to nearest
+ * even, Q = 448 / 127 (the product is within 4 ulp of f32 of y / s: a value that close to the middle between two held ones may go
+ * to either).  group: 32, 64, 128 or 256 columns (the last one may be shorter), 0: the row.  A group of zeros (or below 2^-119) holds zeros; one with a NaN or an infinity has a NaN or infinite scale and stands for NaN.  y is dense.  The number of rows
+ * chooses the order of a row's sum, so a row's last bits may differ between calls of different shapes; the same call repeats itself exactly. */
 typedef struct ib200_rmsnorm_args {
   const void *x, *residual, *w;
   void *y, *h;
@@ -333,7 +334,7 @@ IB200_API size_t ib200_w4_scratch_bytes(int x_dtype, int64_t m, int64_t n, int64
  *
  * append: the block of a head gets the scale s' = max(s, max|new| * (1/Q)), s = 0 where the block begins with a new token; values held before are
  * rounded again to q * s / s' where s' > s, new ones to x / s' (nearest even).  Slots behind a sequence's end are left as they are.
- * No two sequences may append to one page in the same call. */
+ * No page may take new tokens twice in the same call, from two sequences or from two blocks of one. */
 typedef struct ib200_kv8_append_args {
   const void *k, *v; /* [tokens, heads, dim] */
   void *k_cache, *v_cache;
@@ -348,7 +349,9 @@ IB200_API int ib200_kv8_append(const ib200_kv8_append_args* args, void* stream);
 /* Attention of the new tokens over that cache (they are in it already): o[t, h] = sum_j softmax_j(scale * q[t, h] . k[j]) v[j] over the keys
  * j <= p of the token's sequence, p = lens - (new tokens) + its place among them, and j > p - window where window > 0; query heads
  * h * q_heads / heads .. share a key head.  o is dense and 8-byte aligned.  lse (f32 [tokens, q_heads], NULL: none) is the log of the softmax's
- * denominator.  A row without keys is 0 with lse -inf; one that needs a page outside the cache or a token outside the table is NaN.
+ * denominator.  The softmax's numerators times v's scales enter the product with v in f16: rounded once (2^-12 of each) for bf16 results, in two
+ * parts (2^-22) for f16 ones, relative to the row's own largest; sums are f32.  A row without keys is 0 with lse -inf; one that
+ * needs a page outside the cache or a token outside the table is NaN.
  * scratch: 256-byte aligned, ib200_attention_kv8_scratch_bytes(...) bytes, contents irrelevant, not shared with a launch that may
  * run at the same time. */
 typedef struct ib200_attention_kv8_args {

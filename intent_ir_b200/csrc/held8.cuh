@@ -7,7 +7,7 @@
 
 namespace ib200 {
 
-enum : int { HELD_NONE = 0, HELD_E4M3 = 1, HELD_I8 = 2 };
+enum : int { HELD_E4M3 = 1, HELD_I8 = 2 };
 
 #ifdef __CUDACC__
 template <int HELD> __device__ __forceinline__ constexpr float held_top() { return HELD == HELD_E4M3 ? 448.0f : 127.0f; }

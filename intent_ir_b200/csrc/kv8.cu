@@ -17,7 +17,7 @@ namespace {
 //   s' = max(s, max|new| * (1 / Q)), s = 0 for a block that begins here; held values become round(q * s / s') where s' > s, new ones round(x / s')
 // Quotients round as IEEE divisions do: the held values depend on nothing but their definition.  The new values are read once
 // into registers (up to KEEP vectors of 8 a thread: 16 tokens of 128 in a warp, 64 in a CTA; more are read again) and written 8 bytes at a time.
-// Bound by instruction issue (two thirds of the slots) and the chain length -> table -> scale in front of each CTA: 30 000 tokens of 8 heads of 128,
+// Bound by instruction issue (77 % of the slots) and the chain length -> table -> scale in front of each CTA: 30 000 tokens of 8 heads of 128,
 // f16 -> int8, blocks of 64, take 46 us (4.1 TB/s) where the bytes alone would take 29; 128 sequences x 1 token 3.3 us.  One CTA for keys and values
 // saves a chain (57 -> 52 us; a warp that did both would take 4.2 instead of 3.3); 64 registers a thread let four CTAs share an SM (52 -> 46; five spill: 62).
 template <typename T> __device__ __forceinline__ uint4 read_new(const T* p, bool vec) {

@@ -17,10 +17,11 @@
 // or 2^-35 of the largest.  A key that a row does not see or give weight to does not enter that, whatever scale its page has; one whose weight is below
 // 2^-112 of the row's largest may count for less than its scale would make of it.
 //
-// With 8 rows to a unit HBM bounds it: 64 sequences of up to 8193 keys, 32 / 8 heads of 128, e4m3, 93 us (5.8 TB/s, 0.89 of a copy's rate); 2 of 131 073 keys,
-// 64 / 8 heads, 69 us (5.4 TB/s).  With more rows the instructions around the products do (39 to 45 % of the issue slots, the rest waits on their chains): 16 x 5
-// new tokens over 15 000 keys 82 us (3.3 TB/s, 133 TFLOP/s).  Short work is a chain of latencies: 702 keys 7.0 us, 33 x up to 5 new tokens in a window of 2048 20.6 us.
-// One power for all rows instead, led by every page's scale, would take 64 sequences in 92 us, 16 x 5 new tokens in 81; it lost a window's keys to a page in front of it.
+// With 8 rows to a unit HBM bounds it: 64 sequences of up to 8193 keys, 32 / 8 heads of 128, e4m3, 94 us (5.7 TB/s, 0.87 of a copy's rate); 2 of 131 073 keys,
+// 64 / 8 heads, 69 us (5.4 TB/s).  With more rows no unit is full: 16 x 5 new tokens over 15 000 keys 83 us (3.3 TB/s, 131 TFLOP/s) with 42 % of the issue slots and a third
+// of the tensor cycles taken, by eight warps to an SM that wait on fixed latencies, each step a chain of product, maximum, exponential, transpose, product.  6 x 512 new
+// tokens over 4608 keys 856 us (256 TFLOP/s).  Short work is a chain of latencies: 702 keys 7.0 us, 33 x up to 5 new tokens in a window of 2048 21.4 us.
+// One power for all rows instead, led by every page's scale, took 64 sequences in 92 us, 16 x 5 new tokens in 81; a page in front of a window cost the window's keys their bits.
 // A third stage of copies changed nothing at a width of 64 (20.8 / 20.7 us; 64 sequences 58.0 / 55.9).
 #include <algorithm>
 #include <atomic>
@@ -34,7 +35,8 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32, kStep = 32, kTile = kWarps * kStep, kStages = 2;
 // What beginning a unit costs, in tiles: tables, pages and queries are fetched one after the other and the warps' results joined.
-// 64 sequences of up to 8193 tokens: 115 us with 0, 106 with 1, 98 with 2, 95 with 4, 96 with 6.
+// 64 sequences of up to 8193 tokens: 113 us with 0, 97 with 2, 94 with 4, 95 with 6; 16 x 5 new tokens over 15 000 keys 108, 92, 83, 79; 33 x up to 5 in a window of
+// 2048 24.2, 20.3, 21.4, 22.2.
 constexpr int kStart = 4;
 constexpr float kNone = -3.402823466e38f;  // a row's maxima before its first key: finite, so that differences of two are numbers
 constexpr float kUp = 14.0f;               // a row's numerators p * vs are raised to at most 2^kUp
@@ -141,7 +143,8 @@ template <typename T, int HELD, int D, int NT, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? Cfg<D>::kCtas : Cfg<D>::kCtas - 1) attention_kernel(const Kv8Attention a, const Scratch sc, const Divisors by, const int q_vec) {
   using C = Cfg<D>;
   constexpr int ROWS = 8 * NT, HALVES = D / 64, MT = D / 16, CH = D / 16;  // CH: 16-byte chunks of a token
-  // An f16 result is off by 2^-12 of itself, no more than p rounded to f16 once: there p is multiplied in two parts.  (bf16's 2^-9 hides it.)
+  // An f16 result is off by 2^-12 of itself, no more than p rounded to f16 once: there p is multiplied in two parts.  (bf16's 2^-9 hides it; two parts
+  // there would take 16 x 5 new tokens over 15 000 keys from 83 to 94 us, as f16 has it.)
   constexpr bool kTwice = std::is_same<T, __half>::value;
   static_assert((kWarps + (CLUSTER ? 1 : 0)) * ROWS * C::kPitch * 4 <= C::kSmem, "the warps' results, and a cluster's piece, where the stages were");
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -728,9 +731,9 @@ int64_t most_ctas(int64_t dim, int nt) { return (int64_t)kSmCount * ((dim == 128
 
 // Rows of a unit, in eights: one where 8 rows suffice, two or three where a sequence has more (several new tokens, many heads to a group) so
 // that its keys are read and widened less often.  A unit of three takes 1.36 to 1.6 times a unit of two: 16 x 15 000 keys of 128 for 20 rows (one unit or
-// two) 82 / 102 us, 40 rows (two or three) 137 / 151, chunks of up to 512 tokens 357 / 388, but 33 x up to 8 tokens x 4 heads 36 / 34, and 11.3 / 10.4 us where
-// two sequences of 700 keys leave the GPU room for every tile of twice the units.  With offsets only the average number of new tokens is known here.
-// (Units of three spill up to 39 registers at D = 128 and f16, 7 in bf16.)
+// two) 84 / 104 us, 40 rows (two or three) 139 / 154, 6 x 512 tokens over 4608 keys 857 / 933, up to 512 with offsets 616 / 661, but 33 x up to 8 tokens x 4 heads of 64 27.6 / 24.8, and
+// 11.5 / 10.1 us where two sequences of 705 keys leave the GPU room for every tile of twice the units.  With offsets only the average number of new tokens is known here.
+// (Units of three spill up to 38 words at D = 128, 27 at 64.)
 int tiles_of_rows(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, bool uniform) {
   const int64_t rows = group * ((tokens + batch - 1) / batch), two = (rows + 15) / 16, three = (rows + 23) / 24;
   if (rows <= 8) return 1;
@@ -746,8 +749,8 @@ int64_t grid_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int
 }
 
 // CTAs of a cluster that takes a unit, 0 where the general form is to be used.  Its CTAs must all run at once and have at most eight tiles each, by the
-// room in the table.  Device time against the general form's: 1 sequence of 701 tokens 6.9 / 9.0 us, 1 of 8000 13.6 / 15.1, 16 of up to 3000 18.4 / 20.5, 48 of
-// up to 900 17.5 / 21.2, and 4.5 us less to enqueue; with sixteen tiles 2 of 16 000 take 22.4 / 19.2: longer ones gain from the even split of all tiles.
+// room in the table.  Device time against the general form's: 1 sequence of 701 tokens 7.0 / 9.1 us, 1 of 8000 13.4 / 14.9, 16 of up to 3000 18.6 / 21.0, 48 of
+// up to 900 17.3 / 21.5, and 4.5 us less to enqueue; with sixteen tiles 2 of 16 000 took 22.4 / 19.2: longer ones gain from the even split of all tiles.
 int cluster_of(int64_t tokens, int64_t batch, int64_t heads, int64_t group, int64_t dim, int64_t block, int64_t table_blocks, int nt, bool uniform) {
   if (!uniform) return 0;
   const int64_t units = batch * heads * ((tokens / batch * group + 8 * nt - 1) / (8 * nt)), tiles = (table_blocks * block + kTile - 1) / kTile;
@@ -787,8 +790,8 @@ template <typename T, int HELD, int D, int NT, bool CLUSTER> int run_attention(c
   }
   kern<<<grid, kThreads, Cfg<D>::kSmem, s>>>(a, sc, by, q_vec);
   if (cudaPeekAtLastError() != cudaSuccess) return cuda_fail(cudaGetLastError(), "attention_kv8 launch");
-  // few rows have many pieces each: a CTA for a row (2 sequences of 131 073 keys: 69.2 us in all, 73.5 with a warp); many rows have few: a warp (64 of up to
-  // 8193: 93.2, 94.4 with a CTA)
+  // few rows have many pieces each: a CTA for a row (2 sequences of 131 073 keys: 70.5 us in all, 74.7 with a warp); many rows have few: a warp (64 of up to
+  // 8193: 94.0, 95.3 with a CTA)
   const int64_t rows = a.tokens * a.q_heads;
   const bool many = rows > 4 * kSmCount;
   cfg.gridDim = dim3((unsigned)(many ? (rows + 3) / 4 : rows));

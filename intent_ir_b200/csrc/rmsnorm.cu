@@ -66,7 +66,8 @@ template <typename T> __device__ __forceinline__ float load_w(const RmsArgs& a, 
 __device__ __forceinline__ float top_inverse(int type) { return type == IB200_E4M3 ? held_unit<HELD_E4M3>() : held_unit<HELD_I8>(); }
 __device__ __forceinline__ float inverse_of(int type, float top) { return type == IB200_E4M3 ? held_inverse<HELD_E4M3>(top) : held_inverse<HELD_I8>(top); }
 
-// The same to 2 ulp without a division, for the scales of groups, of which there are many
+// The same to 2 ulp without a division, for the scales of groups, of which there are many: a value within 4 ulp of the middle between two held ones may go to
+// the other than a division would send it to.  The error against the unheld value is half a step either way.
 __device__ __forceinline__ float inverse_fast(int type, float top) {
   float r;
   asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(top));
@@ -79,9 +80,9 @@ __device__ __forceinline__ float inverse_fast(int type, float top) {
 // or 8 * THREADS apart (16-byte accesses).  Rows that do not begin on 16-byte boundaries are read element by
 // element, or two by two where 16-bit rows allow it; a warp then has 256 * NV adjacent columns, lane by lane (coalesced).  Either way the columns that share a scale
 // lie in one warp.
-// bf16 16384 x 8192 + residual -> e4m3 with scales of 128: 154 us (6.1 TB/s, 0.93 of a copy's rate); three passes over the row took 254, and divisions
-// instead of the approximate reciprocal for the scales of groups 180, bound by instruction issue.  f32 1021 x 5001, where no row is aligned:
-// 15.4 us (5.3 TB/s) lane by lane, 46.6 with eight adjacent columns to a thread.  16 x 4096: 3.0 us, one chain of load, two reductions and store.
+// bf16 16384 x 8192 + residual -> e4m3 with scales of 128: 155 us (6.1 TB/s, 0.93 of a copy's rate; 70 % of the issue slots); three passes over the row took 254, and
+// divisions instead of the approximate reciprocal for the scales of groups 180, bound by instruction issue.  f32 1021 x 5001, where no row is aligned:
+// 18.0 us (4.5 TB/s) lane by lane, 46.6 with eight adjacent columns to a thread.  16 x 4096: 3.0 us, one chain of load, two reductions and store.
 template <typename T> struct Raw { uint4 v[sizeof(T) / 2]; };  // 8 elements as they lie in memory
 template <typename T> __device__ __forceinline__ Raw<T> read8(const T* p) {
   Raw<T> r;

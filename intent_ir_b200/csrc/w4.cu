@@ -44,9 +44,10 @@ __device__ __forceinline__ float float_of(const void* p, int64_t i, int type) {
 // group; the group's sum is then scaled in f32.  A word gives pairs (0, 4), (1, 5), (2, 6), (3, 7), so x is laid down in that order, in
 // the order in which the warps read it.  128 + q in bf16 (1024 + q in f16) is q under the exponent of 128 (1024); minus 128 + z it is exact.
 // A ninth warp brings the weights and x as said; it and the others meet at mbarriers only.  The scales are read by the threads that use them.
-// 8192 x 8192 of groups of 128 and one row of bf16: 16.4 us (2.1 TB/s); 4096 x 4096: 6.6 us, of which two stages of loads and the cluster's sum are most; 7 x 5003 x 8192 in
-// groups of 32 with zero points, f16: 15.0 us.  Instruction issue and the waits between stages bound it, not HBM: eight weights cost nine instructions in front
-// of their products.  A ring filled by all warps took 24 us for the last, one warp to an output 161.
+// 8192 x 8192 of groups of 128 and one row of bf16: 15.2 us (2.3 TB/s); 4096 x 4096: 6.5 us, of which two stages of loads and the cluster's sum are most; 7 x 5003 x 8192 in
+// groups of 32 with zero points, f16: 15.5 us.  Waits bound it, not HBM: eight weights cost nine instructions in front of their products, but only 42 % of the issue slots
+// (36 % in the last case) are taken.  The warps stand at barriers longest (the scale blocks' and the cluster's), then on fixed latencies and in the pipeline's filling.
+// A ring filled by all warps took 24 us for the last case, one warp to an output 161.
 constexpr int kRows = 128, kThreads = 288, kStageK = 256, kRowBytes = kStageK / 2;
 enum : int { X_BF16 = 0, X_F16 = 1, X_E4M3 = 2, X_I8 = 3 };
 constexpr int kRowScales = 144;  // a row's two blocks of eight scales, then of eight zero points' patterns; 16 bytes keep rows in different banks
@@ -532,8 +533,9 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t at) {
 //   warp 16     brings the operands; x comes permuted and widened by a small launch in front, on which only x's copies wait
 //   warps 17-18 one thread each issues the MMAs of a block
 // Chunk i's widened weights arriving says that chunk i - 2 has been read back, so its buffers need no barrier of their own.
-// 64 x 16384 x 8192, e4m3, groups of 128: 34.8 us (494 TFLOP/s; the weights' bytes alone 11 us).  Issue of the widening's instructions bounds it (55 % of the slots; the tensor
-// cores are busy 15 % of the time).  On mma.sync the same product took 110 us; with eight widening warps 43, with scales fetched when they were needed 58.
+// 64 x 16384 x 8192, e4m3, groups of 128: 35.1 us (490 TFLOP/s; the weights' bytes alone 11 us).  The widening is most of it: its instructions take 56 % of the issue slots, the tensor
+// cores are busy 27 % of the time, and 128 CTAs leave 20 of 148 SMs without work.  512 rows widen all weights eight times: 233 us (590 TFLOP/s).
+// On mma.sync the product of 64 rows took 110 us; with eight widening warps 43, with scales fetched when they were needed 58.
 constexpr int kTcRowScales = 100;  // a row's two blocks of eight scales, then of eight zero points' patterns; 25 words, so that rows lie in different banks
 constexpr int kTcRows = 256, kTcThreads = 608;
 template <int NX, int G> struct TcStage {
@@ -849,9 +851,12 @@ template <int XK> int run_tc_rows(const W4Args& a, void* scratch, cudaStream_t s
 
 }  // namespace
 
-// Which kernel: up to 8 rows of x the weights stream into mma.sync (8192 x 8192, groups of 128, bf16: 16.4 us against 16.7 through tensor memory, and
-// 4096 x 4096 7.2 against 9.9), above 16 they go through tensor memory.  Between, mma.sync takes two column tiles: 10.2 against 10.4 us at 4096 x 4096, but 22.7
-// against 17.2 at 8192 x 8192, and 11.2 against 16.7 with groups of 32, whose sums come back four times as often.
+// Which kernel: up to 8 rows of x the weights stream into mma.sync (bf16, groups of 128: one row of 8192 x 8192 14.8 us against 16.6 through tensor memory, 4096 x 4096 6.4 against
+// 9.8; eight rows 16.2 / 17.1 and 7.0 / 10.2), above 16 they go through tensor memory.  Between, mma.sync takes two column tiles; 12 and 16 rows of square matrices:
+//   groups of 128: 4096 8.8 / 10.4 and 9.1 / 11.1 us, 5760 12.8 / 13.3 and 13.9 / 13.4, 8192 20.5 / 17.6 and 21.0 / 17.5
+//   groups of 64:  4096 9.2 / 11.3 and 9.7 / 12.0 us, 5760 14.6 / 15.4 and 15.9 / 15.7, 8192 22.5 / 20.3 and 22.9 / 20.4 (streamed: a rule for them would gain 10 % there)
+//   groups of 32, whose sums come back four times as often: 4096 10.3 / 14.1 us, 8192 25.8 / 28.5
+// The sides meet between 2^25 and 2^26 weights; 2^26 is the first size measured where tensor memory wins for 12 rows and 16 alike.
 static bool through_tensor_memory(int64_t m, int64_t n, int64_t k, int64_t group) {
   return k > 0 && (m > 16 || (m > 8 && group == 128 && n * k >= (int64_t)1 << 26));
 }

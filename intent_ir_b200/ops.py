@@ -336,8 +336,9 @@ def rmsnorm(x: torch.Tensor, w: Optional[torch.Tensor] = None, residual: Optiona
     """``h = x + residual`` and ``y = h / sqrt(mean(h * h) + eps) * w`` over the last axis, in f32 from the unrounded sum; returns
     ``(y, scale, h)``.  ``h`` has the type of ``x`` and is None without a residual; ``residual_out`` says where it goes (it may be
     ``residual`` or ``x`` itself).  ``out_dtype`` float8_e4m3fn or int8 holds y in 8 bits, ``y * scale`` standing for the result,
-    with one f32 scale for each row (``group`` 0) or for each 32, 64, 128 or 256 columns; otherwise y has the type of x and
-    scale is None.  x is f32, bf16 or f16; w has its type or f32; x, residual and residual_out may be matrices of spaced rows."""
+    with one f32 scale for each row (``group`` 0) or for each 32, 64, 128 or 256 columns (``max|y| / Q``; y times ``Q / max|y|``, in f32, is
+    rounded to nearest); otherwise y has the type of x and scale is None.  x is f32, bf16 or f16; w has its type or f32; x, residual and
+    residual_out may be matrices of spaced rows.  A row's last bits may differ between calls of different shapes."""
     index = _first("x", x)
     if index != _current_device():
         with torch.cuda.device(index):
@@ -388,9 +389,10 @@ def w4_matmul(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: Opt
               out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x @ w.T + bias`` for weights of 4 bits, ``w[n, k] = scales[n, k // group] * (q[n, k] - zeros[n, k // group])``, with f32 sums.
     ``q`` is uint8 [N, K/2] with the even k of a byte in its low half, ``scales`` [N, ceil(K / group)] f32 / bf16 / f16, ``zeros``
-    uint8 of that shape (default 8), 0 to 127: one above makes its row of weights, a column of the result, NaN.  ``x`` [.., K] is bf16 or f16, or float8_e4m3fn / int8 with ``x_scale`` f32 [.., 1] or
-    [.., ceil(K / group)], as ``rmsnorm`` returns them.  A wait inside the kernel that runs out is reported by ``check_device_status``.  ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.
-    K is a multiple of 32 (up to 2^30 for more than 16 rows, or 8 in groups of 128), the group 32, 64 or 128."""
+    uint8 of that shape (default 8), 0 to 127: one above makes its row of weights, a column of the result, NaN.  ``x`` [.., K] is
+    bf16 or f16, or float8_e4m3fn / int8 with ``x_scale`` f32 [.., 1] or [.., ceil(K / group)], as ``rmsnorm`` returns them.
+    ``out_dtype`` (default: the type of x, bf16 for 8-bit x) is also the bias's.  K is a multiple of 32 (up to 2^30 for more than 16
+    rows, or 8 in groups of 128), the group 32, 64 or 128.  A wait inside the kernel that runs out is reported by ``check_device_status``."""
     index = _first("x", x)
     if index != _current_device():
         with torch.cuda.device(index):
@@ -503,7 +505,8 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache:
     [pages, heads].  ``block_table`` [sequences, blocks] int32 names the pages, ``seq_lens`` [sequences] int32 the lengths with the
     new tokens, ``cu_new`` [sequences + 1] int32 where each sequence's new tokens lie (None: the same number for each).  A scale
     grows with its block's largest value, and the values held before are rounded again; slots behind the end, tokens behind
-    ``cu_new[-1]``, and pages or tokens outside the cache and the table are left alone.  No two sequences may append to one page."""
+    ``cu_new[-1]``, and pages or tokens outside the cache and the table are left alone.  No page may take new tokens twice in a call, from two
+    sequences or two blocks of one."""
     index = _first("k", k)
     if index != _current_device():
         with torch.cuda.device(index):
@@ -529,8 +532,9 @@ def attention_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     and values into (same arguments): token i of a sequence's n new ones sees the keys up to its own place, seq_len - n + i, and
     with ``window`` > 0 only the last that many of them.  ``scale`` defaults to 1 / sqrt(dim); consecutive query heads share a key
     head.  Returns ``o`` of q's shape and dtype (``out``, if given), with ``return_lse`` also the f32 [tokens, query heads] logs of
-    the softmax's denominators.  Rows without keys are 0 (lse -inf); rows that need a page outside the cache or a token outside the
-    table are NaN; tokens behind ``cu_new[-1]`` are not written."""
+    the softmax's denominators.  The softmax's numerators are rounded to f16 once (2^-12) for bf16 results and held in two f16 parts for f16
+    ones, whatever scales the pages that a row does not see have; sums are f32.  Rows without keys are 0 (lse -inf); rows that need a
+    page outside the cache or a token outside the table are NaN; tokens behind ``cu_new[-1]`` are not written."""
     index = _first("q", q)
     if index != _current_device():
         with torch.cuda.device(index):

@@ -128,6 +128,36 @@ def test_rmsnorm_rows_without_columns_have_the_scale_zero(ops, out):
         assert scale.shape == (rows, 0)
 
 
+# ---- append: a block that fills token by token ------------------------------------------------------
+
+@pytest.mark.parametrize("held", [E4M3, I8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("block", [16, 64])
+def test_append_values_held_and_rounded_again_stay_near_what_was_appended(ops, held, dtype, block):
+    """Against the values themselves: a value is off by half a step when it is held and by half a step more for every growth of its block's scale
+    since, a step being the scale (int8), or 2^-3 of the value and at least 2^-9 of the scale (e4m3); 2^-20 of the value more for the 32-bit arithmetic."""
+    heads, dim, n = 2, 64, block + block // 2
+    d = _paged(80, [1], [n], heads, dim, block, dtype, held)
+    dev = _cuda(d)
+    x = {c: torch.randn(n, heads, dim, generator=_gen(i)).to(dtype) * torch.linspace(0.2, 3.0, n)[:, None, None].to(dtype) for i, c in enumerate("kv")}
+    off = {c: torch.zeros(n, heads, dim, dtype=torch.float64) for c in "kv"}
+    scales = {c: torch.zeros(heads, dtype=torch.float64) for c in "kv"}
+    for i in range(n):
+        ops.kv8_append(x["k"][i:i + 1].cuda(), x["v"][i:i + 1].cuda(), *(dev[c] for c in CACHE), dev["block_table"], torch.tensor([i + 1], dtype=torch.int32).cuda())
+        page, first = int(d["block_table"][0, i // block]), i // block * block
+        for c in "kv":
+            now = dev[c + "_scale"][page].cpu().double()
+            grew = (now != scales[c]) if i > first else torch.ones(heads, dtype=torch.bool)
+            for t in range(first, i + 1):
+                size = x[c][t].double().abs() + off[c][t]  # what is rounded
+                half = 0.5 * now[:, None] if held == I8 else torch.maximum(size * 2.0**-4, now[:, None] * 2.0**-10)
+                off[c][t] += torch.where((grew | (t == i))[:, None], half + size * 2.0**-20, torch.zeros(()))
+            scales[c] = now
+            got = dev[c + "_cache"][page].cpu().double() * now[:, None, None]
+            wrong = (got[:, :i + 1 - first].transpose(0, 1) - x[c][first:i + 1].double()).abs()
+            assert (wrong <= off[c][first:i + 1]).all(), (i, (wrong / off[c][first:i + 1]).max())
+
+
 # ---- attention: value scales that lie far apart -----------------------------------------------------
 
 def _tight_bound(q, d, scale, window):
