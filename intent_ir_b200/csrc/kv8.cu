@@ -203,7 +203,7 @@ int check_kv8(const char* what, int64_t pages, int64_t heads, int64_t block, int
   if (heads > 65535 || pages > INT32_MAX || tokens > INT32_MAX - 65536 || batch > INT32_MAX - 65536) return fail(IB200_ERR_UNSUPPORTED, w + ": extents are below 2^31 (heads: 2^16)");
   if (beyond_any_device(pages, heads, block * dim) || beyond_any_device(batch, table_blocks) || table_blocks * block > INT32_MAX)
     return fail(IB200_ERR_INVALID, w + ": extents beyond any device (or sequences of 2^31 tokens)");
-  if (!cu && batch > 0 && tokens % batch) return fail(IB200_ERR_INVALID, w + ": without offsets every sequence has the same number of new tokens");
+  if (!cu && (batch > 0 ? tokens % batch != 0 : tokens > 0)) return fail(IB200_ERR_INVALID, w + ": without offsets every sequence has the same number of new tokens");
   return IB200_OK;
 }
 

@@ -11,7 +11,7 @@ pytest.importorskip("torch")
 
 from intent_ir_b200 import _lib  # noqa: E402
 
-from .test_serving_cpu import _norm, _w4  # noqa: E402
+from .test_serving_cpu import P, _append, _attention, _norm, _w4  # noqa: E402
 
 
 def test_rows_without_columns_need_room_for_their_scales():
@@ -79,3 +79,9 @@ except B200RuntimeError:
 def test_the_entries_import_where_torch_was_built_without_cuda():
     done = subprocess.run([sys.executable, "-c", WITHOUT_CUDA], cwd=os.path.dirname(_lib.HERE), capture_output=True, text=True, timeout=300)
     assert done.stdout == "imported\n", done.stderr[-2000:]
+
+
+def test_tokens_of_no_sequence_are_refused():
+    """Without offsets the tokens are dealt out evenly: to no sequences none can be, and the result would be left unwritten."""
+    assert _append(batch=0) == _lib.ERR_INVALID and _attention(batch=0) == _lib.ERR_INVALID
+    assert _append(batch=0, cu=P) == _lib.OK and _attention(batch=0, cu=P) == _lib.OK  # all tokens lie behind the last sequence
